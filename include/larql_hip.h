@@ -522,6 +522,128 @@ int  larql_hip_moe_layer_forward(larql_hip_ctx *ctx, larql_hip_moe_layer *layer,
 int  larql_hip_dev_moe_layer_forward(larql_hip_ctx *ctx, larql_hip_moe_layer *layer, const float *router_in, const float *x,
                                      size_t tokens, float *out, uint32_t *experts, float *weights);
 
+/* ---- device tier: what a decoder layer does between its matrix products ------
+ * The residual stream with its norms, the rotation and the paged 8-bit key/value cache, and the attention that reads it:
+ * with the matvec and MoE entry points a layer's whole step stays on the device.  Only enqueued, like every device-tier
+ * call.  Formats of activations are LARQL_FMT_F32, LARQL_FMT_BF16 or LARQL_FMT_F16; results in 16 bits are rounded to
+ * nearest even (the framework's f32_to_bf16 truncates).  No counterpart on this path of the reference, whose attention
+ * substrate runs on the CPU (larql-compute/src/attention); norm_offset and eps as its MoE norms have them. */
+
+/* h' = h + residual_scale * gate . rms(b; post_weight);  n = rms(h'; pre_weight), with
+ * rms(x; w) = x / sqrt(mean(x^2) + eps) * (norm_offset + w), a row each: the norm behind a block, its gate, the residual
+ * and the norm before the next block in one pass.  Every part is optional: block NULL (h' = h), post_weight NULL (b as it
+ * is), gate NULL (1), residual_out NULL (h' not wanted), normed NULL (n not wanted), pre_weight NULL (weights of n all
+ * ones: norm_offset does not enter).  gate is f32 [hidden] for all rows (gate_stride 0) or one row for each.  n is taken
+ * from h' before h' is rounded to its format.  residual_out may be residual, and normed may be block; no other overlap.
+ * Strides are elements between rows, at least hidden.  hidden <= 32768 (else LARQL_UNSUPPORTED). */
+typedef struct {
+    size_t rows, hidden;
+    const void *block;
+    size_t block_stride;
+    int block_format;
+    int residual_format;           /* of residual and residual_out */
+    const void *residual;
+    size_t residual_stride;
+    void *residual_out;
+    size_t residual_out_stride;
+    void *normed;
+    size_t normed_stride;
+    int normed_format;
+    float residual_scale;
+    const float *gate;
+    size_t gate_stride;
+    const float *post_weight, *pre_weight;  /* [hidden] */
+    float norm_offset, eps;
+} larql_hip_residual_norm;
+int larql_hip_dev_residual_norm(larql_hip_ctx *ctx, const larql_hip_residual_norm *args);
+
+/* One layer's paged cache.  A block of page_tokens tokens of one head has one scale, a power of two 2^e with -40 <= e <= 60;
+ * an element is its e4m3 (OCP) code times the scale.  e is the smallest with max |x| <= 448 * 2^e over the tokens written to
+ * the block; while the block fills it only grows, and the codes that are there are rounded again for the larger scale
+ * (exact unless a code becomes subnormal).  A block that met a NaN, an infinity or a magnitude above 448 * 2^60 has the
+ * scale NaN, and every query that sees one of its tokens a NaN result; codes are always finite.  Value codes lie
+ * transposed, so that the attention's matrix instructions load them as they are.  page_tokens 16, 32, 64 or 128;
+ * head_dim a multiple of 32 up to 256; codes 16-byte aligned (else LARQL_REFUSED_SHAPE). */
+typedef struct {
+    uint8_t *k_codes;              /* [num_pages, kv_heads, page_tokens, head_dim] */
+    uint8_t *v_codes;              /* [num_pages, kv_heads, head_dim, page_tokens] */
+    float *k_scales, *v_scales;    /* [num_pages, kv_heads] */
+    size_t num_pages, kv_heads, head_dim, page_tokens;
+} larql_hip_kv_cache;
+/* The sequences of a step, in device memory, so that a recorded call follows them as they grow.  kv_len[s] counts the
+ * tokens of sequence s with the new ones; its new tokens are rows q_start[s] .. q_start[s+1] of the activations and the last
+ * ones of the sequence.  block_table[s] lists its pages; an entry outside [0, num_pages) is a hole: nothing is written
+ * there, and its tokens are masked.  A sequence whose rows do not fit (q_start falling, beyond `tokens`, or more than
+ * max_new_tokens of them) is left out, its rows untouched. */
+typedef struct {
+    const int32_t *kv_len;         /* [sequences] */
+    const int32_t *block_table;    /* [sequences, table_width] */
+    const int32_t *q_start;        /* [sequences + 1] */
+    size_t sequences, table_width;
+    size_t tokens;                 /* rows that the activations hold */
+    size_t max_new_tokens;         /* at least the longest sequence's new tokens */
+} larql_hip_kv_batch;
+
+/* Appends the new tokens: keys (rms norm per head with k_norm unless NULL, then rotation) and values into their blocks, and
+ * the queries, normed (q_norm) and rotated alike, to q_out (q NULL: none).  Channel pairs (i, i + rot_dim/2), or
+ * (2i, 2i+1) where `interleaved`, of the first rot_dim channels turn by position * inv_freq[i] (the angle is reduced in 64
+ * bits) and are scaled by rope_scale; rot_dim 0: no rotation.  Positions count from the sequence's first token.  Rows are
+ * [heads, head_dim], strides elements between tokens (k, v and q may be parts of one fused row); q_out may be q.
+ * Two sequences must not append to one page.  Appending the same tokens again changes nothing. */
+typedef struct {
+    int format;                    /* of q, k, v and q_out */
+    int interleaved;
+    size_t q_heads;
+    const void *q;
+    size_t q_stride;
+    void *q_out;
+    size_t q_out_stride;
+    const void *k;
+    size_t k_stride;
+    const void *v;
+    size_t v_stride;
+    const float *inv_freq;         /* [rot_dim / 2] */
+    size_t rot_dim;
+    float rope_scale;
+    float norm_offset, norm_eps;
+    const float *q_norm, *k_norm;  /* [head_dim], or NULL */
+} larql_hip_kv_append;
+int larql_hip_dev_kv_append(larql_hip_ctx *ctx, const larql_hip_kv_cache *cache, const larql_hip_kv_batch *batch,
+                            const larql_hip_kv_append *args);
+
+/* Attention of the new tokens over their sequences' pages: query head i reads key/value head i / (q_heads / kv_heads).
+ * x = scale * q.k, softcap * tanh(x / softcap) where softcap > 0; a query at position p sees keys <= p (`causal`) and
+ * > p - window (window > 0); `sinks` [q_heads] (or NULL) adds exp(sink) to the sum of the weights.  A query that sees
+ * nothing gives zeros.  Sums are f32; where `out` is f32 queries and weights enter the matrix instructions as f16 pairs
+ * (about 22 bits), otherwise as one f16 each.  Results may differ in their last bits with the batch around a sequence: long
+ * rows are split by the work that there is.  workspace: larql_hip_attention_workspace_bytes(...) of device memory, 16-byte
+ * aligned, not shared with a call that may run at the same time. */
+typedef struct {
+    const void *q;
+    size_t q_stride;
+    int q_format, out_format;
+    void *out;
+    size_t out_stride;
+    size_t q_heads;
+    size_t window;
+    int causal;
+    float scale, softcap;
+    const float *sinks;
+} larql_hip_attention;
+size_t larql_hip_attention_workspace_bytes(const larql_hip_kv_cache *cache, const larql_hip_kv_batch *batch,
+                                           const larql_hip_attention *args);
+int larql_hip_dev_attention(larql_hip_ctx *ctx, const larql_hip_kv_cache *cache, const larql_hip_kv_batch *batch,
+                            const larql_hip_attention *args, void *workspace, size_t workspace_bytes);
+
+/* The three as plans, so that a sequence records a layer's whole step (larql_hip_sequence_create): the arguments are taken
+ * by value, what they point to is read at every run.  Lengths, tables and activations may change between runs, within the
+ * batch's sizes. */
+int larql_hip_plan_create_residual_norm(larql_hip_ctx *ctx, const larql_hip_residual_norm *args, larql_hip_plan **out);
+int larql_hip_plan_create_kv_append(larql_hip_ctx *ctx, const larql_hip_kv_cache *cache, const larql_hip_kv_batch *batch,
+                                    const larql_hip_kv_append *args, larql_hip_plan **out);
+int larql_hip_plan_create_attention(larql_hip_ctx *ctx, const larql_hip_kv_cache *cache, const larql_hip_kv_batch *batch,
+                                    const larql_hip_attention *args, void *workspace, size_t workspace_bytes, larql_hip_plan **out);
+
 /* ---- device tier: encoders (bit-exact with the reference's host encoders) --- */
 /* quantize_q4_k — larql-compute/src/cpu/ops/q4_common/quantize.rs:89-189. */
 int larql_hip_dev_quantize_q4_k(larql_hip_ctx *ctx, const float *src, size_t n, uint8_t *dst);

@@ -54,6 +54,39 @@ class MatvecJob(C.Structure):
                 ("out", vp), ("rows", u64), ("k", u64)]
 
 
+class ResidualNorm(C.Structure):
+    """larql_hip_residual_norm: the residual between two blocks and the norms around it."""
+    _fields_ = [("rows", sz), ("hidden", sz), ("block", vp), ("block_stride", sz), ("block_format", ci), ("residual_format", ci),
+                ("residual", vp), ("residual_stride", sz), ("residual_out", vp), ("residual_out_stride", sz), ("normed", vp),
+                ("normed_stride", sz), ("normed_format", ci), ("residual_scale", C.c_float), ("gate", vp), ("gate_stride", sz),
+                ("post_weight", vp), ("pre_weight", vp), ("norm_offset", C.c_float), ("eps", C.c_float)]
+
+
+class KvCache(C.Structure):
+    """larql_hip_kv_cache: one layer's paged cache of e4m3 codes with a scale for each page and head."""
+    _fields_ = [("k_codes", vp), ("v_codes", vp), ("k_scales", vp), ("v_scales", vp), ("num_pages", sz), ("kv_heads", sz),
+                ("head_dim", sz), ("page_tokens", sz)]
+
+
+class KvBatch(C.Structure):
+    """larql_hip_kv_batch: the sequences of a step (lengths, pages, rows of the new tokens), in device memory."""
+    _fields_ = [("kv_len", vp), ("block_table", vp), ("q_start", vp), ("sequences", sz), ("table_width", sz), ("tokens", sz),
+                ("max_new_tokens", sz)]
+
+
+class KvAppend(C.Structure):
+    """larql_hip_kv_append: queries, keys and values of the new tokens, their norms and rotation."""
+    _fields_ = [("format", ci), ("interleaved", ci), ("q_heads", sz), ("q", vp), ("q_stride", sz), ("q_out", vp), ("q_out_stride", sz),
+                ("k", vp), ("k_stride", sz), ("v", vp), ("v_stride", sz), ("inv_freq", vp), ("rot_dim", sz), ("rope_scale", C.c_float),
+                ("norm_offset", C.c_float), ("norm_eps", C.c_float), ("q_norm", vp), ("k_norm", vp)]
+
+
+class Attention(C.Structure):
+    """larql_hip_attention: queries, results and masks of a step's attention."""
+    _fields_ = [("q", vp), ("q_stride", sz), ("q_format", ci), ("out_format", ci), ("out", vp), ("out_stride", sz), ("q_heads", sz),
+                ("window", sz), ("causal", ci), ("scale", C.c_float), ("softcap", C.c_float), ("sinks", vp)]
+
+
 # name -> (restype, argtypes): every symbol include/larql_hip.h declares
 SIGNATURES = {
     "larql_hip_create": (ci, [C.POINTER(vp), ci]),
@@ -132,6 +165,13 @@ SIGNATURES = {
     "larql_hip_moe_layer_destroy": (None, [vp, vp]),
     "larql_hip_moe_layer_forward": (ci, [vp, vp, vp, vp, sz, vp, vp, vp]),
     "larql_hip_dev_moe_layer_forward": (ci, [vp, vp, vp, vp, sz, vp, vp, vp]),
+    "larql_hip_dev_residual_norm": (ci, [vp, C.POINTER(ResidualNorm)]),
+    "larql_hip_dev_kv_append": (ci, [vp, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvAppend)]),
+    "larql_hip_attention_workspace_bytes": (sz, [C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(Attention)]),
+    "larql_hip_dev_attention": (ci, [vp, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(Attention), vp, sz]),
+    "larql_hip_plan_create_residual_norm": (ci, [vp, C.POINTER(ResidualNorm), C.POINTER(vp)]),
+    "larql_hip_plan_create_kv_append": (ci, [vp, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvAppend), C.POINTER(vp)]),
+    "larql_hip_plan_create_attention": (ci, [vp, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(Attention), vp, sz, C.POINTER(vp)]),
     "larql_hip_dev_quantize_q4_k": (ci, [vp, vp, sz, vp]),
     "larql_hip_dev_quantize_q6_k": (ci, [vp, vp, sz, vp]),
     "larql_hip_dev_quantize_q8_0": (ci, [vp, vp, sz, vp]),

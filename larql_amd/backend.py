@@ -559,6 +559,36 @@ class HipBackend:
     def dev_moe_layer_forward(self, layer: int, router_in: int, x: int, tokens: int, out: int, experts: int, weights: int) -> bool:
         return self._some(lib.larql_hip_dev_moe_layer_forward(self._h, layer, router_in, x, tokens, out, experts, weights))
 
+    # -- between a layer's matrix products: residual and norms, paged cache, attention ---------------------------
+    def dev_residual_norm(self, args: "L.ResidualNorm") -> bool:
+        return self._some(lib.larql_hip_dev_residual_norm(self._h, C.byref(args)))
+
+    def dev_kv_append(self, cache: "L.KvCache", batch: "L.KvBatch", args: "L.KvAppend") -> bool:
+        return self._some(lib.larql_hip_dev_kv_append(self._h, C.byref(cache), C.byref(batch), C.byref(args)))
+
+    def attention_workspace_bytes(self, cache: "L.KvCache", batch: "L.KvBatch", args: "L.Attention") -> int:
+        return lib.larql_hip_attention_workspace_bytes(C.byref(cache), C.byref(batch), C.byref(args))
+
+    def dev_attention(self, cache: "L.KvCache", batch: "L.KvBatch", args: "L.Attention", workspace: int, workspace_bytes: int) -> bool:
+        return self._some(lib.larql_hip_dev_attention(self._h, C.byref(cache), C.byref(batch), C.byref(args), workspace, workspace_bytes))
+
+    def plan_create_residual_norm(self, args: "L.ResidualNorm") -> Optional[int]:
+        """A plan like plan_create's, for sequence_create: a layer's step between its matvecs."""
+        p = C.c_void_p()
+        return p.value if self._some(lib.larql_hip_plan_create_residual_norm(self._h, C.byref(args), C.byref(p))) else None
+
+    def plan_create_kv_append(self, cache: "L.KvCache", batch: "L.KvBatch", args: "L.KvAppend") -> Optional[int]:
+        p = C.c_void_p()
+        ok = self._some(lib.larql_hip_plan_create_kv_append(self._h, C.byref(cache), C.byref(batch), C.byref(args), C.byref(p)))
+        return p.value if ok else None
+
+    def plan_create_attention(self, cache: "L.KvCache", batch: "L.KvBatch", args: "L.Attention", workspace: int,
+                              workspace_bytes: int) -> Optional[int]:
+        p = C.c_void_p()
+        ok = self._some(lib.larql_hip_plan_create_attention(self._h, C.byref(cache), C.byref(batch), C.byref(args), workspace,
+                                                            workspace_bytes, C.byref(p)))
+        return p.value if ok else None
+
     def dev_quantize_q4_k(self, src: int, n: int, dst: int) -> bool:
         return self._some(lib.larql_hip_dev_quantize_q4_k(self._h, src, n, dst))
 

@@ -5,6 +5,7 @@
 // the HIP kernels or refuses.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <chrono>
 #include <cmath>
 #include <cstdarg>
@@ -12,11 +13,13 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
 #include "../../include/larql_hip.h"
 #include "kernels.h"
+#include "layer.h"
 
 using namespace larql;
 
@@ -1558,9 +1561,40 @@ int larql_hip_dev_matvec_batch(larql_hip_ctx *c, const larql_hip_matvec_job *pj,
     return enqueue_jobs(c, jobs);
 }
 
-struct larql_hip_plan {
-    std::vector<PreparedLaunch> launches;
+// A call between a layer's matvecs, recorded by value.
+struct LayerCall {
+    enum Kind { NONE, NORM, APPEND, ATTENTION } kind = NONE;
+    union {
+        NormArgs norm;
+        KvAppendArgs append;
+        AttentionArgs attention;
+    };
+    void *workspace = nullptr;
+    LayerCall() {}
+    int launches() const { return kind == NONE ? 0 : kind == ATTENTION ? attention_launches(attention) : 1; }
+    hipError_t enqueue(hipStream_t s) const {
+        switch (kind) {
+        case NORM: return residual_norm_launch(s, norm);
+        case APPEND: return kv_append_launch(s, append);
+        case ATTENTION: return attention_launch(s, attention, workspace);
+        default: return hipSuccess;
+        }
+    }
 };
+
+struct larql_hip_plan {
+    std::vector<PreparedLaunch> launches;  // of matvecs, or
+    LayerCall layer;                       // one of these
+    int launch_count() const { return (int)launches.size() + layer.launches(); }
+};
+
+static hipError_t enqueue_plan(larql_hip_ctx *c, const larql_hip_plan *plan) {
+    for (const PreparedLaunch &P : plan->launches) {
+        const hipError_t e = gemv_launch(c->stream, P.kind, P.L, P.threads, P.grid, P.lds);
+        if (e != hipSuccess) return e;
+    }
+    return plan->layer.enqueue(c->stream);
+}
 
 int larql_hip_plan_create(larql_hip_ctx *c, const larql_hip_matvec_job *pj, size_t n_jobs, larql_hip_plan **out) {
     if (!c || !out || (!pj && n_jobs)) return LARQL_E_ARG;
@@ -1601,11 +1635,11 @@ int larql_hip_plan_run(larql_hip_ctx *c, larql_hip_plan *plan) {
     if (!c || !plan) return LARQL_E_ARG;
     std::lock_guard<std::mutex> lk(c->mu);
     HIPCHECK(c, hipSetDevice(c->device));
-    for (const PreparedLaunch &P : plan->launches) HIPCHECK(c, gemv_launch(c->stream, P.kind, P.L, P.threads, P.grid, P.lds));
+    HIPCHECK(c, enqueue_plan(c, plan));
     return LARQL_OK;
 }
 
-int larql_hip_plan_launch_count(const larql_hip_plan *plan) { return plan ? (int)plan->launches.size() : 0; }
+int larql_hip_plan_launch_count(const larql_hip_plan *plan) { return plan ? plan->launch_count() : 0; }
 
 struct larql_hip_sequence {
     hipGraph_t graph = nullptr;
@@ -1621,18 +1655,15 @@ int larql_hip_sequence_create(larql_hip_ctx *c, larql_hip_plan *const *plans, si
     std::lock_guard<std::mutex> lk(c->mu);
     HIPCHECK(c, hipSetDevice(c->device));
     // once eagerly: whatever a kernel's first launch sets up (its LDS limit) happens outside the recording
-    for (size_t i = 0; i < n_plans; i++)
-        for (const PreparedLaunch &P : plans[i]->launches) HIPCHECK(c, gemv_launch(c->stream, P.kind, P.L, P.threads, P.grid, P.lds));
+    for (size_t i = 0; i < n_plans; i++) HIPCHECK(c, enqueue_plan(c, plans[i]));
     HIPCHECK(c, wait_stream(c));
     larql_hip_sequence *seq = new larql_hip_sequence();
     hipError_t e = hipStreamBeginCapture(c->stream, hipStreamCaptureModeThreadLocal);
     if (e == hipSuccess) {
-        for (size_t i = 0; i < n_plans && e == hipSuccess; i++)
-            for (const PreparedLaunch &P : plans[i]->launches) {
-                e = gemv_launch(c->stream, P.kind, P.L, P.threads, P.grid, P.lds);
-                if (e != hipSuccess) break;
-                seq->launches++;
-            }
+        for (size_t i = 0; i < n_plans && e == hipSuccess; i++) {
+            e = enqueue_plan(c, plans[i]);
+            if (e == hipSuccess) seq->launches += plans[i]->launch_count();
+        }
         hipGraph_t g = nullptr;
         const hipError_t e2 = hipStreamEndCapture(c->stream, &g);  // (always ends the recording, also after a failed launch)
         seq->graph = g;
@@ -2522,6 +2553,238 @@ int larql_hip_dev_gate_walk(larql_hip_ctx *c, int format, const void *const *gat
                   score_out, count_out, c->nan_flag);
     if (rc) return rc;
     return LARQL_OK;
+}
+
+// ---- device tier: what a decoder layer does between its matrix products ---------------------------
+
+// An activation format of the layer operators; -1 for any other.
+static int elem_type(int format) {
+    return format == LARQL_FMT_F32 ? ELEM_F32 : format == LARQL_FMT_BF16 ? ELEM_BF16 : format == LARQL_FMT_F16 ? ELEM_F16 : -1;
+}
+
+static int check_residual_norm(larql_hip_ctx *c, const larql_hip_residual_norm *a, NormArgs &A) {
+    if (!a) return LARQL_E_ARG;
+    memset(&A, 0, sizeof A);
+    if (a->rows == 0 || a->hidden == 0) return LARQL_OK;
+    if (a->hidden > kNormMaxHidden || a->rows > 0x7FFFFFFFull) return fail(c, LARQL_UNSUPPORTED, "residual_norm: hidden above 32768");
+    A.residual_type = elem_type(a->residual_format);
+    A.block_type = a->block ? elem_type(a->block_format) : ELEM_F32;
+    A.normed_type = a->normed ? elem_type(a->normed_format) : ELEM_F32;
+    if (A.residual_type < 0 || A.block_type < 0 || A.normed_type < 0)
+        return fail(c, LARQL_UNSUPPORTED, "residual_norm: formats are f32, bf16 and f16");
+    if (!a->residual || (!a->residual_out && !a->normed)) return LARQL_E_ARG;
+    if (a->rows > 1 && ((a->block && a->block_stride < a->hidden) || a->residual_stride < a->hidden ||
+                        (a->residual_out && a->residual_out_stride < a->hidden) || (a->normed && a->normed_stride < a->hidden) ||
+                        (a->gate && a->gate_stride && a->gate_stride < a->hidden)))
+        return fail(c, LARQL_REFUSED_SHAPE, "residual_norm: a row stride below hidden");
+    A.block = a->block; A.residual = a->residual; A.residual_out = a->residual_out; A.normed = a->normed;
+    A.gate = a->block ? a->gate : nullptr;
+    A.post_weight = a->block ? a->post_weight : nullptr;
+    A.pre_weight = a->pre_weight;
+    A.block_stride = a->block_stride; A.residual_stride = a->residual_stride; A.residual_out_stride = a->residual_out_stride;
+    A.normed_stride = a->normed_stride; A.gate_stride = a->gate_stride;
+    A.rows = (uint32_t)a->rows; A.hidden = (uint32_t)a->hidden;
+    A.residual_scale = a->residual_scale; A.norm_offset = a->norm_offset; A.eps = a->eps;
+    const size_t es = elem_bytes(A.residual_type), eb = elem_bytes(A.block_type), en = elem_bytes(A.normed_type);
+    const auto whole = [&](const void *p, size_t stride, size_t item) { return !p || (((uintptr_t)p & 15) == 0 && stride * item % 16 == 0); };
+    const auto natural = [](const void *p, size_t item) { return ((uintptr_t)p & (item - 1)) == 0; };
+    if (!natural(A.block, eb) || !natural(A.residual, es) || !natural(A.residual_out, es) || !natural(A.normed, en) || !natural(A.gate, 4) ||
+        !natural(A.post_weight, 4) || !natural(A.pre_weight, 4))
+        return fail(c, LARQL_REFUSED_SHAPE, "residual_norm: an operand is not aligned to its elements");
+    const size_t several = a->rows > 1;  // (one row: its stride is not used)
+    A.vec = a->hidden % 8 == 0 && whole(A.block, several * A.block_stride, eb) && whole(A.residual, several * A.residual_stride, es) &&
+            whole(A.residual_out, several * A.residual_out_stride, es) && whole(A.normed, several * A.normed_stride, en) &&
+            whole(A.gate, several * A.gate_stride, 4) && whole(A.post_weight, 0, 4) && whole(A.pre_weight, 0, 4);
+    return LARQL_OK;
+}
+
+// The cache and the sequences, as the kernels take them; nothing to do where *empty.
+static int check_kv(larql_hip_ctx *c, const char *what, const larql_hip_kv_cache *k, const larql_hip_kv_batch *b, KvArgs &A, bool *empty) {
+    if (!k || !b) return LARQL_E_ARG;
+    memset(&A, 0, sizeof A);
+    if (k->head_dim == 0 || k->head_dim > 256 || k->head_dim % 32 != 0)
+        return fail(c, LARQL_REFUSED_SHAPE, "%s: head_dim is a multiple of 32 up to 256", what);
+    if (k->page_tokens != 16 && k->page_tokens != 32 && k->page_tokens != 64 && k->page_tokens != 128)
+        return fail(c, LARQL_REFUSED_SHAPE, "%s: page_tokens is 16, 32, 64 or 128", what);
+    if (k->kv_heads == 0 || k->kv_heads > 1024) return fail(c, LARQL_REFUSED_SHAPE, "%s: 1 to 1024 key/value heads", what);
+    *empty = b->sequences == 0 || b->tokens == 0 || b->max_new_tokens == 0;
+    if (*empty) return LARQL_OK;
+    if (k->num_pages == 0 || b->table_width == 0) return fail(c, LARQL_REFUSED_SHAPE, "%s: a cache without pages", what);
+    if (k->num_pages > 0x7FFFFFFFull || b->sequences > (1u << 20) || b->table_width > 0x7FFFFFFFull || b->tokens > (1u << 24))
+        return fail(c, LARQL_UNSUPPORTED, "%s: too large", what);
+    if (!k->k_codes || !k->v_codes || !k->k_scales || !k->v_scales || !b->kv_len || !b->block_table || !b->q_start) return LARQL_E_ARG;
+    if (((uintptr_t)k->k_codes | (uintptr_t)k->v_codes) & 15) return fail(c, LARQL_REFUSED_SHAPE, "%s: codes must be 16-byte aligned", what);
+    if (((uintptr_t)k->k_scales | (uintptr_t)k->v_scales | (uintptr_t)b->kv_len | (uintptr_t)b->block_table | (uintptr_t)b->q_start) & 3)
+        return fail(c, LARQL_REFUSED_SHAPE, "%s: scales and tables must be 4-byte aligned", what);
+    A.k_codes = k->k_codes; A.v_codes = k->v_codes; A.k_scales = k->k_scales; A.v_scales = k->v_scales;
+    A.kv_len = b->kv_len; A.block_table = b->block_table; A.q_start = b->q_start;
+    A.num_pages = (uint32_t)k->num_pages; A.kv_heads = (uint32_t)k->kv_heads; A.head_dim = (uint32_t)k->head_dim;
+    A.page_shift = (uint32_t)__builtin_ctzll(k->page_tokens);
+    A.sequences = (uint32_t)b->sequences; A.table_width = (uint32_t)b->table_width; A.tokens = (uint32_t)b->tokens;
+    A.max_new = (uint32_t)std::min(b->max_new_tokens, b->tokens);
+    return LARQL_OK;
+}
+// rows of whole heads: 16-byte aligned, with room for all heads
+static bool row_fits(const void *p, size_t stride, int type, size_t heads, size_t head_dim) {
+    return ((uintptr_t)p & 15) == 0 && stride * elem_bytes(type) % 16 == 0 && stride >= heads * head_dim;
+}
+
+static int check_kv_append(larql_hip_ctx *c, const larql_hip_kv_cache *k, const larql_hip_kv_batch *b, const larql_hip_kv_append *a, KvAppendArgs &A,
+                           bool *empty) {
+    if (!a) return LARQL_E_ARG;
+    memset(&A, 0, sizeof A);
+    int rc = check_kv(c, "kv_append", k, b, A.kv, empty);
+    if (rc || *empty) return rc;
+    A.type = elem_type(a->format);
+    if (A.type < 0) return fail(c, LARQL_UNSUPPORTED, "kv_append: formats are f32, bf16 and f16");
+    if (!a->k || !a->v || (a->rot_dim && !a->inv_freq)) return LARQL_E_ARG;
+    if (a->rot_dim > k->head_dim || a->rot_dim % 8 != 0) return fail(c, LARQL_REFUSED_SHAPE, "kv_append: rot_dim is a multiple of 8 up to head_dim");
+    const bool with_q = a->q && a->q_heads;
+    if (with_q && !a->q_out) return LARQL_E_ARG;
+    if (with_q && a->q_heads > 65535) return fail(c, LARQL_UNSUPPORTED, "kv_append: too many query heads");
+    if (!row_fits(a->k, a->k_stride, A.type, k->kv_heads, k->head_dim) || !row_fits(a->v, a->v_stride, A.type, k->kv_heads, k->head_dim) ||
+        (with_q && (!row_fits(a->q, a->q_stride, A.type, a->q_heads, k->head_dim) ||
+                    !row_fits(a->q_out, a->q_out_stride, A.type, a->q_heads, k->head_dim))))
+        return fail(c, LARQL_REFUSED_SHAPE, "kv_append: rows must be 16-byte aligned and hold all heads");
+    if (((uintptr_t)a->q_norm | (uintptr_t)a->k_norm) & 15) return fail(c, LARQL_REFUSED_SHAPE, "kv_append: norm weights must be 16-byte aligned");
+    if ((uintptr_t)a->inv_freq & 3) return fail(c, LARQL_REFUSED_SHAPE, "kv_append: inv_freq must be 4-byte aligned");
+    A.q = with_q ? a->q : nullptr; A.k = a->k; A.v = a->v; A.q_out = a->q_out;
+    A.q_stride = a->q_stride; A.q_out_stride = a->q_out_stride; A.k_stride = a->k_stride; A.v_stride = a->v_stride;
+    A.inv_freq = a->inv_freq; A.q_norm = a->q_norm; A.k_norm = a->k_norm;
+    A.q_heads = (uint32_t)a->q_heads; A.rot_dim = (uint32_t)a->rot_dim; A.interleaved = a->interleaved != 0;
+    A.rope_scale = a->rope_scale; A.norm_offset = a->norm_offset; A.norm_eps = a->norm_eps;
+    return LARQL_OK;
+}
+
+static int check_attention(larql_hip_ctx *c, const larql_hip_kv_cache *k, const larql_hip_kv_batch *b, const larql_hip_attention *a,
+                           AttentionArgs &A, bool *empty) {
+    if (!a) return LARQL_E_ARG;
+    memset(&A, 0, sizeof A);
+    int rc = check_kv(c, "attention", k, b, A.kv, empty);
+    if (rc || *empty) return rc;
+    A.q_type = elem_type(a->q_format); A.out_type = elem_type(a->out_format);
+    if (A.q_type < 0 || A.out_type < 0) return fail(c, LARQL_UNSUPPORTED, "attention: formats are f32, bf16 and f16");
+    if (a->q_heads == 0 || a->q_heads % k->kv_heads != 0 || a->q_heads > 65535)
+        return fail(c, LARQL_REFUSED_SHAPE, "attention: q_heads is a multiple of the key/value heads");
+    if (b->tokens * (a->q_heads / k->kv_heads) > (1u << 28)) return fail(c, LARQL_UNSUPPORTED, "attention: too many query rows");
+    if (a->window > 0x7FFFFFFFull) return fail(c, LARQL_UNSUPPORTED, "attention: window too large");
+    if (!(a->softcap >= 0.f) || !std::isfinite(a->softcap) || !std::isfinite(a->scale))
+        return fail(c, LARQL_REFUSED_SHAPE, "attention: scale and softcap are finite, softcap is not negative");
+    if (!a->q || !a->out) return LARQL_E_ARG;
+    if (!row_fits(a->q, a->q_stride, A.q_type, a->q_heads, k->head_dim) || !row_fits(a->out, a->out_stride, A.out_type, a->q_heads, k->head_dim))
+        return fail(c, LARQL_REFUSED_SHAPE, "attention: rows must be 16-byte aligned and hold all heads");
+    if ((uintptr_t)a->sinks & 3) return fail(c, LARQL_REFUSED_SHAPE, "attention: sinks must be 4-byte aligned");
+    A.q = a->q; A.out = a->out; A.q_stride = a->q_stride; A.out_stride = a->out_stride; A.sinks = a->sinks;
+    A.q_heads = (uint32_t)a->q_heads; A.window = (uint32_t)a->window; A.causal = a->causal != 0;
+    A.scale = a->scale; A.softcap = a->softcap;
+    return LARQL_OK;
+}
+
+static int check_attention_workspace(larql_hip_ctx *c, const AttentionArgs &A, const void *workspace, size_t bytes) {
+    if (bytes < attention_workspace_bytes(A)) return fail(c, LARQL_REFUSED_SHAPE, "attention: workspace too small");
+    if (!workspace) return LARQL_E_ARG;
+    if ((uintptr_t)workspace & 15) return fail(c, LARQL_REFUSED_SHAPE, "attention: workspace must be 16-byte aligned");
+    return LARQL_OK;
+}
+
+static int refused_or_arg(int rc) { return rc ? rc : LARQL_E_ARG; }
+
+static int layer_plan(larql_hip_ctx *c, const LayerCall &call, larql_hip_plan **out) {
+    larql_hip_plan *plan = new (std::nothrow) larql_hip_plan();
+    if (!plan) return fail(c, LARQL_E_DEVICE, "plan: out of memory");
+    plan->layer = call;
+    *out = plan;
+    return LARQL_OK;
+}
+
+// (Without a context the arguments are checked all the same: a refusal is a refusal on every machine.)
+int larql_hip_dev_residual_norm(larql_hip_ctx *c, const larql_hip_residual_norm *args) {
+    NormArgs A;
+    if (!c) return refused_or_arg(check_residual_norm(nullptr, args, A));
+    std::lock_guard<std::mutex> lk(c->mu);
+    const int rc = check_residual_norm(c, args, A);
+    if (rc || A.rows == 0) return rc;
+    HIPCHECK(c, hipSetDevice(c->device));
+    HIPCHECK(c, residual_norm_launch(c->stream, A));
+    return LARQL_OK;
+}
+
+int larql_hip_plan_create_residual_norm(larql_hip_ctx *c, const larql_hip_residual_norm *args, larql_hip_plan **out) {
+    if (!c || !out) return LARQL_E_ARG;
+    *out = nullptr;
+    std::lock_guard<std::mutex> lk(c->mu);
+    LayerCall call;
+    const int rc = check_residual_norm(c, args, call.norm);
+    if (rc) return rc;
+    if (call.norm.rows) call.kind = LayerCall::NORM;
+    return layer_plan(c, call, out);
+}
+
+int larql_hip_dev_kv_append(larql_hip_ctx *c, const larql_hip_kv_cache *cache, const larql_hip_kv_batch *batch, const larql_hip_kv_append *args) {
+    KvAppendArgs A;
+    bool empty = false;
+    if (!c) return refused_or_arg(check_kv_append(nullptr, cache, batch, args, A, &empty));
+    std::lock_guard<std::mutex> lk(c->mu);
+    const int rc = check_kv_append(c, cache, batch, args, A, &empty);
+    if (rc || empty) return rc;
+    HIPCHECK(c, hipSetDevice(c->device));
+    HIPCHECK(c, kv_append_launch(c->stream, A));
+    return LARQL_OK;
+}
+
+int larql_hip_plan_create_kv_append(larql_hip_ctx *c, const larql_hip_kv_cache *cache, const larql_hip_kv_batch *batch,
+                                    const larql_hip_kv_append *args, larql_hip_plan **out) {
+    if (!c || !out) return LARQL_E_ARG;
+    *out = nullptr;
+    std::lock_guard<std::mutex> lk(c->mu);
+    LayerCall call;
+    bool empty = false;
+    const int rc = check_kv_append(c, cache, batch, args, call.append, &empty);
+    if (rc) return rc;
+    if (!empty) call.kind = LayerCall::APPEND;
+    return layer_plan(c, call, out);
+}
+
+size_t larql_hip_attention_workspace_bytes(const larql_hip_kv_cache *cache, const larql_hip_kv_batch *batch, const larql_hip_attention *args) {
+    AttentionArgs A;
+    bool empty = false;
+    if (check_attention(nullptr, cache, batch, args, A, &empty) || empty) return 0;
+    return attention_workspace_bytes(A);
+}
+
+int larql_hip_dev_attention(larql_hip_ctx *c, const larql_hip_kv_cache *cache, const larql_hip_kv_batch *batch, const larql_hip_attention *args,
+                            void *workspace, size_t workspace_bytes) {
+    AttentionArgs A;
+    bool empty = false;
+    if (!c) {
+        const int rc = check_attention(nullptr, cache, batch, args, A, &empty);
+        return refused_or_arg(rc || empty ? rc : check_attention_workspace(nullptr, A, workspace, workspace_bytes));
+    }
+    std::lock_guard<std::mutex> lk(c->mu);
+    int rc = check_attention(c, cache, batch, args, A, &empty);
+    if (rc || empty) return rc;
+    rc = check_attention_workspace(c, A, workspace, workspace_bytes);
+    if (rc) return rc;
+    HIPCHECK(c, hipSetDevice(c->device));
+    HIPCHECK(c, attention_launch(c->stream, A, workspace));
+    return LARQL_OK;
+}
+
+int larql_hip_plan_create_attention(larql_hip_ctx *c, const larql_hip_kv_cache *cache, const larql_hip_kv_batch *batch,
+                                    const larql_hip_attention *args, void *workspace, size_t workspace_bytes, larql_hip_plan **out) {
+    if (!c || !out) return LARQL_E_ARG;
+    *out = nullptr;
+    std::lock_guard<std::mutex> lk(c->mu);
+    LayerCall call;
+    bool empty = false;
+    int rc = check_attention(c, cache, batch, args, call.attention, &empty);
+    if (rc) return rc;
+    if (empty) return layer_plan(c, call, out);
+    rc = check_attention_workspace(c, call.attention, workspace, workspace_bytes);
+    if (rc) return rc;
+    call.kind = LayerCall::ATTENTION;
+    call.workspace = workspace;
+    return layer_plan(c, call, out);
 }
 
 // ---- device tier: encoders ---------------------------------------------------------------------

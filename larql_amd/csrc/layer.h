@@ -1,0 +1,153 @@
+// layer.h — what a decoder layer does between its matrix products (norm.hip, kv_append.hip, attention.hip): arguments of the
+// kernels, and what they share on the device.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "wave.h"
+
+namespace larql {
+
+enum ElemType : int32_t { ELEM_F32 = 0, ELEM_BF16 = 1, ELEM_F16 = 2 };
+__host__ __device__ constexpr uint32_t elem_bytes(int t) { return t == ELEM_F32 ? 4u : 2u; }
+
+struct NormArgs {  // strides in elements
+    const void *block, *residual;
+    void *residual_out, *normed;
+    const float *gate, *post_weight, *pre_weight;
+    size_t block_stride, residual_stride, residual_out_stride, normed_stride, gate_stride;
+    int32_t block_type, residual_type, normed_type;
+    uint32_t rows, hidden;
+    float residual_scale, norm_offset, eps;
+    uint32_t vec;  // every row of every operand starts 16-byte aligned and holds whole groups of 8 elements
+};
+constexpr uint32_t kNormMaxHidden = 32768;
+hipError_t residual_norm_launch(hipStream_t s, const NormArgs &A);
+
+// The paged cache and the sequences of a step (larql_hip_kv_cache, larql_hip_kv_batch).
+struct KvArgs {
+    uint8_t *k_codes, *v_codes;
+    float *k_scales, *v_scales;
+    const int32_t *kv_len, *block_table, *q_start;
+    uint32_t num_pages, kv_heads, head_dim, page_shift;  // page_tokens = 1 << page_shift
+    uint32_t sequences, table_width, tokens, max_new;
+};
+constexpr int kScaleMinExp = -40, kScaleMaxExp = 60;
+
+struct KvAppendArgs {
+    KvArgs kv;
+    const void *q, *k, *v;
+    void *q_out;
+    size_t q_stride, q_out_stride, k_stride, v_stride;
+    const float *inv_freq, *q_norm, *k_norm;
+    int32_t type;
+    uint32_t q_heads, rot_dim, interleaved;
+    float rope_scale, norm_offset, norm_eps;
+};
+hipError_t kv_append_launch(hipStream_t s, const KvAppendArgs &A);
+
+struct AttentionArgs {
+    KvArgs kv;
+    const void *q;
+    void *out;
+    size_t q_stride, out_stride;
+    const float *sinks;
+    int32_t q_type, out_type;
+    uint32_t q_heads, window, causal;
+    float scale, softcap;
+};
+size_t attention_workspace_bytes(const AttentionArgs &A);
+int attention_launches(const AttentionArgs &A);
+hipError_t attention_launch(hipStream_t s, const AttentionArgs &A, void *workspace);
+
+// ---- device ---------------------------------------------------------------------------------------------------------
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float bf16_bits_to_f32(uint32_t b) { return __builtin_bit_cast(float, b << 16); }
+// to nearest even; a NaN stays one
+__device__ __forceinline__ uint32_t f32_to_bf16_rne(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    return x != x ? (u >> 16) | 0x40u : (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+}
+__device__ __forceinline__ uint32_t f32_to_f16_bits(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+__device__ __forceinline__ float f16_bits_to_f32(uint32_t b) { return (float)__builtin_bit_cast(_Float16, (uint16_t)b); }
+
+// element i of a row
+__device__ __forceinline__ float load_elem(const void *p, int type, size_t i) {
+    if (type == ELEM_F32) return ((const float *)p)[i];
+    const uint32_t b = ((const uint16_t *)p)[i];
+    return type == ELEM_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+}
+__device__ __forceinline__ void store_elem(void *p, int type, size_t i, float v) {
+    if (type == ELEM_F32) ((float *)p)[i] = v;
+    else ((uint16_t *)p)[i] = (uint16_t)(type == ELEM_BF16 ? f32_to_bf16_rne(v) : f32_to_f16_bits(v));
+}
+// 8 elements from an element offset at which the address is 16-byte aligned
+__device__ __forceinline__ void load8(const void *p, int type, size_t i, float (&o)[8]) {
+    if (type == ELEM_F32) {
+        const f32x4_t a = *(const f32x4_t *)((const float *)p + i), b = *(const f32x4_t *)((const float *)p + i + 4);
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] = a[j], o[4 + j] = b[j];
+        return;
+    }
+    const u32x4_t a = *(const u32x4_t *)((const uint16_t *)p + i);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        o[2 * j] = type == ELEM_BF16 ? bf16_bits_to_f32(a[j] & 0xFFFFu) : f16_bits_to_f32(a[j] & 0xFFFFu);
+        o[2 * j + 1] = type == ELEM_BF16 ? __builtin_bit_cast(float, a[j] & 0xFFFF0000u) : f16_bits_to_f32(a[j] >> 16);
+    }
+}
+__device__ __forceinline__ uint32_t pack2(int type, float a, float b) {
+    return type == ELEM_BF16 ? f32_to_bf16_rne(a) | f32_to_bf16_rne(b) << 16 : f32_to_f16_bits(a) | f32_to_f16_bits(b) << 16;
+}
+__device__ __forceinline__ void store8(void *p, int type, size_t i, const float (&v)[8]) {
+    if (type == ELEM_F32) {
+        *(f32x4_t *)((float *)p + i) = f32x4_t{v[0], v[1], v[2], v[3]};
+        *(f32x4_t *)((float *)p + i + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+        return;
+    }
+    *(u32x4_t *)((uint16_t *)p + i) = u32x4_t{pack2(type, v[0], v[1]), pack2(type, v[2], v[3]), pack2(type, v[4], v[5]), pack2(type, v[6], v[7])};
+}
+// 4 elements, 8-byte (16 bits) or 16-byte (f32) aligned
+__device__ __forceinline__ void load4(const void *p, int type, size_t i, float (&o)[4]) {
+    if (type == ELEM_F32) {
+        const f32x4_t a = *(const f32x4_t *)((const float *)p + i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] = a[j];
+        return;
+    }
+    const u32x2_t a = *(const u32x2_t *)((const uint16_t *)p + i);
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        o[2 * j] = type == ELEM_BF16 ? bf16_bits_to_f32(a[j] & 0xFFFFu) : f16_bits_to_f32(a[j] & 0xFFFFu);
+        o[2 * j + 1] = type == ELEM_BF16 ? __builtin_bit_cast(float, a[j] & 0xFFFF0000u) : f16_bits_to_f32(a[j] >> 16);
+    }
+}
+__device__ __forceinline__ void store4(void *p, int type, size_t i, const float (&v)[4]) {
+    if (type == ELEM_F32) *(f32x4_t *)((float *)p + i) = f32x4_t{v[0], v[1], v[2], v[3]};
+    else *(u32x2_t *)((uint16_t *)p + i) = u32x2_t{pack2(type, v[0], v[1]), pack2(type, v[2], v[3])};
+}
+
+// The page of a sequence's token at `key` (its table's row at `table`), or ~0: a hole, or beyond the table.
+__host__ __device__ __forceinline__ uint32_t kv_page(const KvArgs &kv, const int32_t *table, uint32_t key) {
+    const uint32_t j = key >> kv.page_shift;
+    if (j >= kv.table_width) return ~0u;
+    const uint32_t p = (uint32_t)table[j];
+    return p < kv.num_pages ? p : ~0u;
+}
+
+// New tokens of sequence s: their first row, or none where the rows do not fit.
+struct NewTokens {
+    uint32_t row, n;
+    int32_t len;  // of the sequence, new tokens included
+};
+__host__ __device__ __forceinline__ NewTokens new_tokens(const KvArgs &kv, uint32_t s) {
+    const int32_t a = kv.q_start[s], b = kv.q_start[s + 1], len = kv.kv_len[s];
+    const bool fits = a >= 0 && b >= a && (uint32_t)b <= kv.tokens && (uint32_t)(b - a) <= kv.max_new;
+    return {fits ? (uint32_t)a : 0u, fits ? (uint32_t)(b - a) : 0u, len < 0 ? 0 : len};
+}
+
+}  // namespace larql

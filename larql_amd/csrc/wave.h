@@ -52,6 +52,17 @@ __device__ __forceinline__ float row16_max(float v) {
     return dpp_max<0x140>(v); // row_mirror
 }
 
+// the wavefront's sum, in one order whatever the values
+__device__ __forceinline__ float wave_fsum(float v) {
+    v += dpp_move<0xB1>(v);         // quad_perm [1,0,3,2]
+    v += dpp_move<0x4E>(v);         // quad_perm [2,3,0,1]
+    v += dpp_move<0x141>(v);        // row_half_mirror
+    v += dpp_move<0x140>(v);        // row_mirror: every lane holds its row's sum
+    v += dpp_move<0x142, 0xA>(v);   // row_bcast:15 into rows 1 and 3
+    v += dpp_move<0x143, 0xC>(v);   // row_bcast:31 into rows 2 and 3
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 // inclusive sums
 __device__ __forceinline__ uint32_t wave_inclusive_sum(uint32_t v) {
     v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);  // row_shr:1
