@@ -119,7 +119,7 @@ struct Partials {
 };
 
 template <int NK, bool PAIRS, bool CAP>
-__global__ void __launch_bounds__(kAttnThreads) attention_rows_kernel(AttentionArgs A, Partials part) {
+__global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_rows_kernel(AttentionArgs A, Partials part) {
     constexpr uint32_t D = NK * 32, kPad = D + 4;
     __shared__ float sh_acc[kAttnWaves][kTile][kPad];
     __shared__ float sh_ml[kAttnWaves][kTile][2];
@@ -181,7 +181,6 @@ __global__ void __launch_bounds__(kAttnThreads) attention_rows_kernel(AttentionA
     all_hi = __builtin_amdgcn_readfirstlane(all_hi), all_lo = __builtin_amdgcn_readfirstlane(all_lo);
     any_hi = __builtin_amdgcn_readfirstlane(any_hi), any_lo = __builtin_amdgcn_readfirstlane(any_lo);
 
-    const uint32_t step_end = min(sh.step_lo + (it.piece + 1) * it.chunk, sh.step_lo + sh.steps);
     const int32_t *table = kv.block_table + (size_t)it.s * kv.table_width;
     const uint32_t page_mask = (1u << kv.page_shift) - 1;
     const size_t head_codes = (size_t)D << kv.page_shift;
@@ -190,53 +189,77 @@ __global__ void __launch_bounds__(kAttnThreads) attention_rows_kernel(AttentionA
     for (int i = 0; i < 2 * NK; i++) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float M = kNoMax, L = 0.f;
 
-    for (uint32_t step = sh.step_lo + it.piece * it.chunk + wave; step < step_end; step += kAttnWaves) {
-        const int32_t key0 = (int32_t)(step * kStep);
-        if (key0 > any_hi || key0 + (int32_t)kStep <= any_lo) continue;
-        // pages of the 16 keys whose rows this lane loads of K, and of those that it holds of V and of the weights
-        const uint32_t gk = n / 4;
-        const auto page_of = [&](uint32_t grp) -> uint32_t {
-            const uint32_t key = (uint32_t)key0 + grp * 16;
-            return (int32_t)key >= sh.len ? ~0u : kv_page(kv, table, key);
-        };
-        const uint32_t page_k = page_of(gk), page_v = page_of(g);
+    // Steps of this piece that some row sees, every kAttnWaves-th of them this wavefront's.  A step's page numbers are read two steps
+    // ahead, its key codes one step ahead (while the step before multiplies values), its value codes while its scores form: a
+    // wavefront always has a load of its own 64 x head_dim bytes or more in flight.
+    const uint32_t step_end = any_hi < 0 ? 0u : min(min(sh.step_lo + (it.piece + 1) * it.chunk, sh.step_lo + sh.steps), (uint32_t)any_hi / kStep + 1);
+    uint32_t step = max(sh.step_lo + it.piece * it.chunk, any_lo == 0x7FFFFFFF ? step_end : (uint32_t)any_lo / kStep) + wave;
+    const uint32_t gk = n / 4;  // this lane loads keys of group gk, and values and weights of group g, of a step
+    const auto page_of = [&](uint32_t st, uint32_t grp) -> uint32_t {
+        const uint32_t key = st * kStep + grp * 16;
+        return st >= step_end || (int32_t)key >= sh.len ? ~0u : kv_page(kv, table, key);
+    };
+    u32x4_t kc[4][(NK + 1) / 2], vc[2 * NK];
+    float ks = 0.f, vs = 1.f;
+    const auto load_keys = [&](uint32_t st, uint32_t page_k, uint32_t page_v) {
         const uint8_t *kp = kv.k_codes + ((size_t)(page_k == ~0u ? 0u : page_k) * kv.kv_heads + kvh) * head_codes +
-                            (size_t)(((uint32_t)key0 + gk * 16) & page_mask) * D;
-        const uint8_t *vp = kv.v_codes + ((size_t)(page_v == ~0u ? 0u : page_v) * kv.kv_heads + kvh) * head_codes + (((uint32_t)key0 + g * 16) & page_mask);
-        const size_t scale_at = (size_t)(page_v == ~0u ? 0u : page_v) * kv.kv_heads + kvh;
-        float ks = kv.k_scales[scale_at];
-        const float vs = kv.v_scales[scale_at];
+                            (size_t)((st * kStep + gk * 16) & page_mask) * D;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int k = 0; k < NK; k += 2) {
+                const uint8_t *kr = kp + (size_t)(4 * t + n % 4) * D + k * 32;
+                if (k + 1 < NK) {
+                    kc[t][k / 2] = *(const u32x4_t *)(kr + g * 16);
+                } else {
+                    const u32x2_t c = *(const u32x2_t *)(kr + g * 8);
+                    kc[t][k / 2] = u32x4_t{c[0], c[1], 0u, 0u};
+                }
+            }
+        const size_t at = (size_t)(page_v == ~0u ? 0u : page_v) * kv.kv_heads + kvh;
+        ks = kv.k_scales[at];
+        vs = kv.v_scales[at];
+    };
+    uint32_t page_k = page_of(step, gk), page_v = page_of(step, g);
+    if (step < step_end) load_keys(step, page_k, page_v);
+    uint32_t next_k = page_of(step + kAttnWaves, gk), next_v = page_of(step + kAttnWaves, g);
 
+    for (; step < step_end; step += kAttnWaves) {
+        const int32_t key0 = (int32_t)(step * kStep);
+        const bool hole = page_v == ~0u;
+        {
+            const uint8_t *vp = kv.v_codes + ((size_t)(hole ? 0u : page_v) * kv.kv_heads + kvh) * head_codes + (((uint32_t)key0 + g * 16) & page_mask);
+#pragma unroll
+            for (int d = 0; d < 2 * NK; d++) vc[d] = *(const u32x4_t *)(vp + ((size_t)(d * 16 + n) << kv.page_shift));
+        }
+        __builtin_amdgcn_sched_barrier(0);
         f32x4_t S[4];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const uint8_t *kr = kp + (size_t)(4 * t + n % 4) * D;
             S[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < NK; k += 2) {
-                f16x8_t ka, kb;
-                if (k + 1 < NK) {
-                    const u32x4_t c = *(const u32x4_t *)(kr + k * 32 + g * 16);
-                    ka = codes_f16(u32x2_t{c[0], c[1]});
-                    kb = codes_f16(u32x2_t{c[2], c[3]});
-                } else {
-                    ka = codes_f16(*(const u32x2_t *)(kr + k * 32 + g * 8));
-                }
+            for (int k = 0; k < NK; k++) {
+                const u32x4_t c = kc[t][k / 2];
+                const f16x8_t ka = codes_f16(k % 2 ? u32x2_t{c[2], c[3]} : u32x2_t{c[0], c[1]});
                 S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[k], S[t], 0, 0, 0);
                 if constexpr (PAIRS) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[k], S[t], 0, 0, 0);
-                if (k + 1 < NK) {
-                    S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qh[k + 1 < NK ? k + 1 : k], S[t], 0, 0, 0);
-                    if constexpr (PAIRS) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, ql[k + 1 < NK ? k + 1 : k], S[t], 0, 0, 0);
-                }
             }
         }
+        float cur_ks = ks;
+        const float cur_vs = vs;
+        __builtin_amdgcn_sched_barrier(0);
+        page_k = next_k, page_v = next_v;
+        if (step + kAttnWaves < step_end) {
+            load_keys(step + kAttnWaves, page_k, page_v);
+            next_k = page_of(step + 2 * kAttnWaves, gk), next_v = page_of(step + 2 * kAttnWaves, g);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         // Logarithms (base 2) of the weights times the value scale.  A scale that is not a number makes its tokens' scores NaN.
-        const bool hole = page_v == ~0u;
-        const bool odd = !(vs == vs);
-        if (odd) ks = __builtin_nanf("");
-        const int ev = odd || hole ? 0 : (int)(__builtin_bit_cast(uint32_t, vs) >> 23 & 0xFFu) - 127;
+        const bool odd = !(cur_vs == cur_vs);
+        if (odd) cur_ks = __builtin_nanf("");
+        const int ev = odd || hole ? 0 : (int)(__builtin_bit_cast(uint32_t, cur_vs) >> 23 & 0xFFu) - 127;
         const float unscale = __builtin_bit_cast(float, (uint32_t)(127 - ev) << 23);
-        const float a = factor * ks;
+        const float a = factor * cur_ks;
         float x[16];
 #pragma unroll
         for (int t = 0; t < 4; t++)
@@ -283,7 +306,7 @@ __global__ void __launch_bounds__(kAttnThreads) attention_rows_kernel(AttentionA
         }
 #pragma unroll
         for (int d = 0; d < 2 * NK; d++) {
-            u32x4_t c = *(const u32x4_t *)(vp + ((size_t)(d * 16 + n) << kv.page_shift));
+            u32x4_t c = vc[d];
             if (!plain) {  // bytes behind the last key may be anything
                 const int32_t have = hole ? 0 : sh.len - key0 - (int32_t)g * 16;
 #pragma unroll
@@ -336,35 +359,67 @@ __global__ void __launch_bounds__(kAttnThreads) attention_rows_kernel(AttentionA
     }
 }
 
-// The pieces of split rows as one: a wavefront for each query row of a tile.
+// The pieces of split rows as one: a workgroup for each query row of a tile (rows of tiles that are not split leave at once), its
+// wavefronts a quarter of the pieces each.
 __global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttentionArgs A, Partials part, uint32_t items_per_head) {
+    __shared__ float sh_acc[kAttnWaves][256], sh_ml[kAttnWaves][2];
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, D = A.kv.head_dim;
-    const uint32_t kvh = blockIdx.y, group = A.q_heads / A.kv.kv_heads;
+    const uint32_t kvh = blockIdx.y, group = A.q_heads / A.kv.kv_heads, r = blockIdx.z;
     Item it;
     uint32_t first_item;
     if (!find_item(A, blockIdx.x, true, it, first_item) || it.pieces < 2) return;
     const Share sh = share_of(A, it.s, group);
-    const size_t item0 = (size_t)kvh * items_per_head + first_item;
-    for (uint32_t r = wave; r < kTile; r += kAttnWaves) {
-        const uint32_t q = it.tile * kTile + r;
-        if (q >= sh.n * group) break;
-        float top = kNoMax;
-        for (uint32_t p = lane; p < it.pieces; p += 64) top = fmaxf(top, part.ml[((item0 + p) * kTile + r) * 2]);
-        top = wave_fmax(top);
-        float l = 0.f;
-        f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        for (uint32_t p = 0; p < it.pieces; p++) {
-            const float *ml = part.ml + ((item0 + p) * kTile + r) * 2;
-            const float f = __builtin_amdgcn_exp2f(ml[0] - top);
-            l = fmaf(f, ml[1], l);
-            if (lane * 4 < D) o += *(const f32x4_t *)(part.acc + ((item0 + p) * kTile + r) * D + lane * 4) * f;
+    const uint32_t q = it.tile * kTile + r;
+    if (q >= sh.n * group) return;
+    const size_t at = ((size_t)kvh * items_per_head + first_item) * kTile + r;  // row r of the first piece; the next kTile rows on
+    float top = kNoMax, l = 0.f;
+    f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    const uint32_t dim = min(lane * 4, D - 4);
+    for (uint32_t p0 = wave; p0 < it.pieces; p0 += 8 * kAttnWaves) {
+        float m[8], s[8];
+        f32x4_t a[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {  // (beyond the last piece: the last once more, with no weight)
+            const uint32_t p = p0 + i * kAttnWaves;
+            const size_t x = at + (size_t)min(p, it.pieces - 1) * kTile;
+            m[i] = p < it.pieces ? part.ml[2 * x] : kNoMax;
+            s[i] = part.ml[2 * x + 1];
+            a[i] = *(const f32x4_t *)(part.acc + x * D + dim);
         }
-        const uint32_t h = kvh * group + q % group;
-        if (A.sinks && l != 0.f) l += __builtin_amdgcn_exp2f(A.sinks[h] * kLog2E - top + kBias);
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-        if (lane * 4 < D) store4(A.out, A.out_type, (size_t)(sh.row + q / group) * A.out_stride + (size_t)h * D + lane * 4, v);
+        float next = top;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) next = fmaxf(next, m[i]);
+        const float f = __builtin_amdgcn_exp2f(top - next);
+        o *= f;
+        l *= f;
+        top = next;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            if (p0 + i * kAttnWaves >= it.pieces) break;
+            const float w = __builtin_amdgcn_exp2f(m[i] - top);
+            l = fmaf(w, s[i], l);
+            o += a[i] * w;
+        }
     }
+    if (lane == 0) sh_ml[wave][0] = top, sh_ml[wave][1] = l;
+    if (lane * 4 < D) *(f32x4_t *)&sh_acc[wave][lane * 4] = o;
+    __syncthreads();
+    if (wave || lane * 4 >= D) return;
+#pragma unroll
+    for (uint32_t w = 1; w < kAttnWaves; w++) top = fmaxf(top, sh_ml[w][0]);
+    l = 0.f;
+    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (uint32_t w = 0; w < kAttnWaves; w++) {
+        const float f = __builtin_amdgcn_exp2f(sh_ml[w][0] - top);
+        l = fmaf(f, sh_ml[w][1], l);
+        o += *(const f32x4_t *)&sh_acc[w][lane * 4] * f;
+    }
+    const uint32_t h = kvh * group + q % group;
+    if (A.sinks && l != 0.f) l += __builtin_amdgcn_exp2f(A.sinks[h] * kLog2E - top + kBias);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+    store4(A.out, A.out_type, (size_t)(sh.row + q / group) * A.out_stride + (size_t)h * D + lane * 4, v);
 }
 
 static size_t items_of(const AttentionArgs &A) { return (size_t)items_bound(A) * A.kv.kv_heads; }
@@ -401,7 +456,8 @@ hipError_t attention_launch(hipStream_t s, const AttentionArgs &A, void *workspa
     default: return hipErrorInvalidValue;
     }
     const uint64_t group = A.q_heads / A.kv.kv_heads, tiles = A.kv.tokens * group / kTile + A.kv.sequences;
-    hipLaunchKernelGGL(attention_join_kernel, dim3((uint32_t)tiles, A.kv.kv_heads), dim3(kAttnThreads), 0, s, A, part, (uint32_t)items);
+    const uint32_t join_rows = (uint32_t)std::min<uint64_t>(A.kv.max_new * group, kTile);
+    hipLaunchKernelGGL(attention_join_kernel, dim3((uint32_t)tiles, A.kv.kv_heads, join_rows), dim3(kAttnThreads), 0, s, A, part, (uint32_t)items);
     return hipGetLastError();
 }
 
