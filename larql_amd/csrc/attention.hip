@@ -18,18 +18,29 @@ namespace larql {
 
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr uint32_t kStep = 64;          // keys of a step
 constexpr uint32_t kAttnThreads = 256;
 constexpr uint32_t kAttnWaves = kAttnThreads / 64;
-constexpr uint32_t kTile = 16;          // query rows of a workgroup
-constexpr uint32_t kTargetItems = 1024; // pieces that long rows are split into, over all heads
-constexpr uint32_t kMinSteps = 4;       // steps of a piece at least
+constexpr uint32_t kRowsTile = 16;      // query rows of a workgroup of the kernel for few rows
+constexpr uint32_t kTilesTile = 128;    // ... for many
+constexpr uint32_t kFewRows = 32;       // a sequence with at most this many rows for each key/value head goes through the former
 constexpr float kLog2E = 1.44269504088896341f;
 // Weights are held as 2^(t + e - M + 12) with t + e - M <= 3, so that the f16 pair of an f32 weight keeps 22 bits down to 2^-15 of the
 // largest and 2^-37 of it beyond; M only moves where a score leaves that range.
 constexpr float kBias = 12.f, kSlack = 3.f;
 constexpr float kNoMax = -1e30f;
+
+// How one of the two kernels shares its work out.
+struct Plan {
+    uint32_t tile;                // query rows of a workgroup
+    uint32_t rows_min, rows_max;  // sequences with this many rows for each key/value head are its own
+    uint32_t target;              // pieces of one head's work that long rows are split into
+    uint32_t min_steps;           // steps of a piece at least
+    uint32_t split;               // whether rows are split at all
+};
 
 // A sequence's share of the work: its query rows in tiles, and the steps of keys that any of them sees.
 struct Share {
@@ -37,69 +48,90 @@ struct Share {
     int32_t len, first;   // keys, position of the first new token
     uint32_t tiles, step_lo, steps;
 };
-__device__ __forceinline__ Share share_of(const AttentionArgs &A, uint32_t s, uint32_t group) {
+__device__ __forceinline__ Share share_of(const AttentionArgs &A, const Plan &P, uint32_t s, uint32_t group) {
     const NewTokens t = new_tokens(A.kv, s);
     Share h;
     h.row = t.row;
     h.n = t.n;
     h.len = (int32_t)min((uint64_t)t.len, (uint64_t)A.kv.table_width << A.kv.page_shift);
     h.first = t.len - (int32_t)t.n;
-    h.tiles = (t.n * group + kTile - 1) / kTile;
+    const uint32_t rows = t.n * group;
+    h.tiles = rows < P.rows_min || rows > P.rows_max ? 0u : (rows + P.tile - 1) / P.tile;
     const int32_t lo = A.window ? (int32_t)max((int64_t)h.first - (int64_t)A.window + 1, (int64_t)0) : 0;
     h.step_lo = (uint32_t)lo / kStep;
-    h.steps = h.n && h.len > lo ? ((uint32_t)h.len + kStep - 1) / kStep - h.step_lo : 0;
+    h.steps = h.tiles && h.len > lo ? ((uint32_t)h.len + kStep - 1) / kStep - h.step_lo : 0;
     return h;
 }
 
 // What the wavefront that serves item `item` of a head works on; false beyond the last.  Every wavefront finds it from the lengths:
-// pieces of `chunk` steps, as many as kTargetItems over all heads asks for.
+// tiles of sequences in order, each tile's keys in pieces of `chunk` steps, as many as P.target asks for.  Pieces of split tiles
+// have places for their partial results, `slot` on; `split_tiles`: items count split tiles instead.
 struct Item {
-    uint32_t s, tile, piece, pieces, chunk;
+    uint32_t s, tile, piece, pieces, chunk, slot;
 };
-__device__ __forceinline__ bool find_item(const AttentionArgs &A, uint32_t item, bool by_tile, Item &it, uint32_t &first_item) {
+__device__ __forceinline__ bool find_item(const AttentionArgs &A, const Plan &P, uint32_t item, bool split_tiles, Item &it) {
     const uint32_t lane = threadIdx.x % 64, group = A.q_heads / A.kv.kv_heads;
-    float units = 0.f;  // (tiles x steps; their sum need not be exact)
-    for (uint32_t base = 0; base < A.kv.sequences; base += 64)
-        if (base + lane < A.kv.sequences) {
-            const Share h = share_of(A, base + lane, group);
-            units += (float)h.tiles * (float)h.steps;
-        }
-    units = wave_fsum(units);
-    const uint32_t target = max(kTargetItems / A.kv.kv_heads, 1u);
-    const uint32_t chunk = max((uint32_t)ceilf(units / (float)target), kMinSteps);
-    first_item = 0;
+    it.chunk = 0x7FFFFFFFu;
+    if (P.split) {
+        float units = 0.f;  // (tiles x steps; their sum need not be exact)
+        for (uint32_t base = 0; base < A.kv.sequences; base += 64)
+            if (base + lane < A.kv.sequences) {
+                const Share h = share_of(A, P, base + lane, group);
+                units += (float)h.tiles * (float)h.steps;
+            }
+        it.chunk = max((uint32_t)ceilf(wave_fsum(units) / (float)P.target), P.min_steps);
+    }
+    it.slot = 0;
     for (uint32_t base = 0; base < A.kv.sequences; base += 64) {
         uint32_t tiles = 0, pieces = 1;
         if (base + lane < A.kv.sequences) {
-            const Share h = share_of(A, base + lane, group);
+            const Share h = share_of(A, P, base + lane, group);
             tiles = h.tiles;
-            pieces = max((h.steps + chunk - 1) / chunk, 1u);
+            pieces = max(h.steps / it.chunk + (h.steps % it.chunk ? 1u : 0u), 1u);
         }
-        const uint32_t weight = by_tile ? tiles : tiles * pieces;
+        const uint32_t slots = pieces > 1 ? tiles * pieces : 0u, weight = split_tiles ? (pieces > 1 ? tiles : 0u) : tiles * pieces;
         const uint32_t upto = wave_inclusive_sum(weight), all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-        const uint32_t items_upto = by_tile ? wave_inclusive_sum(tiles * pieces) : upto;
+        const uint32_t slots_upto = P.split ? wave_inclusive_sum(slots) : 0u;
         if (item < all) {
             const int at = (int)__builtin_ctzll(__ballot(upto > item));
             it.pieces = (uint32_t)__builtin_amdgcn_readlane((int)pieces, at);
             const uint32_t in = item - (uint32_t)__builtin_amdgcn_readlane((int)(upto - weight), at);
             it.s = base + (uint32_t)at;
-            it.tile = by_tile ? in : in / it.pieces;
-            it.piece = by_tile ? 0 : in % it.pieces;
-            it.chunk = chunk;
-            first_item += (uint32_t)__builtin_amdgcn_readlane((int)(items_upto - tiles * pieces), at) + it.tile * it.pieces;
+            it.tile = split_tiles ? in : in / it.pieces;
+            it.piece = split_tiles ? 0 : in % it.pieces;
+            it.slot += (uint32_t)__builtin_amdgcn_readlane((int)(slots_upto - slots), at) + it.tile * it.pieces;
             return true;
         }
         item -= all;
-        first_item += (uint32_t)__builtin_amdgcn_readlane((int)items_upto, 63);
+        it.slot += P.split ? (uint32_t)__builtin_amdgcn_readlane((int)slots_upto, 63) : 0u;
     }
     return false;
 }
 
-// Items of one head at most: every sequence's last piece may be short.
-static uint64_t items_bound(const AttentionArgs &A) {
-    const uint64_t group = A.q_heads / A.kv.kv_heads;
-    const uint64_t tiles = A.kv.tokens * group / kTile + A.kv.sequences;
-    return tiles + std::max(kTargetItems / A.kv.kv_heads, 1u) + 1;
+// The two kernels' plans, and what the host has to know of them: items of one head at most (the last piece of a tile may be
+// short), places for partial results (split tiles have at least two pieces: twice the target), and tiles that may be split.
+struct Plans {
+    Plan rows, tiles;
+    bool use_rows, use_tiles;
+    static uint64_t items(const AttentionArgs &A, const Plan &P) {
+        return A.kv.tokens * (uint64_t)(A.q_heads / A.kv.kv_heads) / P.tile + A.kv.sequences + (P.split ? P.target + 1 : 0);
+    }
+    static uint64_t slots(const Plan &P) { return P.split ? 2 * P.target + 2 : 0; }
+    static uint64_t split_tiles(const Plan &P) { return P.split ? P.target + 1 : 0; }
+};
+static Plans plans_of(const AttentionArgs &A) {
+    const uint64_t group = A.q_heads / A.kv.kv_heads, most = A.kv.max_new * group;
+    const uint64_t steps = (((uint64_t)A.kv.table_width << A.kv.page_shift) + kStep - 1) / kStep;
+    const uint32_t cus = 256, per_cu = A.kv.head_dim > 128 ? 1 : 2;  // workgroups of a kernel that a compute unit holds
+    Plans p;
+    p.rows = {kRowsTile, 1, kFewRows, std::max(2 * cus * per_cu / A.kv.kv_heads, 1u), 4, 1};
+    p.rows.split = steps > p.rows.min_steps;
+    p.tiles = {kTilesTile, kFewRows + 1, 0xFFFFFFFFu, std::max(cus * per_cu / A.kv.kv_heads, 1u), 8, 1};
+    p.tiles.split = steps > p.tiles.min_steps && A.kv.tokens * group / kTilesTile + A.kv.sequences < p.tiles.target;
+    p.use_tiles = most > kFewRows;
+    p.use_rows = !p.use_tiles || A.kv.sequences > 1;
+    if (!p.use_rows) p.tiles.rows_min = 1;  // one sequence: one kernel, whatever its number of new tokens turns out to be
+    return p;
 }
 
 // 8 codes as f16
@@ -113,26 +145,71 @@ __device__ __forceinline__ f16x8_t codes_f16(u32x2_t v) {
     return o;
 }
 
-// Partial results of a piece: [items][kTile][head_dim] weighted sums, then [items][kTile] maxima and sums of weights.
+// two weights as f16, or as f16 pairs
+template <bool PAIRS>
+__device__ __forceinline__ void weights_f16(f32x2_t p, f16x8_t &h, f16x8_t &l, int at) {
+    const f16x2_t a = __builtin_convertvector(p, f16x2_t);
+    h[at] = a[0], h[at + 1] = a[1];
+    if constexpr (PAIRS) {
+        const f16x2_t b = __builtin_convertvector(p - __builtin_convertvector(a, f32x2_t), f16x2_t);
+        l[at] = b[0], l[at + 1] = b[1];
+    }
+}
+
+// Partial results of pieces: [kv_heads][slots][tile][head_dim] weighted sums, and [kv_heads][slots][tile] maxima and sums of weights.
 struct Partials {
     float *acc, *ml;
+    uint32_t slots;
 };
 
+// A result row's end: the sink, the quotient.
+__device__ __forceinline__ float inverse_sum(const AttentionArgs &A, float l, float top, uint32_t head) {
+    if (A.sinks && l != 0.f) l += __builtin_amdgcn_exp2f(A.sinks[head] * kLog2E - top + kBias);
+    return l == 0.f ? 0.f : 1.f / l;
+}
+
+// A query row's elements (spread over lanes 32 apart, and 16 apart where QUARTERS) as f16 or f16 pairs after a power-of-two scale that brings
+// the largest to [2^14, 2^15); returns what scores are multiplied by.  A row that is not finite gets NaN there.
+template <int N, bool PAIRS, bool CAP, bool QUARTERS>
+__device__ __forceinline__ float query_f16(const AttentionArgs &A, const float (&q)[N][8], f16x8_t (&qh)[N], f16x8_t (&ql)[PAIRS ? N : 1]) {
+    uint32_t amax = 0;
+#pragma unroll
+    for (int k = 0; k < N; k++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) amax = max(amax, __builtin_bit_cast(uint32_t, q[k][i]) & 0x7FFFFFFFu);
+    if constexpr (QUARTERS) amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16, 64));
+    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32, 64));
+    const bool finite = amax < 0x7F800000u;
+    const int e = min(max((int)(amax >> 23) - 127 - 14, -114), 114);
+    const float inv = finite ? __builtin_bit_cast(float, (uint32_t)(127 - e) << 23) : 0.f;
+    // (the scale's sign goes into the query: factors of scores are not negative)
+    const float sign = A.scale < 0.f ? -inv : inv;
+#pragma unroll
+    for (int k = 0; k < N; k++)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const f32x2_t x = {finite ? q[k][i] * sign : 0.f, finite ? q[k][i + 1] * sign : 0.f};
+            f16x8_t rest;
+            weights_f16<PAIRS>(x, qh[k], PAIRS ? ql[PAIRS ? k : 0] : rest, i);
+        }
+    const float factor = fabsf(A.scale) * (CAP ? 1.f : kLog2E) * __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+    return finite ? factor : __builtin_nanf("");
+}
+
 template <int NK, bool PAIRS, bool CAP>
-__global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_rows_kernel(AttentionArgs A, Partials part) {
+__global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_rows_kernel(AttentionArgs A, Plan P, Partials part) {
     constexpr uint32_t D = NK * 32, kPad = D + 4;
-    __shared__ float sh_acc[kAttnWaves][kTile][kPad];
-    __shared__ float sh_ml[kAttnWaves][kTile][2];
+    __shared__ float sh_acc[kAttnWaves][kRowsTile][kPad];
+    __shared__ float sh_ml[kAttnWaves][kRowsTile][2];
     const KvArgs &kv = A.kv;
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = lane % 16, g = lane / 16;
     const uint32_t kvh = blockIdx.y, group = A.q_heads / kv.kv_heads;
     Item it;
-    uint32_t first_item;
-    if (!find_item(A, blockIdx.x, false, it, first_item)) return;
-    const Share sh = share_of(A, it.s, group);
+    if (!find_item(A, P, blockIdx.x, false, it)) return;
+    const Share sh = share_of(A, P, it.s, group);
 
     // The lane's query row: token and head, what it sees, its elements as f16 after a power-of-two scale.
-    const uint32_t row = it.tile * kTile + n, tok = row / group, head = kvh * group + row % group;
+    const uint32_t row = it.tile * kRowsTile + n, tok = row / group, head = kvh * group + row % group;
     const bool live = tok < sh.n;
     const int32_t pos = sh.first + (int32_t)tok;
     const int32_t key_hi = !live ? -1 : (A.causal ? min(pos, sh.len - 1) : sh.len - 1);
@@ -141,32 +218,14 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_rows_k
     float factor;
     {
         float q[NK][8];
-        uint32_t amax = 0;
 #pragma unroll
         for (int k = 0; k < NK; k++) {
             const uint32_t d = (k | 1) < NK ? (uint32_t)(k & ~1) * 32 + g * 16 + (uint32_t)(k & 1) * 8 : (uint32_t)k * 32 + g * 8;
 #pragma unroll
             for (int i = 0; i < 8; i++) q[k][i] = 0.f;
             if (live) load8(A.q, A.q_type, (size_t)(sh.row + tok) * A.q_stride + (size_t)head * D + d, q[k]);
-#pragma unroll
-            for (int i = 0; i < 8; i++) amax = max(amax, __builtin_bit_cast(uint32_t, q[k][i]) & 0x7FFFFFFFu);
         }
-        amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16, 64));
-        amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32, 64));
-        // largest |q| to [2^14, 2^15)
-        const int e = max((int)(amax >> 23) - 127, -100) - 14;
-        const float inv = __builtin_bit_cast(float, (uint32_t)(127 - min(max(e, -126), 126)) << 23);
-        factor = A.scale * __builtin_bit_cast(float, (uint32_t)(127 + min(max(e, -126), 126)) << 23);
-        if (amax >= 0x7F800000u) factor = __builtin_nanf("");
-#pragma unroll
-        for (int k = 0; k < NK; k++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float x = amax >= 0x7F800000u ? 0.f : q[k][i] * inv;
-                qh[k][i] = (_Float16)x;
-                if constexpr (PAIRS) ql[k][i] = (_Float16)(x - (float)qh[k][i]);
-            }
-        if constexpr (!CAP) factor *= kLog2E;
+        factor = query_f16<NK, PAIRS, CAP, true>(A, q, qh, ql);
     }
     // steps that every live row of the tile sees whole need no mask
     int32_t all_hi = live ? key_hi : 0x7FFFFFFF, all_lo = live ? key_lo : 0;
@@ -297,13 +356,14 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_rows_k
             for (int i = 0; i < 2 * NK; i++) acc[i] *= f;
         }
         f16x8_t ph[2], pl[2];
+        float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float p = __builtin_amdgcn_exp2f(x[i] - M + kBias);
-            L = fmaf(p, unscale, L);
-            ph[i / 8][i % 8] = (_Float16)p;
-            if constexpr (PAIRS) pl[i / 8][i % 8] = (_Float16)(p - (float)ph[i / 8][i % 8]);
+        for (int i = 0; i < 16; i += 2) {
+            const f32x2_t p = {__builtin_amdgcn_exp2f(x[i] - M + kBias), __builtin_amdgcn_exp2f(x[i + 1] - M + kBias)};
+            sum += p[0] + p[1];
+            weights_f16<PAIRS>(p, ph[i / 8], pl[i / 8], i % 8);
         }
+        L = fmaf(sum, unscale, L);
 #pragma unroll
         for (int d = 0; d < 2 * NK; d++) {
             u32x4_t c = vc[d];
@@ -331,9 +391,9 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_rows_k
 #pragma unroll
     for (int d = 0; d < 2 * NK; d++) *(f32x4_t *)&sh_acc[wave][n][d * 16 + g * 4] = acc[d];
     __syncthreads();
-    const uint32_t item = blockIdx.y * gridDim.x + blockIdx.x;
-    for (uint32_t i = threadIdx.x; i < kTile * (D / 4); i += kAttnThreads) {
-        const uint32_t r = i / (D / 4), d = i % (D / 4) * 4, q = it.tile * kTile + r;
+    const size_t slot = (size_t)kvh * part.slots + it.slot + it.piece;
+    for (uint32_t i = threadIdx.x; i < kRowsTile * (D / 4); i += kAttnThreads) {
+        const uint32_t r = i / (D / 4), d = i % (D / 4) * 4, q = it.tile * kRowsTile + r;
         if (q >= sh.n * group) continue;
         float top = kNoMax;
 #pragma unroll
@@ -347,31 +407,263 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_rows_k
             o += *(const f32x4_t *)&sh_acc[w][r][d] * f;
         }
         if (it.pieces > 1) {
-            *(f32x4_t *)(part.acc + ((size_t)item * kTile + r) * D + d) = o;
-            if (d == 0) part.ml[((size_t)item * kTile + r) * 2] = top, part.ml[((size_t)item * kTile + r) * 2 + 1] = l;
+            *(f32x4_t *)(part.acc + (slot * kRowsTile + r) * D + d) = o;
+            if (d == 0) part.ml[(slot * kRowsTile + r) * 2] = top, part.ml[(slot * kRowsTile + r) * 2 + 1] = l;
             continue;
         }
         const uint32_t h = kvh * group + q % group;
-        if (A.sinks && l != 0.f) l += __builtin_amdgcn_exp2f(A.sinks[h] * kLog2E - top + kBias);
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = inverse_sum(A, l, top, h);
         const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
         store4(A.out, A.out_type, (size_t)(sh.row + q / group) * A.out_stride + (size_t)h * D + d, v);
     }
 }
 
-// The pieces of split rows as one: a workgroup for each query row of a tile (rows of tiles that are not split leave at once), its
+// ---- many query rows -------------------------------------------------------------------------------------------------
+//
+// 128 query rows a workgroup, 32 a wavefront, as the columns of v_mfma_f32_32x32x16_f16; the steps' codes are converted to f16 once and
+// lie in LDS, two steps' worth, rows padded by 16 bytes (an odd number of 16-byte pieces: consecutive rows in other banks).  Row p of S^T is
+// the key whose index is p with bits 2 and 3 exchanged: a lane then holds weights of 8 consecutive keys for each k step of the second
+// product, within one group of 16 keys, so a block's scales are the same for all of them.
+template <int NK, bool PAIRS, bool CAP>
+__global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_kernel(AttentionArgs A, Plan P, Partials part) {
+    constexpr uint32_t D = NK * 32, kKeyPad = D + 8, kValPad = kStep + 8;
+    constexpr int kPieces = (int)(kStep * D / 16 / kAttnThreads) + (kStep * D / 16 % kAttnThreads ? 1 : 0);  // 16-byte pieces of a thread
+    __shared__ __align__(16) _Float16 sh_k[2][kStep][kKeyPad];
+    __shared__ __align__(16) _Float16 sh_v[2][D][kValPad];
+    __shared__ float sh_s[2][4][4];  // of each group of 16 keys: key scale, log2 of the value scale, and one over it
+    const KvArgs &kv = A.kv;
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = lane % 32, hi = lane / 32;
+    const uint32_t kvh = blockIdx.x % kv.kv_heads, group = A.q_heads / kv.kv_heads;  // (neighbours: the heads, one for each XCD's cache)
+    Item it;
+    if (!find_item(A, P, blockIdx.x / kv.kv_heads, false, it)) return;
+    const Share sh = share_of(A, P, it.s, group);
+    const uint32_t rows = sh.n * group;
+    const uint32_t tile = sh.tiles - 1 - it.tile;  // (the last rows see the most keys: first)
+
+    const uint32_t row = tile * kTilesTile + wave * 32 + n, tok = row / group, head = kvh * group + row % group;
+    const bool live = row < rows;
+    const int32_t pos = sh.first + (int32_t)tok;
+    const int32_t key_hi = !live ? -1 : (A.causal ? min(pos, sh.len - 1) : sh.len - 1);
+    const int32_t key_lo = A.window ? (int32_t)max((int64_t)pos - (int64_t)A.window + 1, (int64_t)0) : 0;
+    f16x8_t qh[2 * NK], ql[PAIRS ? 2 * NK : 1];
+    float factor;
+    {
+        float q[2 * NK][8];
+#pragma unroll
+        for (int k = 0; k < 2 * NK; k++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) q[k][i] = 0.f;
+            if (live) load8(A.q, A.q_type, (size_t)(sh.row + tok) * A.q_stride + (size_t)head * D + (uint32_t)k * 16 + hi * 8, q[k]);
+        }
+        factor = query_f16<2 * NK, PAIRS, CAP, false>(A, q, qh, ql);
+    }
+    // what all and any of the wavefront's rows see (whole rows of lanes: the first and the last live one say it)
+    const uint32_t first_row = tile * kTilesTile + wave * 32, last_row = min(first_row + 31, rows - 1);
+    const bool any_live = first_row < rows;
+    const auto hi_of = [&](uint32_t r) { return A.causal ? min(sh.first + (int32_t)(r / group), sh.len - 1) : sh.len - 1; };
+    const auto lo_of = [&](uint32_t r) {
+        return A.window ? (int32_t)max((int64_t)sh.first + (int64_t)(r / group) - (int64_t)A.window + 1, (int64_t)0) : 0;
+    };
+    const int32_t all_hi = hi_of(first_row), any_hi = any_live ? hi_of(last_row) : -1;
+    const int32_t any_lo = lo_of(first_row), all_lo = lo_of(any_live ? last_row : first_row);
+    // the workgroup's steps: those of its piece that any of its rows sees
+    const int32_t tile_hi = hi_of(min(tile * kTilesTile + kTilesTile - 1, rows - 1)), tile_lo = lo_of(tile * kTilesTile);
+    const uint64_t piece_lo = (uint64_t)sh.step_lo + (uint64_t)it.piece * it.chunk;
+    const uint32_t end = tile_hi < 0 ? 0u : (uint32_t)min(min(piece_lo + it.chunk, (uint64_t)(sh.step_lo + sh.steps)), (uint64_t)((uint32_t)tile_hi / kStep + 1));
+    uint32_t step = (uint32_t)max(piece_lo, (uint64_t)((uint32_t)tile_lo / kStep));
+
+    const int32_t *table = kv.block_table + (size_t)it.s * kv.table_width;
+    const uint32_t page_mask = (1u << kv.page_shift) - 1;
+    const size_t head_codes = (size_t)D << kv.page_shift;
+    // Staging: a piece is 16 channels of a key's row, or 16 keys of a value channel's.
+    u32x4_t kc[kPieces], vc[kPieces];
+    float ks = 0.f, vs = 0.f;
+    const auto page_of = [&](uint32_t st, uint32_t grp) -> uint32_t {
+        const uint32_t key = st * kStep + grp * 16;
+        return st >= end || (int32_t)key >= sh.len ? ~0u : kv_page(kv, table, key);
+    };
+    const auto load_step = [&](uint32_t st) {
+#pragma unroll
+        for (int i = 0; i < kPieces; i++) {
+            const uint32_t p = threadIdx.x + (uint32_t)i * kAttnThreads;
+            if (kStep * D / 16 % kAttnThreads != 0 && p >= kStep * D / 16) break;
+            const uint32_t key = p / (D / 16), page = page_of(st, key / 16);
+            kc[i] = u32x4_t{0u, 0u, 0u, 0u};
+            if (page != ~0u)
+                kc[i] = *(const u32x4_t *)(kv.k_codes + ((size_t)page * kv.kv_heads + kvh) * head_codes + (size_t)((st * kStep + key) & page_mask) * D +
+                                           p % (D / 16) * 16);
+            const uint32_t d = p / 4, grp = p % 4, page_v = page_of(st, grp);
+            vc[i] = u32x4_t{0u, 0u, 0u, 0u};
+            if (page_v != ~0u) {
+                vc[i] = *(const u32x4_t *)(kv.v_codes + ((size_t)page_v * kv.kv_heads + kvh) * head_codes + ((size_t)d << kv.page_shift) +
+                                           ((st * kStep + grp * 16) & page_mask));
+            }
+        }
+        if (threadIdx.x < 4) {
+            const uint32_t page = page_of(st, threadIdx.x);
+            ks = page == ~0u ? 0.f : kv.k_scales[(size_t)page * kv.kv_heads + kvh];
+            vs = page == ~0u ? 0.f : kv.v_scales[(size_t)page * kv.kv_heads + kvh];
+        }
+    };
+    const auto store_step = [&](uint32_t st, uint32_t buf) {
+#pragma unroll
+        for (int i = 0; i < kPieces; i++) {
+            const uint32_t p = threadIdx.x + (uint32_t)i * kAttnThreads;
+            if (kStep * D / 16 % kAttnThreads != 0 && p >= kStep * D / 16) break;
+            const uint32_t key = p / (D / 16), at = (key & ~12u) | (key & 4u) << 1 | (key & 8u) >> 1;
+            f16x8_t *kd = (f16x8_t *)&sh_k[buf][at][p % (D / 16) * 16];
+            kd[0] = codes_f16(u32x2_t{kc[i][0], kc[i][1]});
+            kd[1] = codes_f16(u32x2_t{kc[i][2], kc[i][3]});
+            const int32_t have = sh.len - (int32_t)(st * kStep + p % 4 * 16);
+            if (have < 16) {  // bytes behind the last key may be anything
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int32_t b = have - 4 * j;
+                    vc[i][j] = b >= 4 ? vc[i][j] : (b <= 0 ? 0u : vc[i][j] & ~(~0u << (8 * b)));
+                }
+            }
+            f16x8_t *vd = (f16x8_t *)&sh_v[buf][p / 4][p % 4 * 16];
+            vd[0] = codes_f16(u32x2_t{vc[i][0], vc[i][1]});
+            vd[1] = codes_f16(u32x2_t{vc[i][2], vc[i][3]});
+        }
+        if (threadIdx.x < 4) {
+            // A hole's weights are 2^-inf of codes that are zeros.  A scale that is not a number makes its keys' scores NaN.
+            const bool hole = vs == 0.f, odd = !(vs == vs);
+            const int ev = odd || hole ? 0 : (int)(__builtin_bit_cast(uint32_t, vs) >> 23 & 0xFFu) - 127;
+            sh_s[buf][threadIdx.x][0] = odd ? __builtin_nanf("") : ks;
+            sh_s[buf][threadIdx.x][1] = hole ? -__builtin_inff() : (float)ev;
+            sh_s[buf][threadIdx.x][2] = hole ? 0.f : __builtin_bit_cast(float, (uint32_t)(127 - ev) << 23);
+        }
+    };
+
+    f32x16_t acc[NK];
+#pragma unroll
+    for (int i = 0; i < NK; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
+    float M = kNoMax, L = 0.f;
+    uint32_t buf = 0;
+    if (step < end) {
+        load_step(step);
+        store_step(step, 0);
+        if (step + 1 < end) load_step(step + 1);
+    }
+    for (; step < end; step++, buf ^= 1) {
+        __syncthreads();
+        if (step + 1 < end) store_step(step + 1, buf ^ 1);
+        if (step + 2 < end) load_step(step + 2);
+        const int32_t key0 = (int32_t)(step * kStep);
+        if (key0 > any_hi || key0 + (int32_t)kStep <= any_lo) continue;  // (no row of this wavefront sees the step)
+        f32x16_t S[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) S[t][j] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 2 * NK; k++) {
+                const f16x8_t ka = *(const f16x8_t *)&sh_k[buf][t * 32 + n][k * 16 + hi * 8];
+                S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qh[k], S[t], 0, 0, 0);
+                if constexpr (PAIRS) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, ql[k], S[t], 0, 0, 0);
+            }
+        }
+        // x[c]: the 8 scores of group c of 16 keys, keys 16 c + 8 hi + j; their logarithm (base 2) with the value scale: x a + e
+        float a[4], e[4], unscale[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) a[c] = factor * sh_s[buf][c][0], e[c] = sh_s[buf][c][1], unscale[c] = sh_s[buf][c][2];
+        const bool whole = key0 >= all_lo && key0 + (int32_t)kStep - 1 <= all_hi;
+        if (CAP || !whole) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    float x = S[c / 2][c % 2 * 8 + j] * a[c];
+                    if constexpr (CAP) {
+                        // cap * tanh(s / cap) = cap - 2 cap / (exp(2 s / cap) + 1)
+                        const float z = __builtin_amdgcn_exp2f(x * (2.f * kLog2E / A.softcap));
+                        x = (A.softcap - 2.f * A.softcap * __builtin_amdgcn_rcpf(z + 1.f)) * kLog2E;
+                    }
+                    x += e[c];
+                    const int32_t key = key0 + c * 16 + (int32_t)hi * 8 + j;
+                    S[c / 2][c % 2 * 8 + j] = !whole && (key > key_hi || key < key_lo) ? -__builtin_inff() : x;
+                }
+                a[c] = 1.f, e[c] = 0.f;
+            }
+        }
+        float top = kNoMax;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            float m = S[c / 2][c % 2 * 8];
+#pragma unroll
+            for (int j = 1; j < 8; j++) m = fmaxf(m, S[c / 2][c % 2 * 8 + j]);
+            top = fmaxf(top, fmaf(m, a[c], e[c]));
+        }
+        if (__ballot(top > M + kSlack)) {
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float next = top > M + kSlack ? top : M;
+            const float f = __builtin_amdgcn_exp2f(M - next);
+            M = next;
+            L *= f;
+#pragma unroll
+            for (int i = 0; i < NK; i++) acc[i] *= f;
+        }
+        f16x8_t ph[4], pl[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const float shift = e[c] - M + kBias;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const f32x2_t p = {__builtin_amdgcn_exp2f(fmaf(S[c / 2][c % 2 * 8 + j], a[c], shift)),
+                                   __builtin_amdgcn_exp2f(fmaf(S[c / 2][c % 2 * 8 + j + 1], a[c], shift))};
+                sum += p[0] + p[1];
+                weights_f16<PAIRS>(p, ph[c], pl[c], j);
+            }
+            L = fmaf(sum, unscale[c], L);
+        }
+#pragma unroll
+        for (int d = 0; d < NK; d++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const f16x8_t va = *(const f16x8_t *)&sh_v[buf][d * 32 + n][c * 16 + hi * 8];
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[c], acc[d], 0, 0, 0);
+                if constexpr (PAIRS) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[c], acc[d], 0, 0, 0);
+            }
+    }
+    L += __shfl_xor(L, 32, 64);
+    if (!live) return;
+    // acc[d][4 i + j]: channel 32 d + 8 i + 4 hi + j
+    if (it.pieces > 1) {
+        const size_t at = ((size_t)kvh * part.slots + it.slot + it.piece) * kTilesTile + wave * 32 + n;
+        if (hi == 0) part.ml[2 * at] = M, part.ml[2 * at + 1] = L;
+#pragma unroll
+        for (int d = 0; d < NK; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *(f32x4_t *)(part.acc + at * D + d * 32 + i * 8 + hi * 4) = f32x4_t{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+        return;
+    }
+    const float inv = inverse_sum(A, L, M, head);
+#pragma unroll
+    for (int d = 0; d < NK; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float v[4] = {acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv, acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv};
+            store4(A.out, A.out_type, (size_t)(sh.row + tok) * A.out_stride + (size_t)head * D + d * 32 + i * 8 + hi * 4, v);
+        }
+}
+
+// The pieces of split rows as one: a workgroup for each query row of a split tile, its
 // wavefronts a quarter of the pieces each.
-__global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttentionArgs A, Partials part, uint32_t items_per_head) {
+__global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttentionArgs A, Plan P, Partials part) {
     __shared__ float sh_acc[kAttnWaves][256], sh_ml[kAttnWaves][2];
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, D = A.kv.head_dim;
     const uint32_t kvh = blockIdx.y, group = A.q_heads / A.kv.kv_heads, r = blockIdx.z;
     Item it;
-    uint32_t first_item;
-    if (!find_item(A, blockIdx.x, true, it, first_item) || it.pieces < 2) return;
-    const Share sh = share_of(A, it.s, group);
-    const uint32_t q = it.tile * kTile + r;
+    if (!find_item(A, P, blockIdx.x, true, it)) return;
+    const Share sh = share_of(A, P, it.s, group);
+    const uint32_t q = (P.tile == kTilesTile ? sh.tiles - 1 - it.tile : it.tile) * P.tile + r;
     if (q >= sh.n * group) return;
-    const size_t at = ((size_t)kvh * items_per_head + first_item) * kTile + r;  // row r of the first piece; the next kTile rows on
+    const size_t at = ((size_t)kvh * part.slots + it.slot) * P.tile + r;  // row r of the first piece; the next P.tile rows on
     float top = kNoMax, l = 0.f;
     f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
     const uint32_t dim = min(lane * 4, D - 4);
@@ -381,7 +673,7 @@ __global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttentionA
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {  // (beyond the last piece: the last once more, with no weight)
             const uint32_t p = p0 + i * kAttnWaves;
-            const size_t x = at + (size_t)min(p, it.pieces - 1) * kTile;
+            const size_t x = at + (size_t)min(p, it.pieces - 1) * P.tile;
             m[i] = p < it.pieces ? part.ml[2 * x] : kNoMax;
             s[i] = part.ml[2 * x + 1];
             a[i] = *(const f32x4_t *)(part.acc + x * D + dim);
@@ -416,21 +708,37 @@ __global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttentionA
         o += *(const f32x4_t *)&sh_acc[w][lane * 4] * f;
     }
     const uint32_t h = kvh * group + q % group;
-    if (A.sinks && l != 0.f) l += __builtin_amdgcn_exp2f(A.sinks[h] * kLog2E - top + kBias);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = inverse_sum(A, l, top, h);
     const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     store4(A.out, A.out_type, (size_t)(sh.row + q / group) * A.out_stride + (size_t)h * D + lane * 4, v);
 }
 
-static size_t items_of(const AttentionArgs &A) { return (size_t)items_bound(A) * A.kv.kv_heads; }
-size_t attention_workspace_bytes(const AttentionArgs &A) { return items_of(A) * kTile * (A.kv.head_dim + 2) * sizeof(float) + 16; }
+// Partial results of one of the kernels, from `at` on.
+static Partials partials_of(const AttentionArgs &A, const Plan &P, float *at, float **end) {
+    const size_t rows = Plans::slots(P) * A.kv.kv_heads * P.tile;
+    *end = at + rows * (A.kv.head_dim + 2);
+    return {at, at + rows * A.kv.head_dim, (uint32_t)Plans::slots(P)};
+}
+static size_t partial_floats(const AttentionArgs &A, const Plan &P) { return Plans::slots(P) * A.kv.kv_heads * P.tile * (size_t)(A.kv.head_dim + 2); }
 
-int attention_launches(const AttentionArgs &) { return 2; }
+size_t attention_workspace_bytes(const AttentionArgs &A) {
+    const Plans p = plans_of(A);
+    return ((p.use_rows ? partial_floats(A, p.rows) : 0) + (p.use_tiles ? partial_floats(A, p.tiles) : 0)) * sizeof(float) + 16;
+}
+int attention_launches(const AttentionArgs &A) {
+    const Plans p = plans_of(A);
+    return (p.use_rows ? 1 + (int)p.rows.split : 0) + (p.use_tiles ? 1 + (int)p.tiles.split : 0);
+}
 
 template <int NK>
-static void launch_dim(hipStream_t s, const AttentionArgs &A, const Partials &part, dim3 grid) {
+static void launch_dim(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, bool tiles) {
     const bool pairs = A.out_type == ELEM_F32, cap = A.softcap > 0.f;
-#define LARQL_ATTN(P, C) hipLaunchKernelGGL((attention_rows_kernel<NK, P, C>), grid, dim3(kAttnThreads), 0, s, A, part)
+    const uint32_t items = (uint32_t)Plans::items(A, P);
+#define LARQL_ATTN(PR, C)                                                                                                             \
+    do {                                                                                                                              \
+        if (tiles) hipLaunchKernelGGL((attention_tiles_kernel<NK, PR, C>), dim3(items * A.kv.kv_heads), dim3(kAttnThreads), 0, s, A, P, part); \
+        else hipLaunchKernelGGL((attention_rows_kernel<NK, PR, C>), dim3(items, A.kv.kv_heads), dim3(kAttnThreads), 0, s, A, P, part);  \
+    } while (0)
     if (pairs && cap) LARQL_ATTN(true, true);
     else if (pairs) LARQL_ATTN(true, false);
     else if (cap) LARQL_ATTN(false, true);
@@ -438,27 +746,39 @@ static void launch_dim(hipStream_t s, const AttentionArgs &A, const Partials &pa
 #undef LARQL_ATTN
 }
 
-hipError_t attention_launch(hipStream_t s, const AttentionArgs &A, void *workspace) {
-    if (A.kv.tokens == 0 || A.kv.sequences == 0) return hipSuccess;
-    const uint64_t items = items_bound(A);
-    if (items > 0x7FFFFFFFull) return hipErrorInvalidValue;
-    const Partials part{(float *)workspace, (float *)workspace + items_of(A) * kTile * A.kv.head_dim};
-    const dim3 grid((uint32_t)items, A.kv.kv_heads);
+static hipError_t launch_plan(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, bool tiles) {
+    if (Plans::items(A, P) * A.kv.kv_heads > 0x7FFFFFFFull) return hipErrorInvalidValue;
     switch (A.kv.head_dim / 32) {
-    case 1: launch_dim<1>(s, A, part, grid); break;
-    case 2: launch_dim<2>(s, A, part, grid); break;
-    case 3: launch_dim<3>(s, A, part, grid); break;
-    case 4: launch_dim<4>(s, A, part, grid); break;
-    case 5: launch_dim<5>(s, A, part, grid); break;
-    case 6: launch_dim<6>(s, A, part, grid); break;
-    case 7: launch_dim<7>(s, A, part, grid); break;
-    case 8: launch_dim<8>(s, A, part, grid); break;
+    case 1: launch_dim<1>(s, A, P, part, tiles); break;
+    case 2: launch_dim<2>(s, A, P, part, tiles); break;
+    case 3: launch_dim<3>(s, A, P, part, tiles); break;
+    case 4: launch_dim<4>(s, A, P, part, tiles); break;
+    case 5: launch_dim<5>(s, A, P, part, tiles); break;
+    case 6: launch_dim<6>(s, A, P, part, tiles); break;
+    case 7: launch_dim<7>(s, A, P, part, tiles); break;
+    case 8: launch_dim<8>(s, A, P, part, tiles); break;
     default: return hipErrorInvalidValue;
     }
-    const uint64_t group = A.q_heads / A.kv.kv_heads, tiles = A.kv.tokens * group / kTile + A.kv.sequences;
-    const uint32_t join_rows = (uint32_t)std::min<uint64_t>(A.kv.max_new * group, kTile);
-    hipLaunchKernelGGL(attention_join_kernel, dim3((uint32_t)tiles, A.kv.kv_heads, join_rows), dim3(kAttnThreads), 0, s, A, part, (uint32_t)items);
+    if (P.split) {
+        const uint32_t rows = (uint32_t)std::min<uint64_t>((uint64_t)A.kv.max_new * (A.q_heads / A.kv.kv_heads), P.tile);
+        hipLaunchKernelGGL(attention_join_kernel, dim3((uint32_t)Plans::split_tiles(P), A.kv.kv_heads, rows), dim3(kAttnThreads), 0, s, A, P, part);
+    }
     return hipGetLastError();
+}
+
+hipError_t attention_launch(hipStream_t s, const AttentionArgs &A, void *workspace) {
+    const Plans p = plans_of(A);
+    float *at = (float *)workspace;
+    hipError_t e = hipSuccess;
+    if (p.use_tiles) {
+        const Partials part = partials_of(A, p.tiles, at, &at);
+        e = launch_plan(s, A, p.tiles, part, true);
+    }
+    if (p.use_rows && e == hipSuccess) {
+        const Partials part = partials_of(A, p.rows, at, &at);
+        e = launch_plan(s, A, p.rows, part, false);
+    }
+    return e;
 }
 
 }  // namespace larql
