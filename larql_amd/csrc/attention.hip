@@ -478,31 +478,30 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
     // Staging: a piece is 16 channels of a key's row, or 16 keys of a value channel's.
     u32x4_t kc[kPieces], vc[kPieces];
     float ks = 0.f, vs = 0.f;
-    const auto page_of = [&](uint32_t st, uint32_t grp) -> uint32_t {
-        const uint32_t key = st * kStep + grp * 16;
+    // The pages of a step, that of group lane % 4 in a lane: read one step before its codes.
+    const auto pages_of = [&](uint32_t st) -> uint32_t {
+        const uint32_t key = st * kStep + lane % 4 * 16;
         return st >= end || (int32_t)key >= sh.len ? ~0u : kv_page(kv, table, key);
     };
-    const auto load_step = [&](uint32_t st) {
+    const auto load_step = [&](uint32_t st, uint32_t pages) {
+        const uint32_t page_v = (uint32_t)__shfl((int)pages, (int)(threadIdx.x % 4), 64);
 #pragma unroll
         for (int i = 0; i < kPieces; i++) {
-            const uint32_t p = threadIdx.x + (uint32_t)i * kAttnThreads;
+            const uint32_t p = threadIdx.x + (uint32_t)i * kAttnThreads, key = p / (D / 16);
+            const uint32_t page = (uint32_t)__shfl((int)pages, (int)(key / 16), 64);
             if (kStep * D / 16 % kAttnThreads != 0 && p >= kStep * D / 16) break;
-            const uint32_t key = p / (D / 16), page = page_of(st, key / 16);
             kc[i] = u32x4_t{0u, 0u, 0u, 0u};
             if (page != ~0u)
                 kc[i] = *(const u32x4_t *)(kv.k_codes + ((size_t)page * kv.kv_heads + kvh) * head_codes + (size_t)((st * kStep + key) & page_mask) * D +
                                            p % (D / 16) * 16);
-            const uint32_t d = p / 4, grp = p % 4, page_v = page_of(st, grp);
             vc[i] = u32x4_t{0u, 0u, 0u, 0u};
-            if (page_v != ~0u) {
-                vc[i] = *(const u32x4_t *)(kv.v_codes + ((size_t)page_v * kv.kv_heads + kvh) * head_codes + ((size_t)d << kv.page_shift) +
-                                           ((st * kStep + grp * 16) & page_mask));
-            }
+            if (page_v != ~0u)
+                vc[i] = *(const u32x4_t *)(kv.v_codes + ((size_t)page_v * kv.kv_heads + kvh) * head_codes + ((size_t)(p / 4) << kv.page_shift) +
+                                           ((st * kStep + p % 4 * 16) & page_mask));
         }
         if (threadIdx.x < 4) {
-            const uint32_t page = page_of(st, threadIdx.x);
-            ks = page == ~0u ? 0.f : kv.k_scales[(size_t)page * kv.kv_heads + kvh];
-            vs = page == ~0u ? 0.f : kv.v_scales[(size_t)page * kv.kv_heads + kvh];
+            ks = pages == ~0u ? 0.f : kv.k_scales[(size_t)pages * kv.kv_heads + kvh];
+            vs = pages == ~0u ? 0.f : kv.v_scales[(size_t)pages * kv.kv_heads + kvh];
         }
     };
     const auto store_step = [&](uint32_t st, uint32_t buf) {
@@ -543,15 +542,21 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
         for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
     float M = kNoMax, L = 0.f;
     uint32_t buf = 0;
+    uint32_t pages = ~0u;
     if (step < end) {
-        load_step(step);
+        const uint32_t pages0 = pages_of(step), pages1 = pages_of(step + 1);
+        pages = pages_of(step + 2);
+        load_step(step, pages0);
         store_step(step, 0);
-        if (step + 1 < end) load_step(step + 1);
+        if (step + 1 < end) load_step(step + 1, pages1);
     }
     for (; step < end; step++, buf ^= 1) {
         __syncthreads();
         if (step + 1 < end) store_step(step + 1, buf ^ 1);
-        if (step + 2 < end) load_step(step + 2);
+        if (step + 2 < end) {
+            load_step(step + 2, pages);
+            pages = pages_of(step + 3);
+        }
         const int32_t key0 = (int32_t)(step * kStep);
         if (key0 > any_hi || key0 + (int32_t)kStep <= any_lo) continue;  // (no row of this wavefront sees the step)
         f32x16_t S[2];
@@ -652,29 +657,19 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
         }
 }
 
-// The pieces of split rows as one: a workgroup for each query row of a split tile, its
-// wavefronts a quarter of the pieces each.
-__global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttentionArgs A, Plan P, Partials part) {
-    __shared__ float sh_acc[kAttnWaves][256], sh_ml[kAttnWaves][2];
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, D = A.kv.head_dim;
-    const uint32_t kvh = blockIdx.y, group = A.q_heads / A.kv.kv_heads, r = blockIdx.z;
-    Item it;
-    if (!find_item(A, P, blockIdx.x, true, it)) return;
-    const Share sh = share_of(A, P, it.s, group);
-    const uint32_t q = (P.tile == kTilesTile ? sh.tiles - 1 - it.tile : it.tile) * P.tile + r;
-    if (q >= sh.n * group) return;
-    const size_t at = ((size_t)kvh * part.slots + it.slot) * P.tile + r;  // row r of the first piece; the next P.tile rows on
-    float top = kNoMax, l = 0.f;
-    f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const uint32_t dim = min(lane * 4, D - 4);
-    for (uint32_t p0 = wave; p0 < it.pieces; p0 += 8 * kAttnWaves) {
+// One query row of a split tile: pieces p0, p0 + step, ... as one sum.  `at`: the row in the first piece.
+__device__ __forceinline__ void join_pieces(const Partials &part, uint32_t tile, uint32_t D, size_t at, uint32_t pieces, uint32_t p0, uint32_t step, uint32_t dim,
+                                            float &top, float &l, f32x4_t &o) {
+    top = kNoMax, l = 0.f;
+    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (; p0 < pieces; p0 += 8 * step) {
         float m[8], s[8];
         f32x4_t a[8];
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {  // (beyond the last piece: the last once more, with no weight)
-            const uint32_t p = p0 + i * kAttnWaves;
-            const size_t x = at + (size_t)min(p, it.pieces - 1) * P.tile;
-            m[i] = p < it.pieces ? part.ml[2 * x] : kNoMax;
+            const uint32_t p = p0 + i * step;
+            const size_t x = at + (size_t)min(p, pieces - 1) * tile;
+            m[i] = p < pieces ? part.ml[2 * x] : kNoMax;
             s[i] = part.ml[2 * x + 1];
             a[i] = *(const f32x4_t *)(part.acc + x * D + dim);
         }
@@ -687,30 +682,60 @@ __global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttentionA
         top = next;
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
-            if (p0 + i * kAttnWaves >= it.pieces) break;
+            if (p0 + i * step >= pieces) break;
             const float w = __builtin_amdgcn_exp2f(m[i] - top);
             l = fmaf(w, s[i], l);
             o += a[i] * w;
         }
     }
-    if (lane == 0) sh_ml[wave][0] = top, sh_ml[wave][1] = l;
-    if (lane * 4 < D) *(f32x4_t *)&sh_acc[wave][lane * 4] = o;
-    __syncthreads();
-    if (wave || lane * 4 >= D) return;
+}
+
+// The pieces of split rows as one.  FEW: a workgroup for each query row of a split tile, its wavefronts a quarter of the pieces each;
+// otherwise a wavefront for a row, kJoinRows rows a workgroup.
+constexpr uint32_t kJoinRows = 16;
+template <bool FEW>
+__global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttentionArgs A, Plan P, Partials part) {
+    __shared__ float sh_acc[FEW ? kAttnWaves : 1][256], sh_ml[kAttnWaves][2];
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, D = A.kv.head_dim, dim = min(lane * 4, D - 4);
+    const uint32_t kvh = blockIdx.y, group = A.q_heads / A.kv.kv_heads;
+    Item it;
+    if (!find_item(A, P, blockIdx.x, true, it)) return;
+    const Share sh = share_of(A, P, it.s, group);
+    const uint32_t row0 = (FEW ? it.tile : sh.tiles - 1 - it.tile) * P.tile, rows = sh.n * group;
+    const size_t at = ((size_t)kvh * part.slots + it.slot) * P.tile;
+    const auto put = [&](uint32_t q, float top, float l, const f32x4_t &o) {
+        const uint32_t h = kvh * group + q % group;
+        const float inv = inverse_sum(A, l, top, h);
+        const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+        if (lane * 4 < D) store4(A.out, A.out_type, (size_t)(sh.row + q / group) * A.out_stride + (size_t)h * D + lane * 4, v);
+    };
+    float top, l;
+    f32x4_t o;
+    if constexpr (!FEW) {
+        for (uint32_t r = blockIdx.z * kJoinRows + wave; r < (blockIdx.z + 1) * kJoinRows && row0 + r < rows; r += kAttnWaves) {
+            join_pieces(part, P.tile, D, at + r, it.pieces, 0, 1, dim, top, l, o);
+            put(row0 + r, top, l, o);
+        }
+    } else {
+        const uint32_t r = blockIdx.z;
+        if (row0 + r >= rows) return;
+        join_pieces(part, P.tile, D, at + r, it.pieces, wave, kAttnWaves, dim, top, l, o);
+        if (lane == 0) sh_ml[wave][0] = top, sh_ml[wave][1] = l;
+        if (lane * 4 < D) *(f32x4_t *)&sh_acc[wave][lane * 4] = o;
+        __syncthreads();
+        if (wave) return;
 #pragma unroll
-    for (uint32_t w = 1; w < kAttnWaves; w++) top = fmaxf(top, sh_ml[w][0]);
-    l = 0.f;
-    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (uint32_t w = 1; w < kAttnWaves; w++) top = fmaxf(top, sh_ml[w][0]);
+        l = 0.f;
+        o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (uint32_t w = 0; w < kAttnWaves; w++) {
-        const float f = __builtin_amdgcn_exp2f(sh_ml[w][0] - top);
-        l = fmaf(f, sh_ml[w][1], l);
-        o += *(const f32x4_t *)&sh_acc[w][lane * 4] * f;
+        for (uint32_t w = 0; w < kAttnWaves; w++) {
+            const float f = __builtin_amdgcn_exp2f(sh_ml[w][0] - top);
+            l = fmaf(f, sh_ml[w][1], l);
+            o += *(const f32x4_t *)&sh_acc[w][dim] * f;
+        }
+        put(row0 + r, top, l, o);
     }
-    const uint32_t h = kvh * group + q % group;
-    const float inv = inverse_sum(A, l, top, h);
-    const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-    store4(A.out, A.out_type, (size_t)(sh.row + q / group) * A.out_stride + (size_t)h * D + lane * 4, v);
 }
 
 // Partial results of one of the kernels, from `at` on.
@@ -761,7 +786,9 @@ static hipError_t launch_plan(hipStream_t s, const AttentionArgs &A, const Plan 
     }
     if (P.split) {
         const uint32_t rows = (uint32_t)std::min<uint64_t>((uint64_t)A.kv.max_new * (A.q_heads / A.kv.kv_heads), P.tile);
-        hipLaunchKernelGGL(attention_join_kernel, dim3((uint32_t)Plans::split_tiles(P), A.kv.kv_heads, rows), dim3(kAttnThreads), 0, s, A, P, part);
+        const uint32_t split = (uint32_t)Plans::split_tiles(P);
+        if (tiles) hipLaunchKernelGGL(attention_join_kernel<false>, dim3(split, A.kv.kv_heads, (rows + kJoinRows - 1) / kJoinRows), dim3(kAttnThreads), 0, s, A, P, part);
+        else hipLaunchKernelGGL(attention_join_kernel<true>, dim3(split, A.kv.kv_heads, rows), dim3(kAttnThreads), 0, s, A, P, part);
     }
     return hipGetLastError();
 }
