@@ -360,8 +360,8 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_rows_k
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
             const f32x2_t p = {__builtin_amdgcn_exp2f(x[i] - M + kBias), __builtin_amdgcn_exp2f(x[i + 1] - M + kBias)};
-            sum += p[0] + p[1];
             weights_f16<PAIRS>(p, ph[i / 8], pl[i / 8], i % 8);
+            sum += p[0] + p[1];
         }
         L = fmaf(sum, unscale, L);
 #pragma unroll
@@ -483,21 +483,23 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
         const uint32_t key = st * kStep + lane % 4 * 16;
         return st >= end || (int32_t)key >= sh.len ? ~0u : kv_page(kv, table, key);
     };
+    // A thread's pieces: where they lie in a page (a page of 128 holds two steps), their groups' lanes.
+    const uint32_t page_bytes = (uint32_t)(kv.kv_heads * head_codes);
+    const uint8_t *k_head = kv.k_codes + kvh * head_codes, *v_head = kv.v_codes + kvh * head_codes;
+    uint32_t odd_pages = 0;  // lanes whose page (of the step in kc, vc) is a hole
     const auto load_step = [&](uint32_t st, uint32_t pages) {
-        const uint32_t page_v = (uint32_t)__shfl((int)pages, (int)(threadIdx.x % 4), 64);
+        const uint32_t in_page = (st * kStep) & page_mask;
+        odd_pages = (uint32_t)__ballot(pages == ~0u) & 15u;
+        const uint32_t safe = pages == ~0u ? 0u : pages;
+        const uint8_t *vp = v_head + (uint64_t)(uint32_t)__shfl((int)safe, (int)(threadIdx.x % 4), 64) * page_bytes +
+                            (((threadIdx.x / 4) << kv.page_shift) + in_page + ((threadIdx.x % 4 * 16) & page_mask));
 #pragma unroll
         for (int i = 0; i < kPieces; i++) {
             const uint32_t p = threadIdx.x + (uint32_t)i * kAttnThreads, key = p / (D / 16);
-            const uint32_t page = (uint32_t)__shfl((int)pages, (int)(key / 16), 64);
+            const uint32_t page = (uint32_t)__shfl((int)safe, (int)(key / 16 % 4), 64);
             if (kStep * D / 16 % kAttnThreads != 0 && p >= kStep * D / 16) break;
-            kc[i] = u32x4_t{0u, 0u, 0u, 0u};
-            if (page != ~0u)
-                kc[i] = *(const u32x4_t *)(kv.k_codes + ((size_t)page * kv.kv_heads + kvh) * head_codes + (size_t)((st * kStep + key) & page_mask) * D +
-                                           p % (D / 16) * 16);
-            vc[i] = u32x4_t{0u, 0u, 0u, 0u};
-            if (page_v != ~0u)
-                vc[i] = *(const u32x4_t *)(kv.v_codes + ((size_t)page_v * kv.kv_heads + kvh) * head_codes + ((size_t)(p / 4) << kv.page_shift) +
-                                           ((st * kStep + p % 4 * 16) & page_mask));
+            kc[i] = *(const u32x4_t *)(k_head + (uint64_t)page * page_bytes + ((in_page + (key & page_mask)) * D + p % (D / 16) * 16));
+            vc[i] = *(const u32x4_t *)(vp + ((size_t)(i * kAttnThreads / 4) << kv.page_shift));
         }
         if (threadIdx.x < 4) {
             ks = pages == ~0u ? 0.f : kv.k_scales[(size_t)pages * kv.kv_heads + kvh];
@@ -505,6 +507,19 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
         }
     };
     const auto store_step = [&](uint32_t st, uint32_t buf) {
+        if ((int32_t)(st * kStep + kStep) > sh.len || odd_pages) {  // codes behind the last key and in holes may be anything: they count as zeros
+#pragma unroll
+            for (int i = 0; i < kPieces; i++) {
+                const uint32_t p = threadIdx.x + (uint32_t)i * kAttnThreads, key = p / (D / 16);
+                if ((int32_t)(st * kStep + key) >= sh.len || (odd_pages >> (key / 16 % 4) & 1u)) kc[i] = u32x4_t{0u, 0u, 0u, 0u};
+                const int32_t have = odd_pages >> (p % 4) & 1u ? 0 : sh.len - (int32_t)(st * kStep + p % 4 * 16);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int32_t b = have - 4 * j;
+                    vc[i][j] = b >= 4 ? vc[i][j] : (b <= 0 ? 0u : vc[i][j] & ~(~0u << (8 * b)));
+                }
+            }
+        }
 #pragma unroll
         for (int i = 0; i < kPieces; i++) {
             const uint32_t p = threadIdx.x + (uint32_t)i * kAttnThreads;
@@ -513,14 +528,6 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
             f16x8_t *kd = (f16x8_t *)&sh_k[buf][at][p % (D / 16) * 16];
             kd[0] = codes_f16(u32x2_t{kc[i][0], kc[i][1]});
             kd[1] = codes_f16(u32x2_t{kc[i][2], kc[i][3]});
-            const int32_t have = sh.len - (int32_t)(st * kStep + p % 4 * 16);
-            if (have < 16) {  // bytes behind the last key may be anything
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int32_t b = have - 4 * j;
-                    vc[i][j] = b >= 4 ? vc[i][j] : (b <= 0 ? 0u : vc[i][j] & ~(~0u << (8 * b)));
-                }
-            }
             f16x8_t *vd = (f16x8_t *)&sh_v[buf][p / 4][p % 4 * 16];
             vd[0] = codes_f16(u32x2_t{vc[i][0], vc[i][1]});
             vd[1] = codes_f16(u32x2_t{vc[i][2], vc[i][3]});
@@ -559,18 +566,20 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
         }
         const int32_t key0 = (int32_t)(step * kStep);
         if (key0 > any_hi || key0 + (int32_t)kStep <= any_lo) continue;  // (no row of this wavefront sees the step)
-        f32x16_t S[2];
+        f32x16_t S[2], zero;
+#pragma unroll
+        for (int j = 0; j < 16; j++) zero[j] = 0.f;
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int t = 0; t < 2; t++) {
 #pragma unroll
-            for (int j = 0; j < 16; j++) S[t][j] = 0.f;
-#pragma unroll
             for (int k = 0; k < 2 * NK; k++) {
                 const f16x8_t ka = *(const f16x8_t *)&sh_k[buf][t * 32 + n][k * 16 + hi * 8];
-                S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qh[k], S[t], 0, 0, 0);
+                S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qh[k], k ? S[t] : zero, 0, 0, 0);
                 if constexpr (PAIRS) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, ql[k], S[t], 0, 0, 0);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         // x[c]: the 8 scores of group c of 16 keys, keys 16 c + 8 hi + j; their logarithm (base 2) with the value scale: x a + e
         float a[4], e[4], unscale[4];
 #pragma unroll
@@ -620,11 +629,12 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
             for (int j = 0; j < 8; j += 2) {
                 const f32x2_t p = {__builtin_amdgcn_exp2f(fmaf(S[c / 2][c % 2 * 8 + j], a[c], shift)),
                                    __builtin_amdgcn_exp2f(fmaf(S[c / 2][c % 2 * 8 + j + 1], a[c], shift))};
-                sum += p[0] + p[1];
                 weights_f16<PAIRS>(p, ph[c], pl[c], j);
+                sum += p[0] + p[1];  // (the f32 weights: one of a block of small values may be nothing in f16, and counts here)
             }
             L = fmaf(sum, unscale[c], L);
         }
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int d = 0; d < NK; d++)
 #pragma unroll
@@ -633,6 +643,7 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
                 acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[c], acc[d], 0, 0, 0);
                 if constexpr (PAIRS) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[c], acc[d], 0, 0, 0);
             }
+        __builtin_amdgcn_s_setprio(0);
     }
     L += __shfl_xor(L, 32, 64);
     if (!live) return;
