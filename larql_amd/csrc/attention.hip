@@ -25,7 +25,7 @@ constexpr uint32_t kStep = 64;          // keys of a step
 constexpr uint32_t kAttnThreads = 256;
 constexpr uint32_t kAttnWaves = kAttnThreads / 64;
 constexpr uint32_t kRowsTile = 16;      // query rows of a workgroup of the kernel for few rows
-constexpr uint32_t kTilesTile = 128;    // ... for many
+constexpr uint32_t kTilesTile = 128;    // ... for many, 32 a wavefront
 constexpr uint32_t kFewRows = 32;       // a sequence with at most this many rows for each key/value head goes through the former
 constexpr float kLog2E = 1.44269504088896341f;
 // Weights are held as 2^(t + e - M + 12) with t + e - M <= 3, so that the f16 pair of an f32 weight keeps 22 bits down to 2^-15 of the
@@ -117,7 +117,9 @@ struct Plans {
         return A.kv.tokens * (uint64_t)(A.q_heads / A.kv.kv_heads) / P.tile + A.kv.sequences + (P.split ? P.target + 1 : 0);
     }
     static uint64_t slots(const Plan &P) { return P.split ? 2 * P.target + 2 : 0; }
-    static uint64_t split_tiles(const Plan &P) { return P.split ? P.target + 1 : 0; }
+    static uint64_t split_tiles(const AttentionArgs &A, const Plan &P) {
+        return P.split ? std::min<uint64_t>(P.target + 1, A.kv.tokens * (uint64_t)(A.q_heads / A.kv.kv_heads) / P.tile + A.kv.sequences) : 0;
+    }
 };
 static Plans plans_of(const AttentionArgs &A) {
     const uint64_t group = A.q_heads / A.kv.kv_heads, most = A.kv.max_new * group;
@@ -127,7 +129,7 @@ static Plans plans_of(const AttentionArgs &A) {
     p.rows = {kRowsTile, 1, kFewRows, std::max(2 * cus * per_cu / A.kv.kv_heads, 1u), 4, 1};
     p.rows.split = steps > p.rows.min_steps;
     p.tiles = {kTilesTile, kFewRows + 1, 0xFFFFFFFFu, std::max(cus * per_cu / A.kv.kv_heads, 1u), 8, 1};
-    p.tiles.split = steps > p.tiles.min_steps && A.kv.tokens * group / kTilesTile + A.kv.sequences < p.tiles.target;
+    p.tiles.split = steps > p.tiles.min_steps && A.kv.tokens * group / p.tiles.tile + A.kv.sequences < p.tiles.target;
     p.use_tiles = most > kFewRows;
     p.use_rows = !p.use_tiles || A.kv.sequences > 1;
     if (!p.use_rows) p.tiles.rows_min = 1;  // one sequence: one kernel, whatever its number of new tokens turns out to be
@@ -168,6 +170,15 @@ __device__ __forceinline__ float inverse_sum(const AttentionArgs &A, float l, fl
     return l == 0.f ? 0.f : 1.f / l;
 }
 
+// The logarithm (base 2) of a score's weight, plus e: s a + e, or with the cap on s a (natural units) in between.
+template <bool CAP>
+__device__ __forceinline__ float score(const AttentionArgs &A, float s, float a, float e) {
+    if constexpr (!CAP) return fmaf(s, a, e);
+    // cap * tanh(s / cap) = cap - 2 cap / (exp(2 s / cap) + 1)
+    const float z = __builtin_amdgcn_exp2f(s * a * (2.f * kLog2E / A.softcap));
+    return fmaf(A.softcap - 2.f * A.softcap * __builtin_amdgcn_rcpf(z + 1.f), kLog2E, e);
+}
+
 // A query row's elements (spread over lanes 32 apart, and 16 apart where QUARTERS) as f16 or f16 pairs after a power-of-two scale that brings
 // the largest to [2^14, 2^15); returns what scores are multiplied by.  A row that is not finite gets NaN there.
 template <int N, bool PAIRS, bool CAP, bool QUARTERS>
@@ -196,144 +207,150 @@ __device__ __forceinline__ float query_f16(const AttentionArgs &A, const float (
     return finite ? factor : __builtin_nanf("");
 }
 
+// ---- few query rows --------------------------------------------------------------------------------------------------
+//
+// 16 query rows a workgroup, as the columns of v_mfma_f32_16x16x32_f16; its wavefronts take steps of 64 keys in turn and add up at the
+// end.  A wavefront reads its step's codes straight into the registers that the matrix instructions' operands are converted
+// from, 64 x head_dim bytes of K and then of V through ONE set of registers: as a part of the keys is multiplied its registers take a part
+// of the step's values, and as that is multiplied a part of the next step's keys, so about 64 x head_dim bytes are always in flight and
+// two wavefronts fit a SIMD at every head_dim.  The queries' operands are read from LDS.
 template <int NK, bool PAIRS, bool CAP>
-__global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_rows_kernel(AttentionArgs A, Plan P, Partials part) {
+__global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(AttentionArgs A, Plan P, Partials part) {
     constexpr uint32_t D = NK * 32, kPad = D + 4;
-    __shared__ float sh_acc[kAttnWaves][kRowsTile][kPad];
-    __shared__ float sh_ml[kAttnWaves][kRowsTile][2];
+    constexpr int NP = (NK + 1) / 2;  // parts: 64 channels of the keys, 64 channels of the values
+    struct Queries {
+        f16x8_t q[PAIRS ? 2 : 1][NK][64];
+        float factor[16];
+    };
+    struct Sums {
+        float acc[kAttnWaves][kRowsTile][kPad], ml[kAttnWaves][kRowsTile][2];
+    };
+    __shared__ __align__(16) char shared[sizeof(Queries) > sizeof(Sums) ? sizeof(Queries) : sizeof(Sums)];
+    Queries &sq = *(Queries *)shared;
+    Sums &ss = *(Sums *)shared;
     const KvArgs &kv = A.kv;
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = lane % 16, g = lane / 16;
     const uint32_t kvh = blockIdx.y, group = A.q_heads / kv.kv_heads;
     Item it;
     if (!find_item(A, P, blockIdx.x, false, it)) return;
     const Share sh = share_of(A, P, it.s, group);
+    const uint32_t rows = sh.n * group;
 
-    // The lane's query row: token and head, what it sees, its elements as f16 after a power-of-two scale.
-    const uint32_t row = it.tile * kRowsTile + n, tok = row / group, head = kvh * group + row % group;
-    const bool live = tok < sh.n;
-    const int32_t pos = sh.first + (int32_t)tok;
-    const int32_t key_hi = !live ? -1 : (A.causal ? min(pos, sh.len - 1) : sh.len - 1);
-    const int32_t key_lo = A.window ? (int32_t)max((int64_t)pos - (int64_t)A.window + 1, (int64_t)0) : 0;
-    f16x8_t qh[NK], ql[PAIRS ? NK : 1];
-    float factor;
-    {
+    // The lane's query row: token and head, what it sees.  What all and any of the rows see: the first and the last say it.
+    const uint32_t row0 = it.tile * kRowsTile, row = row0 + n, tok = row / group;
+    const bool live = row < rows;
+    const auto hi_of = [&](uint32_t r) { return A.causal ? min(sh.first + (int32_t)(r / group), sh.len - 1) : sh.len - 1; };
+    const auto lo_of = [&](uint32_t r) {
+        return A.window ? (int32_t)max((int64_t)sh.first + (int64_t)(r / group) - (int64_t)A.window + 1, (int64_t)0) : 0;
+    };
+    const int32_t key_hi = live ? hi_of(row) : -1, key_lo = lo_of(row);
+    const uint32_t last_row = min(row0 + kRowsTile - 1, rows - 1);
+    const int32_t all_hi = hi_of(row0), any_hi = hi_of(last_row), any_lo = lo_of(row0), all_lo = lo_of(last_row);
+
+    const uint64_t piece_lo = (uint64_t)sh.step_lo + (uint64_t)it.piece * it.chunk;
+    const uint32_t end = any_hi < 0 ? 0u : (uint32_t)min(min(piece_lo + it.chunk, (uint64_t)(sh.step_lo + sh.steps)), (uint64_t)((uint32_t)any_hi / kStep + 1));
+    uint32_t step = (uint32_t)max(piece_lo, (uint64_t)((uint32_t)any_lo / kStep)) + wave;
+
+    const int32_t *table = kv.block_table + (size_t)it.s * kv.table_width;
+    const uint32_t page_mask = (1u << kv.page_shift) - 1;
+    const size_t head_codes = (size_t)D << kv.page_shift;
+    const uint8_t *k_head = kv.k_codes + kvh * head_codes, *v_head = kv.v_codes + kvh * head_codes;
+    const uint32_t page_bytes = (uint32_t)(kv.kv_heads * head_codes);
+    const uint32_t gk = n / 4;  // this lane loads keys of group gk, and values and weights of group g, of a step
+    const auto page_of = [&](uint32_t st, uint32_t grp) -> uint32_t {
+        const uint32_t key = st * kStep + grp * 16;
+        return st >= end || (int32_t)key >= sh.len ? ~0u : kv_page(kv, table, key);
+    };
+    u32x4_t ring[NP][4];
+    const auto load_keys = [&](const uint8_t *kp, int p) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const uint8_t *kr = kp + (uint32_t)(4 * t) * D + p * 64;
+            if (2 * p + 1 < NK) {
+                ring[p][t] = *(const u32x4_t *)(kr + g * 16);
+            } else {
+                const u32x2_t c = *(const u32x2_t *)(kr + g * 8);
+                ring[p][t] = u32x4_t{c[0], c[1], 0u, 0u};
+            }
+        }
+    };
+    const auto keys_at = [&](uint32_t st, uint32_t page) {
+        return k_head + (uint64_t)(page == ~0u ? 0u : page) * page_bytes + (((st * kStep + gk * 16) & page_mask) + n % 4) * D;
+    };
+    float ks = 0.f, vs = 1.f;
+    const auto load_scales = [&](uint32_t page) {
+        const size_t at = (size_t)(page == ~0u ? 0u : page) * kv.kv_heads + kvh;
+        ks = kv.k_scales[at];
+        vs = kv.v_scales[at];
+    };
+    uint32_t page_k = page_of(step, gk), page_v = page_of(step, g);
+    if (step < end) {
+        const uint8_t *kp = keys_at(step, page_k);
+#pragma unroll
+        for (int p = 0; p < NP; p++) load_keys(kp, p);
+        load_scales(page_v);
+    }
+    uint32_t next_k = page_of(step + kAttnWaves, gk), next_v = page_of(step + kAttnWaves, g);
+
+    // channel d of the lane's operand k: 64 channels of two operands lie in one 16-byte piece of a key's row
+    if (wave == 0) {
         float q[NK][8];
 #pragma unroll
         for (int k = 0; k < NK; k++) {
             const uint32_t d = (k | 1) < NK ? (uint32_t)(k & ~1) * 32 + g * 16 + (uint32_t)(k & 1) * 8 : (uint32_t)k * 32 + g * 8;
 #pragma unroll
             for (int i = 0; i < 8; i++) q[k][i] = 0.f;
-            if (live) load8(A.q, A.q_type, (size_t)(sh.row + tok) * A.q_stride + (size_t)head * D + d, q[k]);
+            if (live) load8(A.q, A.q_type, (size_t)(sh.row + tok) * A.q_stride + (size_t)(kvh * group + row % group) * D + d, q[k]);
         }
-        factor = query_f16<NK, PAIRS, CAP, true>(A, q, qh, ql);
-    }
-    // steps that every live row of the tile sees whole need no mask
-    int32_t all_hi = live ? key_hi : 0x7FFFFFFF, all_lo = live ? key_lo : 0;
-    int32_t any_hi = key_hi, any_lo = live ? key_lo : 0x7FFFFFFF;
+        f16x8_t qh[NK], ql[PAIRS ? NK : 1];
+        const float f = query_f16<NK, PAIRS, CAP, true>(A, q, qh, ql);
+        if (g == 0) sq.factor[n] = f;
 #pragma unroll
-    for (int m = 1; m < 16; m *= 2) {
-        all_hi = min(all_hi, __shfl_xor(all_hi, m, 64));
-        all_lo = max(all_lo, __shfl_xor(all_lo, m, 64));
-        any_hi = max(any_hi, __shfl_xor(any_hi, m, 64));
-        any_lo = min(any_lo, __shfl_xor(any_lo, m, 64));
+        for (int k = 0; k < NK; k++) {
+            sq.q[0][k][lane] = qh[k];
+            if constexpr (PAIRS) sq.q[PAIRS ? 1 : 0][k][lane] = ql[k];
+        }
     }
-    all_hi = __builtin_amdgcn_readfirstlane(all_hi), all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-    any_hi = __builtin_amdgcn_readfirstlane(any_hi), any_lo = __builtin_amdgcn_readfirstlane(any_lo);
+    __syncthreads();
+    const float factor = sq.factor[n];
 
-    const int32_t *table = kv.block_table + (size_t)it.s * kv.table_width;
-    const uint32_t page_mask = (1u << kv.page_shift) - 1;
-    const size_t head_codes = (size_t)D << kv.page_shift;
     f32x4_t acc[2 * NK];
 #pragma unroll
     for (int i = 0; i < 2 * NK; i++) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float M = kNoMax, L = 0.f;
-
-    // Steps of this piece that some row sees, every kAttnWaves-th of them this wavefront's.  A step's page numbers are read two steps
-    // ahead, its key codes one step ahead (while the step before multiplies values), its value codes while its scores form: a
-    // wavefront always has a load of its own 64 x head_dim bytes or more in flight.
-    const uint32_t step_end = any_hi < 0 ? 0u : min(min(sh.step_lo + (it.piece + 1) * it.chunk, sh.step_lo + sh.steps), (uint32_t)any_hi / kStep + 1);
-    uint32_t step = max(sh.step_lo + it.piece * it.chunk, any_lo == 0x7FFFFFFF ? step_end : (uint32_t)any_lo / kStep) + wave;
-    const uint32_t gk = n / 4;  // this lane loads keys of group gk, and values and weights of group g, of a step
-    const auto page_of = [&](uint32_t st, uint32_t grp) -> uint32_t {
-        const uint32_t key = st * kStep + grp * 16;
-        return st >= step_end || (int32_t)key >= sh.len ? ~0u : kv_page(kv, table, key);
-    };
-    u32x4_t kc[4][(NK + 1) / 2], vc[2 * NK];
-    float ks = 0.f, vs = 1.f;
-    const auto load_keys = [&](uint32_t st, uint32_t page_k, uint32_t page_v) {
-        const uint8_t *kp = kv.k_codes + ((size_t)(page_k == ~0u ? 0u : page_k) * kv.kv_heads + kvh) * head_codes +
-                            (size_t)((st * kStep + gk * 16) & page_mask) * D;
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int k = 0; k < NK; k += 2) {
-                const uint8_t *kr = kp + (size_t)(4 * t + n % 4) * D + k * 32;
-                if (k + 1 < NK) {
-                    kc[t][k / 2] = *(const u32x4_t *)(kr + g * 16);
-                } else {
-                    const u32x2_t c = *(const u32x2_t *)(kr + g * 8);
-                    kc[t][k / 2] = u32x4_t{c[0], c[1], 0u, 0u};
-                }
-            }
-        const size_t at = (size_t)(page_v == ~0u ? 0u : page_v) * kv.kv_heads + kvh;
-        ks = kv.k_scales[at];
-        vs = kv.v_scales[at];
-    };
-    uint32_t page_k = page_of(step, gk), page_v = page_of(step, g);
-    if (step < step_end) load_keys(step, page_k, page_v);
-    uint32_t next_k = page_of(step + kAttnWaves, gk), next_v = page_of(step + kAttnWaves, g);
-
-    for (; step < step_end; step += kAttnWaves) {
+    for (; step < end; step += kAttnWaves) {
         const int32_t key0 = (int32_t)(step * kStep);
         const bool hole = page_v == ~0u;
-        {
-            const uint8_t *vp = kv.v_codes + ((size_t)(hole ? 0u : page_v) * kv.kv_heads + kvh) * head_codes + (((uint32_t)key0 + g * 16) & page_mask);
-#pragma unroll
-            for (int d = 0; d < 2 * NK; d++) vc[d] = *(const u32x4_t *)(vp + ((size_t)(d * 16 + n) << kv.page_shift));
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t *vp = v_head + (uint64_t)(hole ? 0u : page_v) * page_bytes + ((n << kv.page_shift) + (((uint32_t)key0 + g * 16) & page_mask));
         f32x4_t S[4];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            S[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < NP; p++) {
 #pragma unroll
-            for (int k = 0; k < NK; k++) {
-                const u32x4_t c = kc[t][k / 2];
-                const f16x8_t ka = codes_f16(k % 2 ? u32x2_t{c[2], c[3]} : u32x2_t{c[0], c[1]});
-                S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[k], S[t], 0, 0, 0);
-                if constexpr (PAIRS) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[k], S[t], 0, 0, 0);
+            for (int k = 2 * p; k < (2 * p + 2 < NK ? 2 * p + 2 : NK); k++) {
+                const f16x8_t qh = sq.q[0][k][lane], ql = sq.q[PAIRS ? 1 : 0][k][lane];
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const u32x4_t c = ring[p][t];
+                    const f16x8_t ka = codes_f16(k % 2 ? u32x2_t{c[2], c[3]} : u32x2_t{c[0], c[1]});
+                    S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh, k ? S[t] : f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    if constexpr (PAIRS) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql, S[t], 0, 0, 0);
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 4 * p; d < (4 * p + 4 < 2 * NK ? 4 * p + 4 : 2 * NK); d++) ring[p][d % 4] = *(const u32x4_t *)(vp + ((size_t)(16 * d) << kv.page_shift));
+            __builtin_amdgcn_sched_barrier(0);
         }
-        float cur_ks = ks;
-        const float cur_vs = vs;
-        __builtin_amdgcn_sched_barrier(0);
-        page_k = next_k, page_v = next_v;
-        if (step + kAttnWaves < step_end) {
-            load_keys(step + kAttnWaves, page_k, page_v);
-            next_k = page_of(step + 2 * kAttnWaves, gk), next_v = page_of(step + 2 * kAttnWaves, g);
-        }
-        __builtin_amdgcn_sched_barrier(0);
         // Logarithms (base 2) of the weights times the value scale.  A scale that is not a number makes its tokens' scores NaN.
-        const bool odd = !(cur_vs == cur_vs);
-        if (odd) cur_ks = __builtin_nanf("");
-        const int ev = odd || hole ? 0 : (int)(__builtin_bit_cast(uint32_t, cur_vs) >> 23 & 0xFFu) - 127;
+        const bool odd = !(vs == vs);
+        const int ev = odd || hole ? 0 : (int)(__builtin_bit_cast(uint32_t, vs) >> 23 & 0xFFu) - 127;
         const float unscale = __builtin_bit_cast(float, (uint32_t)(127 - ev) << 23);
-        const float a = factor * cur_ks;
+        const float a = factor * (odd ? __builtin_nanf("") : ks);
         float x[16];
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float v;
-                if constexpr (CAP) {
-                    // cap * tanh(s / cap) = cap - 2 cap / (exp(2 s / cap) + 1)
-                    const float z = __builtin_amdgcn_exp2f(S[t][r] * a * (2.f * kLog2E / A.softcap));
-                    v = fmaf(A.softcap - 2.f * A.softcap / (z + 1.f), kLog2E, (float)ev);
-                } else {
-                    v = fmaf(S[t][r], a, (float)ev);
-                }
-                x[4 * t + r] = v;
-            }
+            for (int r = 0; r < 4; r++) x[4 * t + r] = score<CAP>(A, S[t][r], a, (float)ev);
         const bool plain = key0 >= all_lo && key0 + (int32_t)kStep - 1 <= all_hi && __ballot(hole) == 0;
         if (!plain) {
 #pragma unroll
@@ -361,50 +378,64 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_rows_k
         for (int i = 0; i < 16; i += 2) {
             const f32x2_t p = {__builtin_amdgcn_exp2f(x[i] - M + kBias), __builtin_amdgcn_exp2f(x[i + 1] - M + kBias)};
             weights_f16<PAIRS>(p, ph[i / 8], pl[i / 8], i % 8);
-            sum += p[0] + p[1];
+            sum += p[0] + p[1];  // (the f32 weights: one of a block of small values may be nothing in f16, and counts here)
         }
         L = fmaf(sum, unscale, L);
+        if (!plain) {  // bytes behind the last key may be anything
+            const int32_t have = hole ? 0 : sh.len - key0 - (int32_t)g * 16;
 #pragma unroll
-        for (int d = 0; d < 2 * NK; d++) {
-            u32x4_t c = vc[d];
-            if (!plain) {  // bytes behind the last key may be anything
-                const int32_t have = hole ? 0 : sh.len - key0 - (int32_t)g * 16;
+            for (int i = 0; i < 4; i++) {
+                const int32_t b = have - 4 * i;
+                const uint32_t keep = b >= 4 ? ~0u : (b <= 0 ? 0u : ~(~0u << (8 * b)));
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int32_t b = have - 4 * i;
-                    c[i] = b >= 4 ? c[i] : (b <= 0 ? 0u : c[i] & ~(~0u << (8 * b)));
+                for (int d = 0; d < 2 * NK; d++) ring[d / 4][d % 4][i] &= keep;
+            }
+        }
+        page_k = next_k, page_v = next_v;
+        const bool more = step + kAttnWaves < end;
+        const uint8_t *kp = keys_at(step + kAttnWaves, page_k);
+        if (more) {
+            load_scales(page_v);
+            next_k = page_of(step + 2 * kAttnWaves, gk), next_v = page_of(step + 2 * kAttnWaves, g);
+        }
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+#pragma unroll
+            for (int d = 4 * p; d < (4 * p + 4 < 2 * NK ? 4 * p + 4 : 2 * NK); d++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const u32x4_t c = ring[p][d % 4];
+                    const f16x8_t va = codes_f16(u32x2_t{c[2 * u], c[2 * u + 1]});
+                    acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[u], acc[d], 0, 0, 0);
+                    if constexpr (PAIRS) acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[u], acc[d], 0, 0, 0);
                 }
-            }
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const f16x8_t va = codes_f16(u32x2_t{c[2 * u], c[2 * u + 1]});
-                acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[u], acc[d], 0, 0, 0);
-                if constexpr (PAIRS) acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[u], acc[d], 0, 0, 0);
-            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) load_keys(kp, p);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
     // the wavefronts' sums as one
     L += __shfl_xor(L, 16, 64);
     L += __shfl_xor(L, 32, 64);
-    if (g == 0) sh_ml[wave][n][0] = M, sh_ml[wave][n][1] = L;
+    __syncthreads();  // (the sums lie where the queries did)
+    if (g == 0) ss.ml[wave][n][0] = M, ss.ml[wave][n][1] = L;
 #pragma unroll
-    for (int d = 0; d < 2 * NK; d++) *(f32x4_t *)&sh_acc[wave][n][d * 16 + g * 4] = acc[d];
+    for (int d = 0; d < 2 * NK; d++) *(f32x4_t *)&ss.acc[wave][n][d * 16 + g * 4] = acc[d];
     __syncthreads();
     const size_t slot = (size_t)kvh * part.slots + it.slot + it.piece;
-    for (uint32_t i = threadIdx.x; i < kRowsTile * (D / 4); i += kAttnThreads) {
-        const uint32_t r = i / (D / 4), d = i % (D / 4) * 4, q = it.tile * kRowsTile + r;
-        if (q >= sh.n * group) continue;
+    for (uint32_t i = threadIdx.x; i < min(rows - row0, kRowsTile) * (D / 4); i += kAttnThreads) {
+        const uint32_t r = i / (D / 4), d = i % (D / 4) * 4, q = row0 + r;
         float top = kNoMax;
 #pragma unroll
-        for (uint32_t w = 0; w < kAttnWaves; w++) top = fmaxf(top, sh_ml[w][r][0]);
+        for (uint32_t w = 0; w < kAttnWaves; w++) top = fmaxf(top, ss.ml[w][r][0]);
         f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
         float l = 0.f;
 #pragma unroll
         for (uint32_t w = 0; w < kAttnWaves; w++) {
-            const float f = __builtin_amdgcn_exp2f(sh_ml[w][r][0] - top);
-            l = fmaf(f, sh_ml[w][r][1], l);
-            o += *(const f32x4_t *)&sh_acc[w][r][d] * f;
+            const float f = __builtin_amdgcn_exp2f(ss.ml[w][r][0] - top);
+            l = fmaf(f, ss.ml[w][r][1], l);
+            o += *(const f32x4_t *)&ss.acc[w][r][d] * f;
         }
         if (it.pieces > 1) {
             *(f32x4_t *)(part.acc + (slot * kRowsTile + r) * D + d) = o;
@@ -569,17 +600,15 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
         f32x16_t S[2], zero;
 #pragma unroll
         for (int j = 0; j < 16; j++) zero[j] = 0.f;
-        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
+        for (int k = 0; k < 2 * NK; k++) {
 #pragma unroll
-            for (int k = 0; k < 2 * NK; k++) {
+            for (int t = 0; t < 2; t++) {
                 const f16x8_t ka = *(const f16x8_t *)&sh_k[buf][t * 32 + n][k * 16 + hi * 8];
                 S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qh[k], k ? S[t] : zero, 0, 0, 0);
                 if constexpr (PAIRS) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, ql[k], S[t], 0, 0, 0);
             }
         }
-        __builtin_amdgcn_s_setprio(0);
         // x[c]: the 8 scores of group c of 16 keys, keys 16 c + 8 hi + j; their logarithm (base 2) with the value scale: x a + e
         float a[4], e[4], unscale[4];
 #pragma unroll
@@ -590,13 +619,7 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
             for (int c = 0; c < 4; c++) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    float x = S[c / 2][c % 2 * 8 + j] * a[c];
-                    if constexpr (CAP) {
-                        // cap * tanh(s / cap) = cap - 2 cap / (exp(2 s / cap) + 1)
-                        const float z = __builtin_amdgcn_exp2f(x * (2.f * kLog2E / A.softcap));
-                        x = (A.softcap - 2.f * A.softcap * __builtin_amdgcn_rcpf(z + 1.f)) * kLog2E;
-                    }
-                    x += e[c];
+                    const float x = score<CAP>(A, S[c / 2][c % 2 * 8 + j], a[c], e[c]);
                     const int32_t key = key0 + c * 16 + (int32_t)hi * 8 + j;
                     S[c / 2][c % 2 * 8 + j] = !whole && (key > key_hi || key < key_lo) ? -__builtin_inff() : x;
                 }
@@ -634,16 +657,14 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
             }
             L = fmaf(sum, unscale[c], L);
         }
-        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int d = 0; d < NK; d++)
+        for (int c = 0; c < 4; c++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
+            for (int d = 0; d < NK; d++) {
                 const f16x8_t va = *(const f16x8_t *)&sh_v[buf][d * 32 + n][c * 16 + hi * 8];
                 acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[c], acc[d], 0, 0, 0);
                 if constexpr (PAIRS) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[c], acc[d], 0, 0, 0);
             }
-        __builtin_amdgcn_s_setprio(0);
     }
     L += __shfl_xor(L, 32, 64);
     if (!live) return;
@@ -701,51 +722,43 @@ __device__ __forceinline__ void join_pieces(const Partials &part, uint32_t tile,
     }
 }
 
-// The pieces of split rows as one.  FEW: a workgroup for each query row of a split tile, its wavefronts a quarter of the pieces each;
-// otherwise a wavefront for a row, kJoinRows rows a workgroup.
-constexpr uint32_t kJoinRows = 16;
-template <bool FEW>
-__global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttentionArgs A, Plan P, Partials part) {
-    __shared__ float sh_acc[FEW ? kAttnWaves : 1][256], sh_ml[kAttnWaves][2];
+// The pieces of split rows as one: a workgroup for kJoinRows rows of a split tile, `share` of its wavefronts (1, 2, 4 or 8) for a row.
+constexpr uint32_t kJoinRows = 16, kJoinWaves = 8;
+__global__ void __launch_bounds__(kJoinWaves * 64) attention_join_kernel(AttentionArgs A, Plan P, Partials part, uint32_t share) {
+    __shared__ float sh_acc[kJoinWaves][256], sh_ml[kJoinWaves][2];
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, D = A.kv.head_dim, dim = min(lane * 4, D - 4);
     const uint32_t kvh = blockIdx.y, group = A.q_heads / A.kv.kv_heads;
     Item it;
     if (!find_item(A, P, blockIdx.x, true, it)) return;
     const Share sh = share_of(A, P, it.s, group);
-    const uint32_t row0 = (FEW ? it.tile : sh.tiles - 1 - it.tile) * P.tile, rows = sh.n * group;
+    const uint32_t row0 = (P.tile == kTilesTile ? sh.tiles - 1 - it.tile : it.tile) * P.tile;
     const size_t at = ((size_t)kvh * part.slots + it.slot) * P.tile;
-    const auto put = [&](uint32_t q, float top, float l, const f32x4_t &o) {
-        const uint32_t h = kvh * group + q % group;
+    const uint32_t end = min((blockIdx.z + 1) * kJoinRows, min(P.tile, sh.n * group - row0));
+    for (uint32_t r0 = blockIdx.z * kJoinRows; r0 < end; r0 += kJoinWaves / share) {
+        const uint32_t r = r0 + wave / share;
+        float top = kNoMax, l = 0.f;
+        f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if (r < end) join_pieces(part, P.tile, D, at + r, it.pieces, wave % share, share, dim, top, l, o);
+        if (share > 1) {
+            __syncthreads();  // (the rows before have been read)
+            if (lane == 0) sh_ml[wave][0] = top, sh_ml[wave][1] = l;
+            if (lane * 4 < D) *(f32x4_t *)&sh_acc[wave][lane * 4] = o;
+            __syncthreads();
+            if (wave % share) continue;
+            for (uint32_t w = wave + 1; w < wave + share; w++) top = fmaxf(top, sh_ml[w][0]);
+            l = 0.f;
+            o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            for (uint32_t w = wave; w < wave + share; w++) {
+                const float f = __builtin_amdgcn_exp2f(sh_ml[w][0] - top);
+                l = fmaf(f, sh_ml[w][1], l);
+                o += *(const f32x4_t *)&sh_acc[w][dim] * f;
+            }
+        }
+        if (r >= end || lane * 4 >= D) continue;
+        const uint32_t q = row0 + r, h = kvh * group + q % group;
         const float inv = inverse_sum(A, l, top, h);
         const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-        if (lane * 4 < D) store4(A.out, A.out_type, (size_t)(sh.row + q / group) * A.out_stride + (size_t)h * D + lane * 4, v);
-    };
-    float top, l;
-    f32x4_t o;
-    if constexpr (!FEW) {
-        for (uint32_t r = blockIdx.z * kJoinRows + wave; r < (blockIdx.z + 1) * kJoinRows && row0 + r < rows; r += kAttnWaves) {
-            join_pieces(part, P.tile, D, at + r, it.pieces, 0, 1, dim, top, l, o);
-            put(row0 + r, top, l, o);
-        }
-    } else {
-        const uint32_t r = blockIdx.z;
-        if (row0 + r >= rows) return;
-        join_pieces(part, P.tile, D, at + r, it.pieces, wave, kAttnWaves, dim, top, l, o);
-        if (lane == 0) sh_ml[wave][0] = top, sh_ml[wave][1] = l;
-        if (lane * 4 < D) *(f32x4_t *)&sh_acc[wave][lane * 4] = o;
-        __syncthreads();
-        if (wave) return;
-#pragma unroll
-        for (uint32_t w = 1; w < kAttnWaves; w++) top = fmaxf(top, sh_ml[w][0]);
-        l = 0.f;
-        o = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (uint32_t w = 0; w < kAttnWaves; w++) {
-            const float f = __builtin_amdgcn_exp2f(sh_ml[w][0] - top);
-            l = fmaf(f, sh_ml[w][1], l);
-            o += *(const f32x4_t *)&sh_acc[w][dim] * f;
-        }
-        put(row0 + r, top, l, o);
+        store4(A.out, A.out_type, (size_t)(sh.row + q / group) * A.out_stride + (size_t)h * D + lane * 4, v);
     }
 }
 
@@ -797,9 +810,9 @@ static hipError_t launch_plan(hipStream_t s, const AttentionArgs &A, const Plan 
     }
     if (P.split) {
         const uint32_t rows = (uint32_t)std::min<uint64_t>((uint64_t)A.kv.max_new * (A.q_heads / A.kv.kv_heads), P.tile);
-        const uint32_t split = (uint32_t)Plans::split_tiles(P);
-        if (tiles) hipLaunchKernelGGL(attention_join_kernel<false>, dim3(split, A.kv.kv_heads, (rows + kJoinRows - 1) / kJoinRows), dim3(kAttnThreads), 0, s, A, P, part);
-        else hipLaunchKernelGGL(attention_join_kernel<true>, dim3(split, A.kv.kv_heads, rows), dim3(kAttnThreads), 0, s, A, P, part);
+        const uint32_t share = rows <= 1 ? 8 : rows <= 2 ? 4 : rows <= 4 ? 2 : 1;
+        hipLaunchKernelGGL(attention_join_kernel, dim3((uint32_t)Plans::split_tiles(A, P), A.kv.kv_heads, (rows + kJoinRows - 1) / kJoinRows),
+                           dim3(kJoinWaves * 64), 0, s, A, P, part, share);
     }
     return hipGetLastError();
 }
