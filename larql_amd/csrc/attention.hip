@@ -18,7 +18,6 @@ namespace larql {
 
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr uint32_t kStep = 64;          // keys of a step
@@ -124,11 +123,13 @@ struct Plans {
 static Plans plans_of(const AttentionArgs &A) {
     const uint64_t group = A.q_heads / A.kv.kv_heads, most = A.kv.max_new * group;
     const uint64_t steps = (((uint64_t)A.kv.table_width << A.kv.page_shift) + kStep - 1) / kStep;
-    const uint32_t cus = 256, per_cu = A.kv.head_dim > 128 ? 1 : 2;  // workgroups of a kernel that a compute unit holds
+    const uint32_t cus = 256;
     Plans p;
-    p.rows = {kRowsTile, 1, kFewRows, std::max(2 * cus * per_cu / A.kv.kv_heads, 1u), 4, 1};
+    // Pieces of few rows: as many as workgroups are resident, 2 a compute unit above 128 channels (131072 keys of 256, us with 1, 2, 3, 4 of
+    // them: 148, 103, 125, 110, joining included), 3 below (64 sequences, 64 channels: 44, 37, 33, 37); a wavefront's step each at least.
+    p.rows = {kRowsTile, 1, kFewRows, std::max((A.kv.head_dim > 128 ? 2 : 3) * cus / A.kv.kv_heads, 1u), kAttnWaves, 1};
     p.rows.split = steps > p.rows.min_steps;
-    p.tiles = {kTilesTile, kFewRows + 1, 0xFFFFFFFFu, std::max(cus * per_cu / A.kv.kv_heads, 1u), 8, 1};
+    p.tiles = {kTilesTile, kFewRows + 1, 0xFFFFFFFFu, std::max((A.kv.head_dim > 128 ? 1 : 2) * cus / A.kv.kv_heads, 1u), 8, 1};
     p.tiles.split = steps > p.tiles.min_steps && A.kv.tokens * group / p.tiles.tile + A.kv.sequences < p.tiles.target;
     p.use_tiles = most > kFewRows;
     p.use_rows = !p.use_tiles || A.kv.sequences > 1;
@@ -182,7 +183,7 @@ __device__ __forceinline__ float score(const AttentionArgs &A, float s, float a,
 // A query row's elements (spread over lanes 32 apart, and 16 apart where QUARTERS) as f16 or f16 pairs after a power-of-two scale that brings
 // the largest to [2^14, 2^15); returns what scores are multiplied by.  A row that is not finite gets NaN there.
 template <int N, bool PAIRS, bool CAP, bool QUARTERS>
-__device__ __forceinline__ float query_f16(const AttentionArgs &A, const float (&q)[N][8], f16x8_t (&qh)[N], f16x8_t (&ql)[PAIRS ? N : 1]) {
+__device__ __forceinline__ float query_f16(const AttentionArgs &A, const Eight (&q)[N], f16x8_t (&qh)[N], f16x8_t (&ql)[PAIRS ? N : 1]) {
     uint32_t amax = 0;
 #pragma unroll
     for (int k = 0; k < N; k++)
@@ -294,13 +295,12 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(Attenti
 
     // channel d of the lane's operand k: 64 channels of two operands lie in one 16-byte piece of a key's row
     if (wave == 0) {
-        float q[NK][8];
+        Eight q[NK];
 #pragma unroll
         for (int k = 0; k < NK; k++) {
             const uint32_t d = (k | 1) < NK ? (uint32_t)(k & ~1) * 32 + g * 16 + (uint32_t)(k & 1) * 8 : (uint32_t)k * 32 + g * 8;
-#pragma unroll
-            for (int i = 0; i < 8; i++) q[k][i] = 0.f;
-            if (live) load8(A.q, A.q_type, (size_t)(sh.row + tok) * A.q_stride + (size_t)(kvh * group + row % group) * D + d, q[k]);
+            q[k] = {};
+            if (live) q[k] = load8(A.q, A.q_type, (size_t)(sh.row + tok) * A.q_stride + (size_t)(kvh * group + row % group) * D + d);
         }
         f16x8_t qh[NK], ql[PAIRS ? NK : 1];
         const float f = query_f16<NK, PAIRS, CAP, true>(A, q, qh, ql);
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(Attenti
         }
         const uint32_t h = kvh * group + q % group;
         const float inv = inverse_sum(A, l, top, h);
-        const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+        const f32x4_t v = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
         store4(A.out, A.out_type, (size_t)(sh.row + q / group) * A.out_stride + (size_t)h * D + d, v);
     }
 }
@@ -479,12 +479,11 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
     f16x8_t qh[2 * NK], ql[PAIRS ? 2 * NK : 1];
     float factor;
     {
-        float q[2 * NK][8];
+        Eight q[2 * NK];
 #pragma unroll
         for (int k = 0; k < 2 * NK; k++) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) q[k][i] = 0.f;
-            if (live) load8(A.q, A.q_type, (size_t)(sh.row + tok) * A.q_stride + (size_t)head * D + (uint32_t)k * 16 + hi * 8, q[k]);
+            q[k] = {};
+            if (live) q[k] = load8(A.q, A.q_type, (size_t)(sh.row + tok) * A.q_stride + (size_t)head * D + (uint32_t)k * 16 + hi * 8);
         }
         factor = query_f16<2 * NK, PAIRS, CAP, false>(A, q, qh, ql);
     }
@@ -684,7 +683,7 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
     for (int d = 0; d < NK; d++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float v[4] = {acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv, acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv};
+            const f32x4_t v = {acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv, acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv};
             store4(A.out, A.out_type, (size_t)(sh.row + tok) * A.out_stride + (size_t)head * D + d * 32 + i * 8 + hi * 4, v);
         }
 }
@@ -757,7 +756,7 @@ __global__ void __launch_bounds__(kJoinWaves * 64) attention_join_kernel(Attenti
         if (r >= end || lane * 4 >= D) continue;
         const uint32_t q = row0 + r, h = kvh * group + q % group;
         const float inv = inverse_sum(A, l, top, h);
-        const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+        const f32x4_t v = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
         store4(A.out, A.out_type, (size_t)(sh.row + q / group) * A.out_stride + (size_t)h * D + lane * 4, v);
     }
 }

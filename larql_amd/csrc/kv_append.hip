@@ -13,46 +13,48 @@ constexpr uint32_t kAppendThreads = 256;
 
 // 8 channels of one head and token, as four pairs (lo[i], hi[i]) that turn together
 struct Quad {
-    float lo[4], hi[4];
+    f32x4_t lo, hi;
 };
 
 // Channels of the pairs 4g .. 4g+3: (p, p + rot/2) inside the rotated part of a halved layout, else (2p, 2p + 1).
 __device__ __forceinline__ bool halved(const KvAppendArgs &A, uint32_t g) { return !A.interleaved && 8 * g < A.rot_dim; }
-__device__ __forceinline__ void load_quad(const KvAppendArgs &A, const void *row, int type, size_t at, uint32_t g, Quad &q) {
-    if (halved(A, g)) {
-        load4(row, type, at + 4 * g, q.lo);
-        load4(row, type, at + 4 * g + A.rot_dim / 2, q.hi);
-    } else {
-        float x[8];
-        load8(row, type, at + 8 * g, x);
-#pragma unroll
-        for (int i = 0; i < 4; i++) q.lo[i] = x[2 * i], q.hi[i] = x[2 * i + 1];
-    }
+__device__ __forceinline__ Quad load_quad(const KvAppendArgs &A, const void *row, int type, size_t at, uint32_t g) {
+    const bool h = halved(A, g);
+    const size_t a = at + (h ? 4 * g : 8 * g), b = at + (h ? 4 * g + A.rot_dim / 2 : 8 * g + 4);
+    const f32x4_t u = load4(row, type, a), v = load4(row, type, b);
+    if (h) return {u, v};
+    return {f32x4_t{u[0], u[2], v[0], v[2]}, f32x4_t{u[1], u[3], v[1], v[3]}};
 }
 __device__ __forceinline__ void store_quad(const KvAppendArgs &A, void *row, int type, size_t at, uint32_t g, const Quad &q) {
     if (halved(A, g)) {
         store4(row, type, at + 4 * g, q.lo);
         store4(row, type, at + 4 * g + A.rot_dim / 2, q.hi);
     } else {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[2 * i] = q.lo[i], x[2 * i + 1] = q.hi[i];
-        store8(row, type, at + 8 * g, x);
+        store8(row, type, at + 8 * g, {f32x4_t{q.lo[0], q.hi[0], q.lo[1], q.hi[1]}, f32x4_t{q.lo[2], q.hi[2], q.lo[3], q.hi[3]}});
     }
 }
 
-// cos and sin of position * inv_freq[4g + i], times rope_scale.  Far positions lose the angle in 32 bits: whole turns leave in 64.
+// cos and sin of position * inv_freq[4g + i], times rope_scale.  Far positions lose the angle in 32 bits: whole turns leave in 64, then
+// quarter turns; what is left, at most an eighth, goes through the Taylor series (next terms below 2e-9 and 2e-10).
 struct Turn {
-    float c[4], s[4];
+    f32x4_t c, s;
 };
-__device__ __forceinline__ void turn_of(const KvAppendArgs &A, int32_t pos, uint32_t g, Turn &t) {
+__device__ __forceinline__ void turn_of(const KvAppendArgs &A, int32_t pos, f32x4_t freq, Turn &t) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const double turns = (double)pos * (double)A.inv_freq[4 * g + i] * 0.15915494309189533577;
-        sincospif(2.f * (float)(turns - rint(turns)), &t.s[i], &t.c[i]);
-        t.s[i] *= A.rope_scale;
-        t.c[i] *= A.rope_scale;
+        const double turns = (double)pos * (double)freq[i] * 0.15915494309189533577;
+        const float r = (float)(turns - rint(turns)), quarters = rintf(4.f * r);
+        const float x = fmaf(quarters, -0.25f, r) * 6.283185307179586f, x2 = x * x;
+        const float sn = x * fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), 1.f);
+        const float cs = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, -1.f / 3628800.f, 1.f / 40320.f), -1.f / 720.f), 1.f / 24.f), -0.5f), 1.f);
+        const int q = (int)quarters;
+        const float a = q & 1 ? sn : cs, b = q & 1 ? cs : sn;  // |cos|, |sin| of the whole angle; cos < 0 in quarters 1, 2, sin < 0 in 2, 3
+        t.c[i] = ((q + 1) & 2 ? -a : a) * A.rope_scale;
+        t.s[i] = (q & 2 ? -b : b) * A.rope_scale;
     }
+}
+__device__ __forceinline__ f32x4_t load_freq(const KvAppendArgs &A, uint32_t g) {  // (4-byte aligned)
+    return f32x4_t{A.inv_freq[4 * g], A.inv_freq[4 * g + 1], A.inv_freq[4 * g + 2], A.inv_freq[4 * g + 3]};
 }
 __device__ __forceinline__ void rotate(Quad &q, const Turn &t) {
 #pragma unroll
@@ -92,12 +94,6 @@ __device__ __forceinline__ float pow2f(int e) { return __builtin_bit_cast(float,
 // The page (sequence s, place j in its table) that is the item-th of all pages with new tokens; false beyond the last.
 __device__ __forceinline__ bool find_page(const KvArgs &kv, uint32_t item, uint32_t &s, uint32_t &j) {
     const uint32_t lane = threadIdx.x % 64;
-    if (kv.max_new == 1) {  // at most one page for each sequence
-        s = item;
-        const NewTokens t = new_tokens(kv, s);
-        j = (uint32_t)(t.len - 1) >> kv.page_shift;
-        return t.n == 1 && t.len > 0;
-    }
     for (uint32_t base = 0; base < kv.sequences; base += 64) {
         uint32_t pages = 0, first = 0;
         if (base + lane < kv.sequences) {
@@ -132,29 +128,182 @@ __device__ __forceinline__ bool find_token(const KvArgs &kv, uint32_t token, New
     return token >= t.row && token - t.row < t.n;
 }
 
-// LPH lanes (8 channels each) serve a token of a head, kAppendThreads / LPH tokens at once, NP times a page.
+// A page's scale with its new elements: the exponent, and whether it is a number.  amax: the largest new |x| as bits (a NaN or an
+// infinity above every number), older: tokens that the page held before.
+struct Scale {
+    int e, old_e;
+    bool finite;
+};
+__device__ __forceinline__ Scale scale_of(uint32_t amax, bool older, float old_scale) {
+    // 448 = 1.75 * 2^8: the smallest e with |x| <= 448 * 2^e
+    Scale s;
+    s.e = (int)(amax >> 23) - 127 - 8 + ((amax & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    s.finite = amax < 0x7F800000u && s.e <= kScaleMaxExp;
+    s.e = max(s.e, kScaleMinExp);
+    const uint32_t old_bits = __builtin_bit_cast(uint32_t, old_scale) & 0x7FFFFFFFu;
+    s.old_e = (int)(old_bits >> 23) - 127;
+    if (older) {
+        s.finite = s.finite && old_bits < 0x7F800000u;
+        s.e = max(s.e, s.old_e);
+    }
+    return s;
+}
+__device__ __forceinline__ float scale_value(const Scale &s) { return s.finite ? pow2f(s.e) : __builtin_nanf(""); }
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
+__device__ __forceinline__ uint32_t quad_amax(const Quad &q) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) m = max(m, max(abs_bits(q.lo[i]), abs_bits(q.hi[i])));
+    return m;
+}
+
+// The codes of a page's older tokens, for a larger scale, by `threads` threads.
+__device__ __forceinline__ void rescale_keys(uint8_t *codes, uint32_t head_dim, uint32_t older, float ratio, uint32_t thread, uint32_t threads) {
+    for (uint32_t i = thread; i < older * head_dim / 4; i += threads) {
+        uint32_t *at = (uint32_t *)codes + i;
+        *at = rescale_fp8(*at, ratio);
+    }
+}
+__device__ __forceinline__ void rescale_values(uint8_t *codes, uint32_t head_dim, uint32_t page_shift, uint32_t older, float ratio, uint32_t thread,
+                                               uint32_t threads) {
+    const uint32_t words = (older + 3) / 4;
+    for (uint32_t i = thread; i < head_dim * words; i += threads) {
+        const uint32_t c = i % words;
+        uint32_t *at = (uint32_t *)(codes + ((size_t)(i / words) << page_shift)) + c;
+        const uint32_t v = *at, keep = older - 4 * c >= 4 ? 0u : ~0u << (8 * (older - 4 * c));
+        *at = (rescale_fp8(v & ~keep, ratio) & ~keep) | (v & keep);
+    }
+}
+
+// The codes of a key's 8 channels.
+__device__ __forceinline__ void store_key(const KvAppendArgs &A, uint8_t *row, uint32_t g, const Quad &q, float inv, bool finite) {
+    uint32_t a = 0, b = 0;
+    if (finite) {
+        a = pack_fp8(q.lo[0] * inv, q.lo[1] * inv, q.lo[2] * inv, q.lo[3] * inv);
+        b = pack_fp8(q.hi[0] * inv, q.hi[1] * inv, q.hi[2] * inv, q.hi[3] * inv);
+    }
+    if (halved(A, g)) {
+        *(uint32_t *)(row + 4 * g) = a;
+        *(uint32_t *)(row + 4 * g + A.rot_dim / 2) = b;
+    } else {  // lo and hi alternate
+        *(u32x2_t *)(row + 8 * g) = u32x2_t{__builtin_amdgcn_perm(b, a, 0x05010400u), __builtin_amdgcn_perm(b, a, 0x07030602u)};
+    }
+}
+
+// One new token a sequence: LPH lanes (8 channels each) serve a head of it, keys, values and queries alike, with nothing to wait for but
+// the loads (lengths and rows; the activations and the table; the page's scale).
+template <uint32_t LPH>
+__global__ void __launch_bounds__(kAppendThreads) kv_append_one_kernel(KvAppendArgs A, uint32_t blocks) {
+    const KvArgs &kv = A.kv;
+    const uint32_t s = blockIdx.x / blocks, g = threadIdx.x % LPH;
+    const uint32_t head = (blockIdx.x % blocks) * (kAppendThreads / LPH) + threadIdx.x / LPH;  // keys, values, queries
+    const bool is_k = head < kv.kv_heads, is_v = !is_k && head < 2 * kv.kv_heads, is_q = !is_k && !is_v && A.q && head < 2 * kv.kv_heads + A.q_heads;
+    const bool in_head = 8 * g < kv.head_dim && (is_k || is_v || is_q), turns = 8 * g < A.rot_dim && !is_v;
+    const NewTokens t = new_tokens(kv, s);
+    if (t.n != 1) return;
+    const uint32_t h = is_k ? head : is_v ? head - kv.kv_heads : head - 2 * kv.kv_heads;
+    const float *norm = is_k ? A.k_norm : is_q ? A.q_norm : nullptr;
+    Quad x = {}, w = {};
+    f32x4_t freq = {0.f, 0.f, 0.f, 0.f};
+    if (in_head) {
+        const void *src = is_k ? A.k : is_v ? A.v : A.q;
+        const size_t at = t.row * (is_k ? A.k_stride : is_v ? A.v_stride : A.q_stride) + (size_t)h * kv.head_dim;
+        if (is_v) {
+            const Eight v = load8(src, A.type, at + 8 * g);
+            x = {v.a, v.b};
+        } else {
+            x = load_quad(A, src, A.type, at, g);
+            if (norm) w = load_quad(A, norm, ELEM_F32, 0, g);
+            if (turns) freq = load_freq(A, g);
+        }
+    }
+    const uint32_t slot = (uint32_t)max(t.len - 1, 0) & ((1u << kv.page_shift) - 1);
+    const uint32_t page = is_q || t.len == 0 ? ~0u : kv_page(kv, kv.block_table + (size_t)s * kv.table_width, (uint32_t)(t.len - 1));
+    const bool stored = (is_k || is_v) && page != ~0u;
+    const size_t of_page = stored ? (size_t)page * kv.kv_heads + h : 0;
+    float *scale_at = (is_v ? kv.v_scales : kv.k_scales) + of_page;
+    const float old_scale = stored && slot ? *scale_at : 1.f;
+    Quad y = x;
+    if (A.q_norm || A.k_norm) norm_quad<LPH>(A, y, w);  // (whole wavefronts)
+    if (norm) x = y;
+    if (turns) {
+        Turn turn;
+        turn_of(A, t.len - 1, freq, turn);
+        rotate(x, turn);
+    }
+    uint32_t amax = quad_amax(x);
+#pragma unroll
+    for (uint32_t m = 1; m < LPH; m *= 2) amax = max(amax, (uint32_t)__shfl_xor((int)amax, (int)m, 64));
+    if (is_q && in_head) store_quad(A, A.q_out, A.type, t.row * A.q_out_stride + (size_t)h * kv.head_dim, g, x);
+    if (!stored) return;
+    const Scale sc = scale_of(amax, slot != 0, old_scale);
+    uint8_t *codes = (is_v ? kv.v_codes : kv.k_codes) + of_page * ((size_t)kv.head_dim << kv.page_shift);
+    if (sc.finite && slot && sc.e > sc.old_e) {
+        const float ratio = pow2f(max(sc.old_e - sc.e, -126));
+        if (is_v) rescale_values(codes, kv.head_dim, kv.page_shift, slot, ratio, g, LPH);
+        else rescale_keys(codes, kv.head_dim, slot, ratio, g, LPH);
+    }
+    // (a word of a value row can hold older tokens and the new one: its bytes are written by the wavefront that rescaled the word,
+    // after it, and to the same place in memory order)
+    if (is_v) __threadfence_block();
+    if (g == 0) *scale_at = scale_value(sc);
+    if (!in_head) return;
+    const float inv = sc.finite ? pow2f(-sc.e) : 0.f;
+    if (is_k) {
+        store_key(A, codes + (size_t)slot * kv.head_dim, g, x, inv, sc.finite);
+    } else {
+        uint32_t a = 0, b = 0;
+        if (sc.finite) {
+            a = pack_fp8(x.lo[0] * inv, x.lo[1] * inv, x.lo[2] * inv, x.lo[3] * inv);
+            b = pack_fp8(x.hi[0] * inv, x.hi[1] * inv, x.hi[2] * inv, x.hi[3] * inv);
+        }
+        uint8_t *col = codes + ((size_t)(8 * g) << kv.page_shift) + slot;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            col[(size_t)i << kv.page_shift] = (uint8_t)(a >> (8 * i));
+            col[(size_t)(4 + i) << kv.page_shift] = (uint8_t)(b >> (8 * i));
+        }
+    }
+}
+
+// Several new tokens a sequence.  A workgroup serves one head of one page, keys or values, or the queries of one token.  Keys and queries: LPH
+// lanes (8 channels each) a head, kAppendThreads / LPH tokens or heads at once, NP times a page.  Values: a thread takes two channels of 16 keys,
+// so that it stores the 16 bytes that lie together.
 template <uint32_t LPH, int NP>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendArgs A, uint32_t page_blocks) {
     constexpr uint32_t kTokens = kAppendThreads / LPH;
+    constexpr int NV = (NP + 3) / 4;
     __shared__ uint32_t part[kAppendThreads / 64];
     const KvArgs &kv = A.kv;
-    const uint32_t g = threadIdx.x % LPH;
-    const bool in_head = 8 * g < kv.head_dim, turns = 8 * g < A.rot_dim;
-    Quad w;
+    const uint32_t g0 = threadIdx.x % LPH, g = 8 * g0 < kv.head_dim ? g0 : 0;  // (lanes beyond head_dim load what another does)
+    const bool in_head = 8 * g0 < kv.head_dim, turns = 8 * g < A.rot_dim;
+    Quad w = {};
+    f32x4_t freq = {0.f, 0.f, 0.f, 0.f};
     if (blockIdx.x >= page_blocks) {  // the queries of one token
-        const uint32_t token = blockIdx.x - page_blocks;
+        const uint32_t token = blockIdx.x - page_blocks, first = threadIdx.x / LPH;
+        const auto load = [&](uint32_t head) {
+            return load_quad(A, A.q, A.type, token * A.q_stride + (size_t)min(head, A.q_heads - 1) * kv.head_dim, g);
+        };
+        Quad q[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) q[i] = load(first + i * kTokens);
+        if (turns) freq = load_freq(A, g);
+        if (A.q_norm) w = load_quad(A, A.q_norm, ELEM_F32, 0, g);
         NewTokens t;
         if (!find_token(kv, token, t)) return;
         Turn turn;
-        if (turns) turn_of(A, t.len - (int32_t)t.n + (int32_t)(token - t.row), g, turn);
-        if (A.q_norm && in_head) load_quad(A, A.q_norm, ELEM_F32, 0, g, w);
-        for (uint32_t head = threadIdx.x / LPH; head < (A.q_heads + kTokens - 1) / kTokens * kTokens; head += kTokens) {
-            Quad q = {};
-            const bool live = in_head && head < A.q_heads;
-            if (live) load_quad(A, A.q, A.type, token * A.q_stride + (size_t)head * kv.head_dim, g, q);
-            if (A.q_norm) norm_quad<LPH>(A, q, w);
-            if (turns) rotate(q, turn);
-            if (live) store_quad(A, A.q_out, A.type, token * A.q_out_stride + (size_t)head * kv.head_dim, g, q);
+        if (turns) turn_of(A, t.len - (int32_t)t.n + (int32_t)(token - t.row), freq, turn);
+        for (uint32_t head0 = 0; head0 < A.q_heads; head0 += 4 * kTokens) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const uint32_t head = head0 + first + i * kTokens;
+                Quad y = q[i];
+                q[i] = load(head + 4 * kTokens);
+                if (!in_head) y = {};
+                if (A.q_norm) norm_quad<LPH>(A, y, w);
+                if (turns) rotate(y, turn);
+                if (in_head && head < A.q_heads) store_quad(A, A.q_out, A.type, token * A.q_out_stride + (size_t)head * kv.head_dim, g, y);
+            }
         }
         return;
     }
@@ -170,101 +319,86 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendArgs 
     const uint32_t lo = (uint32_t)max(first, (int32_t)base) - base, hi = min((uint32_t)t.len - base, P);  // new slots of this page
     float *scale_at = (is_v ? kv.v_scales : kv.k_scales) + (size_t)page * kv.kv_heads + head;
     const float old_scale = lo ? *scale_at : 1.f;
-
-    // pass 1: the new elements, and the largest |x| as bits (a NaN or an infinity above every number)
-    const void *src = is_v ? A.v : A.k;
-    const size_t stride = is_v ? A.v_stride : A.k_stride;
-    const bool with_norm = !is_v && A.k_norm;
-    if (with_norm && in_head) load_quad(A, A.k_norm, ELEM_F32, 0, g, w);
-    Quad x[NP];
-    uint32_t amax = 0;
-#pragma unroll
-    for (int p = 0; p < NP; p++) {
-        const uint32_t slot = (uint32_t)p * kTokens + threadIdx.x / LPH;
-        const bool live = in_head && slot >= lo && slot < hi;
-        x[p] = {};
-        if (live) {
-            const size_t at = (t.row + (size_t)((int32_t)(base + slot) - first)) * stride + (size_t)head * kv.head_dim;
-            if (is_v) {
-                float v[8];
-                load8(src, A.type, at + 8 * g, v);
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[p].lo[i] = v[i], x[p].hi[i] = v[4 + i];
-            } else {
-                load_quad(A, src, A.type, at, g, x[p]);
-            }
-        }
-        if (with_norm) norm_quad<LPH>(A, x[p], w);
-        if (!is_v && turns && live) {
-            Turn turn;
-            turn_of(A, (int32_t)(base + slot), g, turn);
-            rotate(x[p], turn);
-        }
-        if (live)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                amax = max(amax, max(__builtin_bit_cast(uint32_t, x[p].lo[i]) & 0x7FFFFFFFu, __builtin_bit_cast(uint32_t, x[p].hi[i]) & 0x7FFFFFFFu));
-    }
-    amax = wave_max_u32(amax);
-    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = amax;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t i = 0; i < kAppendThreads / 64; i++) amax = max(amax, part[i]);
-
-    // 448 = 1.75 * 2^8: the smallest e with |x| <= 448 * 2^e
-    int e = (int)(amax >> 23) - 127 - 8 + ((amax & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-    bool finite = amax < 0x7F800000u && e <= kScaleMaxExp;
-    e = max(e, kScaleMinExp);
-    const uint32_t old_bits = __builtin_bit_cast(uint32_t, old_scale) & 0x7FFFFFFFu;
-    if (lo) {
-        finite = finite && old_bits < 0x7F800000u;
-        e = max(e, (int)(old_bits >> 23) - 127);
-    }
     uint8_t *codes = (is_v ? kv.v_codes : kv.k_codes) + ((size_t)page * kv.kv_heads + head) * ((size_t)kv.head_dim << kv.page_shift);
-    if (finite && lo && e > (int)(old_bits >> 23) - 127) {  // the older tokens' codes, for the larger scale
-        const float ratio = pow2f(max((int)(old_bits >> 23) - 127 - e, -126));
-        if (is_v) {
-            const uint32_t words = (lo + 3) / 4;
-            for (uint32_t i = threadIdx.x; i < kv.head_dim * words; i += kAppendThreads) {
-                const uint32_t c = i % words;
-                uint32_t *at = (uint32_t *)(codes + ((size_t)(i / words) << kv.page_shift)) + c;
-                const uint32_t v = *at, keep = lo - 4 * c >= 4 ? 0u : ~0u << (8 * (lo - 4 * c));
-                *at = (rescale_fp8(v & ~keep, ratio) & ~keep) | (v & keep);
+    // the row of a slot (of the nearest new one: loads need no condition)
+    const auto row_of = [&](uint32_t slot) { return t.row + (size_t)((int32_t)(base + min(max(slot, lo), hi - 1)) - first); };
+    const auto page_scale = [&](uint32_t amax) {
+        amax = wave_max_u32(amax);
+        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = amax;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kAppendThreads / 64; i++) amax = max(amax, part[i]);
+        const Scale sc = scale_of(amax, lo != 0, old_scale);
+        if (threadIdx.x == 0) *scale_at = scale_value(sc);
+        return sc;
+    };
+    uint32_t amax = 0;
+    if (!is_v) {
+        Quad x[NP];
+#pragma unroll
+        for (int p = 0; p < NP; p++)
+            x[p] = load_quad(A, A.k, A.type, row_of((uint32_t)p * kTokens + threadIdx.x / LPH) * A.k_stride + (size_t)head * kv.head_dim, g);
+        if (turns) freq = load_freq(A, g);
+        if (A.k_norm) w = load_quad(A, A.k_norm, ELEM_F32, 0, g);
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+            const uint32_t slot = (uint32_t)p * kTokens + threadIdx.x / LPH;
+            if (!in_head) x[p] = {};
+            if (A.k_norm) norm_quad<LPH>(A, x[p], w);
+            if (turns) {
+                Turn turn;
+                turn_of(A, (int32_t)(base + slot), freq, turn);
+                rotate(x[p], turn);
             }
-        } else {
-            for (uint32_t i = threadIdx.x; i < lo * kv.head_dim / 4; i += kAppendThreads) {
-                uint32_t *at = (uint32_t *)codes + i;
-                *at = rescale_fp8(*at, ratio);
-            }
+            if (in_head && slot >= lo && slot < hi) amax = max(amax, quad_amax(x[p]));
         }
+        const Scale sc = page_scale(amax);
+        if (sc.finite && lo && sc.e > sc.old_e) rescale_keys(codes, kv.head_dim, lo, pow2f(max(sc.old_e - sc.e, -126)), threadIdx.x, kAppendThreads);
+        const float inv = sc.finite ? pow2f(-sc.e) : 0.f;
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+            const uint32_t slot = (uint32_t)p * kTokens + threadIdx.x / LPH;
+            if (in_head && slot >= lo && slot < hi) store_key(A, codes + (size_t)slot * kv.head_dim, g, x[p], inv, sc.finite);
+        }
+        return;
     }
-    if (threadIdx.x == 0) *scale_at = finite ? pow2f(e) : __builtin_nanf("");
-    if (is_v) __syncthreads();  // (a word of a value row can hold older and new tokens)
-
-    // pass 2: the codes
-    const float inv = finite ? pow2f(-e) : 0.f;
+    const uint32_t pairs = kv.head_dim / 2, units = pairs * (P / 16);  // (16 keys, two channels) each
+    f32x2_t x[NV][16];
 #pragma unroll
-    for (int p = 0; p < NP; p++) {
-        const uint32_t slot = (uint32_t)p * kTokens + threadIdx.x / LPH;
-        if (!in_head || slot < lo || slot >= hi) continue;
-        uint32_t a = 0, b = 0;  // codes of lo[], hi[]
-        if (finite) {
-            a = pack_fp8(x[p].lo[0] * inv, x[p].lo[1] * inv, x[p].lo[2] * inv, x[p].lo[3] * inv);
-            b = pack_fp8(x[p].hi[0] * inv, x[p].hi[1] * inv, x[p].hi[2] * inv, x[p].hi[3] * inv);
-        }
-        if (is_v) {
+    for (int v = 0; v < NV; v++) {
+        const uint32_t u = min(threadIdx.x + (uint32_t)v * kAppendThreads, units - 1), d = u % pairs * 2, slot0 = u / pairs * 16;
 #pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
-                codes[((size_t)(8 * g + i) << kv.page_shift) + slot] = (uint8_t)(a >> (8 * i));
-                codes[((size_t)(8 * g + 4 + i) << kv.page_shift) + slot] = (uint8_t)(b >> (8 * i));
+        for (int i = 0; i < 16; i++) x[v][i] = load2(A.v, A.type, row_of(slot0 + (uint32_t)i) * A.v_stride + (size_t)head * kv.head_dim + d);
+    }
+#pragma unroll
+    for (int v = 0; v < NV; v++)  // (other threads' units and other slots' rows: elements of this page's new tokens all the same)
+#pragma unroll
+        for (int i = 0; i < 16; i++) amax = max(amax, max(abs_bits(x[v][i][0]), abs_bits(x[v][i][1])));
+    const Scale sc = page_scale(amax);
+    if (sc.finite && lo && sc.e > sc.old_e) {
+        rescale_values(codes, kv.head_dim, kv.page_shift, lo, pow2f(max(sc.old_e - sc.e, -126)), threadIdx.x, kAppendThreads);
+        __syncthreads();  // (a word of a value row can hold older and new tokens)
+    }
+    const float inv = sc.finite ? pow2f(-sc.e) : 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        const uint32_t u = threadIdx.x + (uint32_t)v * kAppendThreads, d = u % pairs * 2, slot0 = u / pairs * 16;
+        if (u >= units || slot0 >= hi || slot0 + 16 <= lo) continue;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            u32x4_t code = {0u, 0u, 0u, 0u};
+            if (sc.finite)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    code[i] = pack_fp8(x[v][4 * i][c] * inv, x[v][4 * i + 1][c] * inv, x[v][4 * i + 2][c] * inv, x[v][4 * i + 3][c] * inv);
+            uint8_t *at = codes + ((size_t)(d + (uint32_t)c) << kv.page_shift) + slot0;
+            if (slot0 >= lo && slot0 + 16 <= hi) {
+                *(u32x4_t *)at = code;
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 16; i++)
+                    if (slot0 + i >= lo && slot0 + i < hi) at[i] = (uint8_t)(code[i / 4] >> (8 * (i % 4)));
             }
-        } else if (halved(A, g)) {
-            *(uint32_t *)(codes + (size_t)slot * kv.head_dim + 4 * g) = a;
-            *(uint32_t *)(codes + (size_t)slot * kv.head_dim + 4 * g + A.rot_dim / 2) = b;
-        } else {  // lo and hi alternate
-            const uint32_t c = (a & 0xFFu) | (b & 0xFFu) << 8 | (a & 0xFF00u) << 8 | (b & 0xFF00u) << 16;
-            const uint32_t d = (a >> 16 & 0xFFu) | (b >> 16 & 0xFFu) << 8 | (a >> 24) << 16 | (b >> 24) << 24;
-            *(u32x2_t *)(codes + (size_t)slot * kv.head_dim + 8 * g) = u32x2_t{c, d};
         }
     }
 }
@@ -284,12 +418,22 @@ static void launch_lanes(hipStream_t s, const KvAppendArgs &A, uint32_t page_blo
 hipError_t kv_append_launch(hipStream_t s, const KvAppendArgs &A) {
     const KvArgs &kv = A.kv;
     const uint64_t P = 1u << kv.page_shift;
-    // n new tokens touch at most (n + 2 P - 2) / P pages, one token one
-    const uint64_t pages = kv.max_new == 1 ? kv.sequences : (kv.tokens + kv.sequences * (2 * P - 2)) / P;
+    // n new tokens touch at most (n + 2 P - 2) / P pages
+    const uint64_t pages = (kv.tokens + kv.sequences * (2 * P - 2)) / P;
     const uint64_t page_blocks = pages * 2 * kv.kv_heads, grid = page_blocks + (A.q ? kv.tokens : 0);
     if (grid > 0x7FFFFFFFull) return hipErrorInvalidValue;
     if (grid == 0) return hipSuccess;
     const uint32_t groups = kv.head_dim / 8;
+    if (kv.max_new == 1) {
+        const uint32_t lanes = groups <= 4 ? 4 : groups <= 8 ? 8 : groups <= 16 ? 16 : 32;
+        const uint32_t blocks = ((2 * kv.kv_heads + (A.q ? A.q_heads : 0)) * lanes + kAppendThreads - 1) / kAppendThreads;
+        const dim3 one(kv.sequences * blocks), threads(kAppendThreads);
+        if (lanes == 4) hipLaunchKernelGGL(kv_append_one_kernel<4>, one, threads, 0, s, A, blocks);
+        else if (lanes == 8) hipLaunchKernelGGL(kv_append_one_kernel<8>, one, threads, 0, s, A, blocks);
+        else if (lanes == 16) hipLaunchKernelGGL(kv_append_one_kernel<16>, one, threads, 0, s, A, blocks);
+        else hipLaunchKernelGGL(kv_append_one_kernel<32>, one, threads, 0, s, A, blocks);
+        return hipGetLastError();
+    }
     if (groups <= 4) launch_lanes<4>(s, A, (uint32_t)page_blocks, (uint32_t)grid);
     else if (groups <= 8) launch_lanes<8>(s, A, (uint32_t)page_blocks, (uint32_t)grid);
     else if (groups <= 16) launch_lanes<16>(s, A, (uint32_t)page_blocks, (uint32_t)grid);

@@ -62,6 +62,7 @@ hipError_t attention_launch(hipStream_t s, const AttentionArgs &A, void *workspa
 
 // ---- device ---------------------------------------------------------------------------------------------------------
 
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
@@ -85,50 +86,45 @@ __device__ __forceinline__ void store_elem(void *p, int type, size_t i, float v)
     if (type == ELEM_F32) ((float *)p)[i] = v;
     else ((uint16_t *)p)[i] = (uint16_t)(type == ELEM_BF16 ? f32_to_bf16_rne(v) : f32_to_f16_bits(v));
 }
-// 8 elements from an element offset at which the address is 16-byte aligned
-__device__ __forceinline__ void load8(const void *p, int type, size_t i, float (&o)[8]) {
-    if (type == ELEM_F32) {
-        const f32x4_t a = *(const f32x4_t *)((const float *)p + i), b = *(const f32x4_t *)((const float *)p + i + 4);
-#pragma unroll
-        for (int j = 0; j < 4; j++) o[j] = a[j], o[4 + j] = b[j];
-        return;
-    }
-    const u32x4_t a = *(const u32x4_t *)((const uint16_t *)p + i);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        o[2 * j] = type == ELEM_BF16 ? bf16_bits_to_f32(a[j] & 0xFFFFu) : f16_bits_to_f32(a[j] & 0xFFFFu);
-        o[2 * j + 1] = type == ELEM_BF16 ? __builtin_bit_cast(float, a[j] & 0xFFFF0000u) : f16_bits_to_f32(a[j] >> 16);
-    }
+// Groups of elements from an offset at which the address is aligned to the group, at most 16 bytes.  (By value: stores through references that
+// both sides of a branch make would keep the array in memory.)
+__device__ __forceinline__ f32x4_t unpack4(int type, u32x2_t a) {
+    if (type == ELEM_BF16)
+        return f32x4_t{bf16_bits_to_f32(a[0]), __builtin_bit_cast(float, a[0] & 0xFFFF0000u), bf16_bits_to_f32(a[1]), __builtin_bit_cast(float, a[1] & 0xFFFF0000u)};
+    return f32x4_t{f16_bits_to_f32(a[0] & 0xFFFFu), f16_bits_to_f32(a[0] >> 16), f16_bits_to_f32(a[1] & 0xFFFFu), f16_bits_to_f32(a[1] >> 16)};
 }
 __device__ __forceinline__ uint32_t pack2(int type, float a, float b) {
     return type == ELEM_BF16 ? f32_to_bf16_rne(a) | f32_to_bf16_rne(b) << 16 : f32_to_f16_bits(a) | f32_to_f16_bits(b) << 16;
 }
-__device__ __forceinline__ void store8(void *p, int type, size_t i, const float (&v)[8]) {
-    if (type == ELEM_F32) {
-        *(f32x4_t *)((float *)p + i) = f32x4_t{v[0], v[1], v[2], v[3]};
-        *(f32x4_t *)((float *)p + i + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
-        return;
-    }
-    *(u32x4_t *)((uint16_t *)p + i) = u32x4_t{pack2(type, v[0], v[1]), pack2(type, v[2], v[3]), pack2(type, v[4], v[5]), pack2(type, v[6], v[7])};
+__device__ __forceinline__ f32x2_t load2(const void *p, int type, size_t i) {
+    if (type == ELEM_F32) return *(const f32x2_t *)((const float *)p + i);
+    const f32x4_t v = unpack4(type, u32x2_t{*(const uint32_t *)((const uint16_t *)p + i), 0u});
+    return f32x2_t{v[0], v[1]};
 }
-// 4 elements, 8-byte (16 bits) or 16-byte (f32) aligned
-__device__ __forceinline__ void load4(const void *p, int type, size_t i, float (&o)[4]) {
-    if (type == ELEM_F32) {
-        const f32x4_t a = *(const f32x4_t *)((const float *)p + i);
-#pragma unroll
-        for (int j = 0; j < 4; j++) o[j] = a[j];
-        return;
-    }
-    const u32x2_t a = *(const u32x2_t *)((const uint16_t *)p + i);
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-        o[2 * j] = type == ELEM_BF16 ? bf16_bits_to_f32(a[j] & 0xFFFFu) : f16_bits_to_f32(a[j] & 0xFFFFu);
-        o[2 * j + 1] = type == ELEM_BF16 ? __builtin_bit_cast(float, a[j] & 0xFFFF0000u) : f16_bits_to_f32(a[j] >> 16);
-    }
+__device__ __forceinline__ f32x4_t load4(const void *p, int type, size_t i) {
+    if (type == ELEM_F32) return *(const f32x4_t *)((const float *)p + i);
+    return unpack4(type, *(const u32x2_t *)((const uint16_t *)p + i));
 }
-__device__ __forceinline__ void store4(void *p, int type, size_t i, const float (&v)[4]) {
-    if (type == ELEM_F32) *(f32x4_t *)((float *)p + i) = f32x4_t{v[0], v[1], v[2], v[3]};
+__device__ __forceinline__ void store4(void *p, int type, size_t i, f32x4_t v) {
+    if (type == ELEM_F32) *(f32x4_t *)((float *)p + i) = v;
     else *(u32x2_t *)((uint16_t *)p + i) = u32x2_t{pack2(type, v[0], v[1]), pack2(type, v[2], v[3])};
+}
+struct Eight {
+    f32x4_t a, b;
+    __device__ __forceinline__ float operator[](int i) const { return i < 4 ? a[i] : b[i - 4]; }
+};
+__device__ __forceinline__ Eight load8(const void *p, int type, size_t i) {
+    if (type == ELEM_F32) return {*(const f32x4_t *)((const float *)p + i), *(const f32x4_t *)((const float *)p + i + 4)};
+    const u32x4_t v = *(const u32x4_t *)((const uint16_t *)p + i);
+    return {unpack4(type, u32x2_t{v[0], v[1]}), unpack4(type, u32x2_t{v[2], v[3]})};
+}
+__device__ __forceinline__ void store8(void *p, int type, size_t i, const Eight &v) {
+    if (type == ELEM_F32) {
+        *(f32x4_t *)((float *)p + i) = v.a;
+        *(f32x4_t *)((float *)p + i + 4) = v.b;
+        return;
+    }
+    *(u32x4_t *)((uint16_t *)p + i) = u32x4_t{pack2(type, v.a[0], v.a[1]), pack2(type, v.a[2], v.a[3]), pack2(type, v.b[0], v.b[1]), pack2(type, v.b[2], v.b[3])};
 }
 
 // The page of a sequence's token at `key` (its table's row at `table`), or ~0: a hole, or beyond the table.

@@ -39,7 +39,9 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_norm_kernel(No
     const auto at = [&](int c, int j) -> uint32_t { return VEC ? (t + (uint32_t)c * TPR) * 8 + (uint32_t)j : t + (uint32_t)(c * 8 + j) * TPR; };
     const auto get = [&](const void *p, int type, int c, float (&o)[8]) {
         if constexpr (VEC) {
-            load8(p, type, at(c, 0), o);
+            const Eight v = load8(p, type, at(c, 0));
+#pragma unroll
+            for (int j = 0; j < 8; j++) o[j] = v[j];
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++) o[j] = at(c, j) < A.hidden ? load_elem(p, type, at(c, j)) : 0.f;
@@ -47,7 +49,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_norm_kernel(No
     };
     const auto put = [&](void *p, int type, int c, const float (&v)[8]) {
         if constexpr (VEC) {
-            store8(p, type, at(c, 0), v);
+            store8(p, type, at(c, 0), Eight{f32x4_t{v[0], v[1], v[2], v[3]}, f32x4_t{v[4], v[5], v[6], v[7]}});
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++)

@@ -891,14 +891,18 @@ def test_an_empty_batch_needs_no_workspace(field):
 
 @gpu
 def test_refused_calls_answer_false_with_a_reason_and_empty_ones_do_nothing(be):
-    s = _sound()
-    s["cache"].head_dim = 48
-    assert not be.dev_kv_append(s["cache"], s["batch"], s["app"]) and "head_dim" in be.last_error()
-    assert be.plan_create_attention(s["cache"], s["batch"], s["att"], 4096, 1 << 30) is None
-    s = _sound()
-    assert not be.dev_attention(s["cache"], s["batch"], s["att"], 4096, 16) and "workspace" in be.last_error()
-    s["batch"].tokens = 0
-    assert be.dev_kv_append(s["cache"], s["batch"], s["app"]) and be.dev_attention(s["cache"], s["batch"], s["att"], 0, 0)
-    plan = be.plan_create_attention(s["cache"], s["batch"], s["att"], 0, 0)
+    layer = Layer(be, np.random.default_rng(30), [(1, 40), (2, 700)])  # (every pointer is one of a buffer, should a call be served after all)
+    cache, batch, ws, n = layer.cache, layer.batch, layer.ws, layer.ws_bytes
+    cache.head_dim = 48
+    assert not be.dev_kv_append(cache, batch, layer.app) and "head_dim" in be.last_error()
+    assert be.plan_create_attention(cache, batch, layer.att, ws, n) is None
+    cache.head_dim = layer.d
+    assert not be.dev_attention(cache, batch, layer.att, ws, n - 1) and "workspace" in be.last_error()
+    before = layer.results()
+    batch.tokens = 0
+    assert be.dev_kv_append(cache, batch, layer.app) and be.dev_attention(cache, batch, layer.att, 0, 0)
+    plan = be.plan_create_attention(cache, batch, layer.att, 0, 0)
     assert plan and be.plan_launch_count(plan) == 0 and be.plan_run(plan)
     be.plan_destroy(plan)
+    for got, want in zip(layer.results(), before):
+        assert (got.view(np.uint8) == want.view(np.uint8)).all()
