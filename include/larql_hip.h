@@ -588,7 +588,7 @@ typedef struct {
  * the queries, normed (q_norm) and rotated alike, to q_out (q NULL: none).  Channel pairs (i, i + rot_dim/2), or
  * (2i, 2i+1) where `interleaved`, of the first rot_dim channels turn by position * inv_freq[i] (the angle is reduced in 64
  * bits) and are scaled by rope_scale; rot_dim 0: no rotation.  Positions count from the sequence's first token.  Rows are
- * [heads, head_dim], strides elements between tokens (k, v and q may be parts of one fused row); q_out may be q.
+ * [heads, head_dim], strides elements between tokens, at most 2^22 (k, v and q may be parts of one fused row); q_out may be q.
  * Two sequences must not append to one page.  Appending the same tokens again changes nothing. */
 typedef struct {
     int format;                    /* of q, k, v and q_out */

@@ -2646,6 +2646,8 @@ static int check_kv_append(larql_hip_ctx *c, const larql_hip_kv_cache *k, const 
         (with_q && (!row_fits(a->q, a->q_stride, A.type, a->q_heads, k->head_dim) ||
                     !row_fits(a->q_out, a->q_out_stride, A.type, a->q_heads, k->head_dim))))
         return fail(c, LARQL_REFUSED_SHAPE, "kv_append: rows must be 16-byte aligned and hold all heads");
+    if (std::max(a->k_stride, a->v_stride) > kMaxRowStride || (with_q && std::max(a->q_stride, a->q_out_stride) > kMaxRowStride))
+        return fail(c, LARQL_UNSUPPORTED, "kv_append: strides of more than 2^22 elements");
     if (((uintptr_t)a->q_norm | (uintptr_t)a->k_norm) & 15) return fail(c, LARQL_REFUSED_SHAPE, "kv_append: norm weights must be 16-byte aligned");
     if ((uintptr_t)a->inv_freq & 3) return fail(c, LARQL_REFUSED_SHAPE, "kv_append: inv_freq must be 4-byte aligned");
     A.q = with_q ? a->q : nullptr; A.k = a->k; A.v = a->v; A.q_out = a->q_out;

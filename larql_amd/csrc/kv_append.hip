@@ -18,14 +18,14 @@ struct Quad {
 
 // Channels of the pairs 4g .. 4g+3: (p, p + rot/2) inside the rotated part of a halved layout, else (2p, 2p + 1).
 __device__ __forceinline__ bool halved(const KvAppendArgs &A, uint32_t g) { return !A.interleaved && 8 * g < A.rot_dim; }
-__device__ __forceinline__ Quad load_quad(const KvAppendArgs &A, const void *row, int type, size_t at, uint32_t g) {
+__device__ __forceinline__ Quad load_quad(const KvAppendArgs &A, const void *row, int type, uint32_t at, uint32_t g) {
     const bool h = halved(A, g);
-    const size_t a = at + (h ? 4 * g : 8 * g), b = at + (h ? 4 * g + A.rot_dim / 2 : 8 * g + 4);
+    const uint32_t a = at + (h ? 4 * g : 8 * g), b = at + (h ? 4 * g + A.rot_dim / 2 : 8 * g + 4);
     const f32x4_t u = load4(row, type, a), v = load4(row, type, b);
     if (h) return {u, v};
     return {f32x4_t{u[0], u[2], v[0], v[2]}, f32x4_t{u[1], u[3], v[1], v[3]}};
 }
-__device__ __forceinline__ void store_quad(const KvAppendArgs &A, void *row, int type, size_t at, uint32_t g, const Quad &q) {
+__device__ __forceinline__ void store_quad(const KvAppendArgs &A, void *row, int type, uint32_t at, uint32_t g, const Quad &q) {
     if (halved(A, g)) {
         store4(row, type, at + 4 * g, q.lo);
         store4(row, type, at + 4 * g + A.rot_dim / 2, q.hi);
@@ -206,8 +206,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_one_kernel(KvAppendA
     Quad x = {}, w = {};
     f32x4_t freq = {0.f, 0.f, 0.f, 0.f};
     if (in_head) {
-        const void *src = is_k ? A.k : is_v ? A.v : A.q;
-        const size_t at = t.row * (is_k ? A.k_stride : is_v ? A.v_stride : A.q_stride) + (size_t)h * kv.head_dim;
+        const void *src = (const char *)(is_k ? A.k : is_v ? A.v : A.q) + t.row * (is_k ? A.k_stride : is_v ? A.v_stride : A.q_stride) * elem_bytes(A.type);
+        const uint32_t at = h * kv.head_dim;
         if (is_v) {
             const Eight v = load8(src, A.type, at + 8 * g);
             x = {v.a, v.b};
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_one_kernel(KvAppendA
     uint32_t amax = quad_amax(x);
 #pragma unroll
     for (uint32_t m = 1; m < LPH; m *= 2) amax = max(amax, (uint32_t)__shfl_xor((int)amax, (int)m, 64));
-    if (is_q && in_head) store_quad(A, A.q_out, A.type, t.row * A.q_out_stride + (size_t)h * kv.head_dim, g, x);
+    if (is_q && in_head) store_quad(A, (char *)A.q_out + t.row * A.q_out_stride * elem_bytes(A.type), A.type, h * kv.head_dim, g, x);
     if (!stored) return;
     const Scale sc = scale_of(amax, slot != 0, old_scale);
     uint8_t *codes = (is_v ? kv.v_codes : kv.k_codes) + of_page * ((size_t)kv.head_dim << kv.page_shift);
@@ -281,28 +281,28 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendArgs 
     f32x4_t freq = {0.f, 0.f, 0.f, 0.f};
     if (blockIdx.x >= page_blocks) {  // the queries of one token
         const uint32_t token = blockIdx.x - page_blocks, first = threadIdx.x / LPH;
-        const auto load = [&](uint32_t head) {
-            return load_quad(A, A.q, A.type, token * A.q_stride + (size_t)min(head, A.q_heads - 1) * kv.head_dim, g);
-        };
-        Quad q[4];
+        const char *src = (const char *)A.q + token * A.q_stride * elem_bytes(A.type);
+        char *dst = (char *)A.q_out + token * A.q_out_stride * elem_bytes(A.type);
+        const auto load = [&](uint32_t head) { return load_quad(A, src, A.type, min(head, A.q_heads - 1) * kv.head_dim, g); };
+        Quad q[2];  // (loads that nothing before them decides: they leave first, and the next heads' before these are done)
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++) q[i] = load(first + i * kTokens);
+        for (uint32_t i = 0; i < 2; i++) q[i] = load(first + i * kTokens);
         if (turns) freq = load_freq(A, g);
         if (A.q_norm) w = load_quad(A, A.q_norm, ELEM_F32, 0, g);
         NewTokens t;
         if (!find_token(kv, token, t)) return;
         Turn turn;
         if (turns) turn_of(A, t.len - (int32_t)t.n + (int32_t)(token - t.row), freq, turn);
-        for (uint32_t head0 = 0; head0 < A.q_heads; head0 += 4 * kTokens) {
+        for (uint32_t head0 = 0; head0 < A.q_heads; head0 += 2 * kTokens) {
 #pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
+            for (uint32_t i = 0; i < 2; i++) {
                 const uint32_t head = head0 + first + i * kTokens;
                 Quad y = q[i];
-                q[i] = load(head + 4 * kTokens);
+                if (head0 + 2 * kTokens < A.q_heads) q[i] = load(head + 2 * kTokens);
                 if (!in_head) y = {};
                 if (A.q_norm) norm_quad<LPH>(A, y, w);
                 if (turns) rotate(y, turn);
-                if (in_head && head < A.q_heads) store_quad(A, A.q_out, A.type, token * A.q_out_stride + (size_t)head * kv.head_dim, g, y);
+                if (in_head && head < A.q_heads) store_quad(A, dst, A.type, head * kv.head_dim, g, y);
             }
         }
         return;
@@ -320,8 +320,11 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendArgs 
     float *scale_at = (is_v ? kv.v_scales : kv.k_scales) + (size_t)page * kv.kv_heads + head;
     const float old_scale = lo ? *scale_at : 1.f;
     uint8_t *codes = (is_v ? kv.v_codes : kv.k_codes) + ((size_t)page * kv.kv_heads + head) * ((size_t)kv.head_dim << kv.page_shift);
-    // the row of a slot (of the nearest new one: loads need no condition)
-    const auto row_of = [&](uint32_t slot) { return t.row + (size_t)((int32_t)(base + min(max(slot, lo), hi - 1)) - first); };
+    // this head's elements of the page's first new token, and how far a slot's are from there (the nearest new slot's: loads need no condition)
+    const char *src = (const char *)(is_v ? A.v : A.k) +
+                      ((t.row + (size_t)((int32_t)(base + lo) - first)) * (is_v ? A.v_stride : A.k_stride) + (size_t)head * kv.head_dim) * elem_bytes(A.type);
+    const uint32_t stride = (uint32_t)(is_v ? A.v_stride : A.k_stride);  // (at most kMaxRowStride: 128 rows within 32 bits)
+    const auto off_of = [&](uint32_t slot) { return (min(max(slot, lo), hi - 1) - lo) * stride; };
     const auto page_scale = [&](uint32_t amax) {
         amax = wave_max_u32(amax);
         if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = amax;
@@ -337,7 +340,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendArgs 
         Quad x[NP];
 #pragma unroll
         for (int p = 0; p < NP; p++)
-            x[p] = load_quad(A, A.k, A.type, row_of((uint32_t)p * kTokens + threadIdx.x / LPH) * A.k_stride + (size_t)head * kv.head_dim, g);
+            x[p] = load_quad(A, src, A.type, off_of((uint32_t)p * kTokens + threadIdx.x / LPH), g);
         if (turns) freq = load_freq(A, g);
         if (A.k_norm) w = load_quad(A, A.k_norm, ELEM_F32, 0, g);
 #pragma unroll
@@ -368,7 +371,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendArgs 
     for (int v = 0; v < NV; v++) {
         const uint32_t u = min(threadIdx.x + (uint32_t)v * kAppendThreads, units - 1), d = u % pairs * 2, slot0 = u / pairs * 16;
 #pragma unroll
-        for (int i = 0; i < 16; i++) x[v][i] = load2(A.v, A.type, row_of(slot0 + (uint32_t)i) * A.v_stride + (size_t)head * kv.head_dim + d);
+        for (int i = 0; i < 16; i++) x[v][i] = load2(src, A.type, off_of(slot0 + (uint32_t)i) + d);
     }
 #pragma unroll
     for (int v = 0; v < NV; v++)  // (other threads' units and other slots' rows: elements of this page's new tokens all the same)

@@ -44,6 +44,7 @@ struct KvAppendArgs {
     uint32_t q_heads, rot_dim, interleaved;
     float rope_scale, norm_offset, norm_eps;
 };
+constexpr size_t kMaxRowStride = 1u << 22;  // elements between tokens
 hipError_t kv_append_launch(hipStream_t s, const KvAppendArgs &A);
 
 struct AttentionArgs {
@@ -96,12 +97,12 @@ __device__ __forceinline__ f32x4_t unpack4(int type, u32x2_t a) {
 __device__ __forceinline__ uint32_t pack2(int type, float a, float b) {
     return type == ELEM_BF16 ? f32_to_bf16_rne(a) | f32_to_bf16_rne(b) << 16 : f32_to_f16_bits(a) | f32_to_f16_bits(b) << 16;
 }
-__device__ __forceinline__ f32x2_t load2(const void *p, int type, size_t i) {
+__device__ __forceinline__ f32x2_t load2(const void *p, int type, uint32_t i) {
     if (type == ELEM_F32) return *(const f32x2_t *)((const float *)p + i);
     const f32x4_t v = unpack4(type, u32x2_t{*(const uint32_t *)((const uint16_t *)p + i), 0u});
     return f32x2_t{v[0], v[1]};
 }
-__device__ __forceinline__ f32x4_t load4(const void *p, int type, size_t i) {
+__device__ __forceinline__ f32x4_t load4(const void *p, int type, uint32_t i) {
     if (type == ELEM_F32) return *(const f32x4_t *)((const float *)p + i);
     return unpack4(type, *(const u32x2_t *)((const uint16_t *)p + i));
 }
