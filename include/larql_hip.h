@@ -612,7 +612,7 @@ int larql_hip_dev_kv_append(larql_hip_ctx *ctx, const larql_hip_kv_cache *cache,
                             const larql_hip_kv_append *args);
 
 /* Attention of the new tokens over their sequences' pages: query head i reads key/value head i / (q_heads / kv_heads).
- * x = scale * q.k, softcap * tanh(x / softcap) where softcap > 0; a query at position p sees keys <= p (`causal`) and
+ * x = scale * q.k, softcap * tanh(x / softcap) where softcap is not 0 (then at least 2^-20); a query at position p sees keys <= p (`causal`) and
  * > p - window (window > 0); `sinks` [q_heads] (or NULL) adds exp(sink) to the sum of the weights.  A query that sees
  * nothing gives zeros.  Sums are f32; where `out` is f32 queries and weights enter the matrix instructions as f16 pairs
  * (about 22 bits), otherwise as one f16 each.  Results may differ in their last bits with the batch around a sequence: long

@@ -2670,8 +2670,8 @@ static int check_attention(larql_hip_ctx *c, const larql_hip_kv_cache *k, const 
         return fail(c, LARQL_REFUSED_SHAPE, "attention: q_heads is a multiple of the key/value heads");
     if (b->tokens * (a->q_heads / k->kv_heads) > (1u << 28)) return fail(c, LARQL_UNSUPPORTED, "attention: too many query rows");
     if (a->window > 0x7FFFFFFFull) return fail(c, LARQL_UNSUPPORTED, "attention: window too large");
-    if (!(a->softcap >= 0.f) || !std::isfinite(a->softcap) || !std::isfinite(a->scale))
-        return fail(c, LARQL_REFUSED_SHAPE, "attention: scale and softcap are finite, softcap is not negative");
+    if (!(a->softcap == 0.f || a->softcap >= 0x1p-20f) || !std::isfinite(a->softcap) || !std::isfinite(a->scale))
+        return fail(c, LARQL_REFUSED_SHAPE, "attention: scale and softcap are finite, softcap 0 or at least 2^-20");
     if (!a->q || !a->out) return LARQL_E_ARG;
     if (!row_fits(a->q, a->q_stride, A.q_type, a->q_heads, k->head_dim) || !row_fits(a->out, a->out_stride, A.out_type, a->q_heads, k->head_dim))
         return fail(c, LARQL_REFUSED_SHAPE, "attention: rows must be 16-byte aligned and hold all heads");

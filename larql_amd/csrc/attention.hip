@@ -39,13 +39,14 @@ struct Plan {
     uint32_t target;              // pieces of one head's work that long rows are split into
     uint32_t min_steps;           // steps of a piece at least
     uint32_t split;               // whether rows are split at all
+    int fits;                     // how often pieces are made longer to meet the target
 };
 
-// A sequence's share of the work: its query rows in tiles, and the steps of keys that any of them sees.
+// A sequence's share of the work: its query rows in tiles, and at most how many steps of keys one of them sees.
 struct Share {
     uint32_t row, n;      // first row of the activations, new tokens
     int32_t len, first;   // keys, position of the first new token
-    uint32_t tiles, step_lo, steps;
+    uint32_t tiles, steps;
 };
 __device__ __forceinline__ Share share_of(const AttentionArgs &A, const Plan &P, uint32_t s, uint32_t group) {
     const NewTokens t = new_tokens(A.kv, s);
@@ -56,49 +57,58 @@ __device__ __forceinline__ Share share_of(const AttentionArgs &A, const Plan &P,
     h.first = t.len - (int32_t)t.n;
     const uint32_t rows = t.n * group;
     h.tiles = rows < P.rows_min || rows > P.rows_max ? 0u : (rows + P.tile - 1) / P.tile;
-    const int32_t lo = A.window ? (int32_t)max((int64_t)h.first - (int64_t)A.window + 1, (int64_t)0) : 0;
-    h.step_lo = (uint32_t)lo / kStep;
-    h.steps = h.tiles && h.len > lo ? ((uint32_t)h.len + kStep - 1) / kStep - h.step_lo : 0;
+    h.steps = h.tiles ? ((uint32_t)h.len + kStep - 1) / kStep : 0;
+    if (A.window) h.steps = min((uint64_t)h.steps, ((uint64_t)A.window + P.tile / group + 1) / kStep + 2);  // (a tile's tokens may straddle)
     return h;
 }
 
 // What the wavefront that serves item `item` of a head works on; false beyond the last.  Every wavefront finds it from the lengths:
-// tiles of sequences in order, each tile's keys in pieces of `chunk` steps, as many as P.target asks for.  Pieces of split tiles
+// tiles of sequences in order, the keys that a tile sees in equal pieces, as many as P.target asks for.  Pieces of split tiles
 // have places for their partial results, `slot` on; `split_tiles`: items count split tiles instead.
 struct Item {
-    uint32_t s, tile, piece, pieces, chunk, slot;
+    uint32_t s, tile, piece, pieces, slot;
+    // the steps of this piece, of those from `first` to before `end` that its tile sees
+    __device__ __forceinline__ uint32_t begin_of(uint32_t first, uint32_t end) const { return first + piece * ((end - first + pieces - 1) / pieces); }
+    __device__ __forceinline__ uint32_t end_of(uint32_t first, uint32_t end) const {
+        return min(first + (piece + 1) * ((end - first + pieces - 1) / pieces), end);
+    }
 };
-__device__ __forceinline__ bool find_item(const AttentionArgs &A, const Plan &P, uint32_t item, bool split_tiles, Item &it) {
+__device__ __forceinline__ bool find_item(const AttentionArgs &A, const Plan &P, uint32_t item, bool split_tiles, Item &it, Share &sh) {
     const uint32_t lane = threadIdx.x % 64, group = A.q_heads / A.kv.kv_heads;
-    it.chunk = 0x7FFFFFFFu;
+    const auto share_at = [&](uint32_t s) { return s < A.kv.sequences ? share_of(A, P, s, group) : Share{}; };
+    const auto pieces_of = [](const Share &h, uint32_t chunk) { return max(h.steps / chunk + (h.steps % chunk ? 1u : 0u), 1u); };
+    const Share first = share_at(lane);  // (read once where 64 sequences are all)
+    const auto sum_of = [&](auto f) {  // over the sequences; a sum that need not be exact
+        float v = f(first);
+        for (uint32_t base = 64; base < A.kv.sequences; base += 64) v += f(share_at(base + lane));
+        return wave_fsum(v);
+    };
+    uint32_t chunk = 0x7FFFFFFFu;  // steps of a piece
     if (P.split) {
-        float units = 0.f;  // (tiles x steps; their sum need not be exact)
-        for (uint32_t base = 0; base < A.kv.sequences; base += 64)
-            if (base + lane < A.kv.sequences) {
-                const Share h = share_of(A, P, base + lane, group);
-                units += (float)h.tiles * (float)h.steps;
-            }
-        it.chunk = max((uint32_t)ceilf(wave_fsum(units) / (float)P.target), P.min_steps);
+        chunk = max((uint32_t)ceilf(sum_of([](const Share &h) { return (float)h.tiles * (float)h.steps; }) / (float)P.target), P.min_steps);
+        for (int i = 0; i < P.fits; i++) {  // pieces are whole: longer ones, until the items are as few as asked for
+            if (sum_of([&](const Share &h) { return (float)h.tiles * (float)pieces_of(h, chunk); }) <= (float)P.target) break;
+            chunk += chunk / 8 + 1;
+        }
     }
     it.slot = 0;
     for (uint32_t base = 0; base < A.kv.sequences; base += 64) {
-        uint32_t tiles = 0, pieces = 1;
-        if (base + lane < A.kv.sequences) {
-            const Share h = share_of(A, P, base + lane, group);
-            tiles = h.tiles;
-            pieces = max(h.steps / it.chunk + (h.steps % it.chunk ? 1u : 0u), 1u);
-        }
+        const Share h = base ? share_at(base + lane) : first;
+        const uint32_t tiles = h.tiles, pieces = pieces_of(h, chunk);
         const uint32_t slots = pieces > 1 ? tiles * pieces : 0u, weight = split_tiles ? (pieces > 1 ? tiles : 0u) : tiles * pieces;
         const uint32_t upto = wave_inclusive_sum(weight), all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
         const uint32_t slots_upto = P.split ? wave_inclusive_sum(slots) : 0u;
         if (item < all) {
             const int at = (int)__builtin_ctzll(__ballot(upto > item));
-            it.pieces = (uint32_t)__builtin_amdgcn_readlane((int)pieces, at);
-            const uint32_t in = item - (uint32_t)__builtin_amdgcn_readlane((int)(upto - weight), at);
+            const auto of_it = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
+            it.pieces = of_it(pieces);
+            const uint32_t in = item - of_it(upto - weight);
             it.s = base + (uint32_t)at;
             it.tile = split_tiles ? in : in / it.pieces;
             it.piece = split_tiles ? 0 : in % it.pieces;
-            it.slot += (uint32_t)__builtin_amdgcn_readlane((int)(slots_upto - slots), at) + it.tile * it.pieces;
+            it.slot += of_it(slots_upto - slots) + it.tile * it.pieces;
+            sh.row = of_it(h.row), sh.n = of_it(h.n), sh.len = (int32_t)of_it((uint32_t)h.len), sh.first = (int32_t)of_it((uint32_t)h.first);
+            sh.tiles = of_it(tiles), sh.steps = of_it(h.steps);
             return true;
         }
         item -= all;
@@ -127,9 +137,9 @@ static Plans plans_of(const AttentionArgs &A) {
     Plans p;
     // Pieces of few rows: as many as workgroups are resident, 2 a compute unit above 128 channels (131072 keys of 256, us with 1, 2, 3, 4 of
     // them: 148, 103, 125, 110, joining included), 3 below (64 sequences, 64 channels: 44, 37, 33, 37); a wavefront's step each at least.
-    p.rows = {kRowsTile, 1, kFewRows, std::max((A.kv.head_dim > 128 ? 2 : 3) * cus / A.kv.kv_heads, 1u), kAttnWaves, 1};
+    p.rows = {kRowsTile, 1, kFewRows, std::max((A.kv.head_dim > 128 ? 2 : 3) * cus / A.kv.kv_heads, 1u), kAttnWaves, 1, 0};
     p.rows.split = steps > p.rows.min_steps;
-    p.tiles = {kTilesTile, kFewRows + 1, 0xFFFFFFFFu, std::max((A.kv.head_dim > 128 ? 1 : 2) * cus / A.kv.kv_heads, 1u), 8, 1};
+    p.tiles = {kTilesTile, kFewRows + 1, 0xFFFFFFFFu, std::max((A.kv.head_dim > 128 ? 1 : 2) * cus / A.kv.kv_heads, 1u), 8, 1, 6};
     p.tiles.split = steps > p.tiles.min_steps && A.kv.tokens * group / p.tiles.tile + A.kv.sequences < p.tiles.target;
     p.use_tiles = most > kFewRows;
     p.use_rows = !p.use_tiles || A.kv.sequences > 1;
@@ -171,13 +181,13 @@ __device__ __forceinline__ float inverse_sum(const AttentionArgs &A, float l, fl
     return l == 0.f ? 0.f : 1.f / l;
 }
 
-// The logarithm (base 2) of a score's weight, plus e: s a + e, or with the cap on s a (natural units) in between.
+// The logarithm (base 2) of a score's weight, plus e: s a + e, or with the cap in between.
 template <bool CAP>
 __device__ __forceinline__ float score(const AttentionArgs &A, float s, float a, float e) {
     if constexpr (!CAP) return fmaf(s, a, e);
-    // cap * tanh(s / cap) = cap - 2 cap / (exp(2 s / cap) + 1)
-    const float z = __builtin_amdgcn_exp2f(s * a * (2.f * kLog2E / A.softcap));
-    return fmaf(A.softcap - 2.f * A.softcap * __builtin_amdgcn_rcpf(z + 1.f), kLog2E, e);
+    // cap * tanh(s / cap) = cap - 2 cap / (exp(2 s / cap) + 1), `a` with the factor 2 log2(e) / cap (query_f16)
+    const float c = A.softcap * kLog2E;
+    return fmaf(-2.f * c, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a) + 1.f), c + e);
 }
 
 // A query row's elements (spread over lanes 32 apart, and 16 apart where QUARTERS) as f16 or f16 pairs after a power-of-two scale that brings
@@ -204,7 +214,7 @@ __device__ __forceinline__ float query_f16(const AttentionArgs &A, const Eight (
             f16x8_t rest;
             weights_f16<PAIRS>(x, qh[k], PAIRS ? ql[PAIRS ? k : 0] : rest, i);
         }
-    const float factor = fabsf(A.scale) * (CAP ? 1.f : kLog2E) * __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+    const float factor = fabsf(A.scale) * (CAP ? 2.f * kLog2E / A.softcap : kLog2E) * __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
     return finite ? factor : __builtin_nanf("");
 }
 
@@ -233,8 +243,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(Attenti
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = lane % 16, g = lane / 16;
     const uint32_t kvh = blockIdx.y, group = A.q_heads / kv.kv_heads;
     Item it;
-    if (!find_item(A, P, blockIdx.x, false, it)) return;
-    const Share sh = share_of(A, P, it.s, group);
+    Share sh;
+    if (!find_item(A, P, blockIdx.x, false, it, sh)) return;
     const uint32_t rows = sh.n * group;
 
     // The lane's query row: token and head, what it sees.  What all and any of the rows see: the first and the last say it.
@@ -248,9 +258,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(Attenti
     const uint32_t last_row = min(row0 + kRowsTile - 1, rows - 1);
     const int32_t all_hi = hi_of(row0), any_hi = hi_of(last_row), any_lo = lo_of(row0), all_lo = lo_of(last_row);
 
-    const uint64_t piece_lo = (uint64_t)sh.step_lo + (uint64_t)it.piece * it.chunk;
-    const uint32_t end = any_hi < 0 ? 0u : (uint32_t)min(min(piece_lo + it.chunk, (uint64_t)(sh.step_lo + sh.steps)), (uint64_t)((uint32_t)any_hi / kStep + 1));
-    uint32_t step = (uint32_t)max(piece_lo, (uint64_t)((uint32_t)any_lo / kStep)) + wave;
+    const uint32_t tile_end = any_hi < any_lo ? 0u : (uint32_t)any_hi / kStep + 1, tile_begin = min((uint32_t)any_lo / kStep, tile_end);
+    const uint32_t end = it.end_of(tile_begin, tile_end);
+    uint32_t step = it.begin_of(tile_begin, tile_end) + wave;
 
     const int32_t *table = kv.block_table + (size_t)it.s * kv.table_width;
     const uint32_t page_mask = (1u << kv.page_shift) - 1;
@@ -451,44 +461,78 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(Attenti
 
 // ---- many query rows -------------------------------------------------------------------------------------------------
 //
-// 128 query rows a workgroup, 32 a wavefront, as the columns of v_mfma_f32_32x32x16_f16; the steps' codes are converted to f16 once and
-// lie in LDS, two steps' worth, rows padded by 16 bytes (an odd number of 16-byte pieces: consecutive rows in other banks).  Row p of S^T is
-// the key whose index is p with bits 2 and 3 exchanged: a lane then holds weights of 8 consecutive keys for each k step of the second
-// product, within one group of 16 keys, so a block's scales are the same for all of them.
+// 128 query rows a workgroup as the columns of matrix instructions; a turn's codes (64 keys) are converted to f16 once and lie in LDS, two
+// turns' worth, rows padded by 16 bytes (an odd number of 16-byte pieces: consecutive rows in other banks).
+//   Wide: four wavefronts of 32 rows, v_mfma_f32_32x32x16_f16.  An operand read from LDS feeds 32 columns; above 128 channels the
+//     registers leave one wavefront a SIMD.
+//   Narrow: eight wavefronts of 16 rows, v_mfma_f32_16x16x32_f16, two a SIMD at every head_dim, for twice the reads from LDS: where f16
+//     pairs double the multiplications anyway, above 128 channels.
+// The order of the keys in S^T's rows is free: they are laid out so that a lane holds the weights of 8 consecutive keys for each k step
+// of the second product, within one group of 16 keys, so a block's scales are the same for all of them.
+template <bool NARROW> struct Shape;
+template <> struct Shape<false> {
+    static constexpr uint32_t kRows = 32, kWaves = 4, kStepDims = 16, kStepKeys = 16, kTileKeys = 32;  // a k step's channels, keys; keys of a score tile
+    typedef f32x16_t Acc;
+    static __device__ __forceinline__ Acc mma(f16x8_t a, f16x8_t b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    // the LDS row of a key: bits 2 and 3 exchanged
+    static __device__ __forceinline__ uint32_t row_of_key(uint32_t key) { return (key & ~12u) | (key & 4u) << 1 | (key & 8u) >> 1; }
+    // score j of a lane's k step c, in its score tiles
+    static constexpr int tile(int c, int) { return c / 2; }
+    static constexpr int reg(int c, int j) { return c % 2 * 8 + j; }
+    static __device__ __forceinline__ uint32_t group(uint32_t c, uint32_t) { return c; }  // of 16 keys
+};
+template <> struct Shape<true> {
+    static constexpr uint32_t kRows = 16, kWaves = 8, kStepDims = 32, kStepKeys = 32, kTileKeys = 16;
+    typedef f32x4_t Acc;
+    static __device__ __forceinline__ Acc mma(f16x8_t a, f16x8_t b, Acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    // keys 8 g + 4 t + r of 32 to rows 16 t + 4 g + r
+    static __device__ __forceinline__ uint32_t row_of_key(uint32_t key) { return (key & ~28u) | (key & 4u) << 2 | (key & 24u) >> 1; }
+    static constexpr int tile(int c, int j) { return 2 * c + j / 4; }
+    static constexpr int reg(int, int j) { return j % 4; }
+    static __device__ __forceinline__ uint32_t group(uint32_t c, uint32_t part) { return 2 * c + part / 2; }
+};
+constexpr bool tiles_narrow(int nk, bool pairs) { return pairs || nk > 4; }
+
 template <int NK, bool PAIRS, bool CAP>
-__global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_kernel(AttentionArgs A, Plan P, Partials part) {
-    constexpr uint32_t D = NK * 32, kKeyPad = D + 8, kValPad = kStep + 8;
-    constexpr int kPieces = (int)(kStep * D / 16 / kAttnThreads) + (kStep * D / 16 % kAttnThreads ? 1 : 0);  // 16-byte pieces of a thread
-    __shared__ __align__(16) _Float16 sh_k[2][kStep][kKeyPad];
+__global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, NK > 4 && !tiles_narrow(NK, PAIRS) ? 1 : 2)
+    attention_tiles_kernel(AttentionArgs A, Plan P, Partials part) {
+    typedef Shape<tiles_narrow(NK, PAIRS)> Sh;
+    constexpr uint32_t D = NK * 32, kKeys = kStep, kThreads = Sh::kWaves * 64, kKeyPad = D + 8, kValPad = kKeys + 8;
+    constexpr int KD = D / Sh::kStepDims, KC = kKeys / Sh::kStepKeys;        // k steps of the two products
+    constexpr int ST = kKeys / Sh::kTileKeys, DT = D / Sh::kRows, G = kKeys / 16;  // score tiles, channel tiles, groups of 16 keys
+    constexpr int kPieces = (int)((kKeys * D / 16 + kThreads - 1) / kThreads);  // 16-byte pieces of a thread
+    constexpr bool kUneven = kKeys * D / 16 % kThreads != 0;
+    static_assert(Sh::kRows * Sh::kWaves == kTilesTile, "a workgroup's rows");
+    __shared__ __align__(16) _Float16 sh_k[2][kKeys][kKeyPad];
     __shared__ __align__(16) _Float16 sh_v[2][D][kValPad];
-    __shared__ float sh_s[2][4][4];  // of each group of 16 keys: key scale, log2 of the value scale, and one over it
+    __shared__ float sh_s[2][G][4];  // of each group of 16 keys: key scale, log2 of the value scale, and one over it
     const KvArgs &kv = A.kv;
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = lane % 32, hi = lane / 32;
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = lane % Sh::kRows, hi = lane / Sh::kRows;  // column; part of a k step
     const uint32_t kvh = blockIdx.x % kv.kv_heads, group = A.q_heads / kv.kv_heads;  // (neighbours: the heads, one for each XCD's cache)
     Item it;
-    if (!find_item(A, P, blockIdx.x / kv.kv_heads, false, it)) return;
-    const Share sh = share_of(A, P, it.s, group);
+    Share sh;
+    if (!find_item(A, P, blockIdx.x / kv.kv_heads, false, it, sh)) return;
     const uint32_t rows = sh.n * group;
     const uint32_t tile = sh.tiles - 1 - it.tile;  // (the last rows see the most keys: first)
 
-    const uint32_t row = tile * kTilesTile + wave * 32 + n, tok = row / group, head = kvh * group + row % group;
+    const uint32_t row = tile * kTilesTile + wave * Sh::kRows + n, tok = row / group, head = kvh * group + row % group;
     const bool live = row < rows;
     const int32_t pos = sh.first + (int32_t)tok;
     const int32_t key_hi = !live ? -1 : (A.causal ? min(pos, sh.len - 1) : sh.len - 1);
     const int32_t key_lo = A.window ? (int32_t)max((int64_t)pos - (int64_t)A.window + 1, (int64_t)0) : 0;
-    f16x8_t qh[2 * NK], ql[PAIRS ? 2 * NK : 1];
+    f16x8_t qh[KD], ql[PAIRS ? KD : 1];
     float factor;
     {
-        Eight q[2 * NK];
+        Eight q[KD];
 #pragma unroll
-        for (int k = 0; k < 2 * NK; k++) {
+        for (int k = 0; k < KD; k++) {
             q[k] = {};
-            if (live) q[k] = load8(A.q, A.q_type, (size_t)(sh.row + tok) * A.q_stride + (size_t)head * D + (uint32_t)k * 16 + hi * 8);
+            if (live) q[k] = load8(A.q, A.q_type, (size_t)(sh.row + tok) * A.q_stride + (size_t)head * D + (uint32_t)k * Sh::kStepDims + hi * 8);
         }
-        factor = query_f16<2 * NK, PAIRS, CAP, false>(A, q, qh, ql);
+        factor = query_f16<KD, PAIRS, CAP, tiles_narrow(NK, PAIRS)>(A, q, qh, ql);
     }
     // what all and any of the wavefront's rows see (whole rows of lanes: the first and the last live one say it)
-    const uint32_t first_row = tile * kTilesTile + wave * 32, last_row = min(first_row + 31, rows - 1);
+    const uint32_t first_row = tile * kTilesTile + wave * Sh::kRows, last_row = min(first_row + Sh::kRows - 1, rows - 1);
     const bool any_live = first_row < rows;
     const auto hi_of = [&](uint32_t r) { return A.causal ? min(sh.first + (int32_t)(r / group), sh.len - 1) : sh.len - 1; };
     const auto lo_of = [&](uint32_t r) {
@@ -498,9 +542,9 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
     const int32_t any_lo = lo_of(first_row), all_lo = lo_of(any_live ? last_row : first_row);
     // the workgroup's steps: those of its piece that any of its rows sees
     const int32_t tile_hi = hi_of(min(tile * kTilesTile + kTilesTile - 1, rows - 1)), tile_lo = lo_of(tile * kTilesTile);
-    const uint64_t piece_lo = (uint64_t)sh.step_lo + (uint64_t)it.piece * it.chunk;
-    const uint32_t end = tile_hi < 0 ? 0u : (uint32_t)min(min(piece_lo + it.chunk, (uint64_t)(sh.step_lo + sh.steps)), (uint64_t)((uint32_t)tile_hi / kStep + 1));
-    uint32_t step = (uint32_t)max(piece_lo, (uint64_t)((uint32_t)tile_lo / kStep));
+    const uint32_t tile_end = tile_hi < tile_lo ? 0u : (uint32_t)tile_hi / kKeys + 1, tile_begin = min((uint32_t)tile_lo / kKeys, tile_end);
+    const uint32_t end = it.end_of(tile_begin, tile_end);
+    uint32_t step = it.begin_of(tile_begin, tile_end);
 
     const int32_t *table = kv.block_table + (size_t)it.s * kv.table_width;
     const uint32_t page_mask = (1u << kv.page_shift) - 1;
@@ -510,7 +554,7 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
     float ks = 0.f, vs = 0.f;
     // The pages of a step, that of group lane % 4 in a lane: read one step before its codes.
     const auto pages_of = [&](uint32_t st) -> uint32_t {
-        const uint32_t key = st * kStep + lane % 4 * 16;
+        const uint32_t key = st * kKeys + lane % G * 16;
         return st >= end || (int32_t)key >= sh.len ? ~0u : kv_page(kv, table, key);
     };
     // A thread's pieces: where they lie in a page (a page of 128 holds two steps), their groups' lanes.
@@ -518,31 +562,31 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
     const uint8_t *k_head = kv.k_codes + kvh * head_codes, *v_head = kv.v_codes + kvh * head_codes;
     uint32_t odd_pages = 0;  // lanes whose page (of the step in kc, vc) is a hole
     const auto load_step = [&](uint32_t st, uint32_t pages) {
-        const uint32_t in_page = (st * kStep) & page_mask;
-        odd_pages = (uint32_t)__ballot(pages == ~0u) & 15u;
+        const uint32_t in_page = (st * kKeys) & page_mask;
+        odd_pages = (uint32_t)__ballot(pages == ~0u) & ((1u << G) - 1);
         const uint32_t safe = pages == ~0u ? 0u : pages;
-        const uint8_t *vp = v_head + (uint64_t)(uint32_t)__shfl((int)safe, (int)(threadIdx.x % 4), 64) * page_bytes +
-                            (((threadIdx.x / 4) << kv.page_shift) + in_page + ((threadIdx.x % 4 * 16) & page_mask));
+        const uint8_t *vp = v_head + (uint64_t)(uint32_t)__shfl((int)safe, (int)(threadIdx.x % G), 64) * page_bytes +
+                            (((threadIdx.x / G) << kv.page_shift) + in_page + ((threadIdx.x % G * 16) & page_mask));
 #pragma unroll
         for (int i = 0; i < kPieces; i++) {
-            const uint32_t p = threadIdx.x + (uint32_t)i * kAttnThreads, key = p / (D / 16);
-            const uint32_t page = (uint32_t)__shfl((int)safe, (int)(key / 16 % 4), 64);
-            if (kStep * D / 16 % kAttnThreads != 0 && p >= kStep * D / 16) break;
+            const uint32_t p = threadIdx.x + (uint32_t)i * kThreads, key = p / (D / 16);
+            const uint32_t page = (uint32_t)__shfl((int)safe, (int)(key / 16 % G), 64);
+            if (kUneven && p >= kKeys * D / 16) break;
             kc[i] = *(const u32x4_t *)(k_head + (uint64_t)page * page_bytes + ((in_page + (key & page_mask)) * D + p % (D / 16) * 16));
-            vc[i] = *(const u32x4_t *)(vp + ((size_t)(i * kAttnThreads / 4) << kv.page_shift));
+            vc[i] = *(const u32x4_t *)(vp + ((size_t)(i * (kThreads / G)) << kv.page_shift));
         }
-        if (threadIdx.x < 4) {
+        if (threadIdx.x < G) {
             ks = pages == ~0u ? 0.f : kv.k_scales[(size_t)pages * kv.kv_heads + kvh];
             vs = pages == ~0u ? 0.f : kv.v_scales[(size_t)pages * kv.kv_heads + kvh];
         }
     };
     const auto store_step = [&](uint32_t st, uint32_t buf) {
-        if ((int32_t)(st * kStep + kStep) > sh.len || odd_pages) {  // codes behind the last key and in holes may be anything: they count as zeros
+        if ((int32_t)(st * kKeys + kKeys) > sh.len || odd_pages) {  // codes behind the last key and in holes may be anything: they count as zeros
 #pragma unroll
             for (int i = 0; i < kPieces; i++) {
-                const uint32_t p = threadIdx.x + (uint32_t)i * kAttnThreads, key = p / (D / 16);
-                if ((int32_t)(st * kStep + key) >= sh.len || (odd_pages >> (key / 16 % 4) & 1u)) kc[i] = u32x4_t{0u, 0u, 0u, 0u};
-                const int32_t have = odd_pages >> (p % 4) & 1u ? 0 : sh.len - (int32_t)(st * kStep + p % 4 * 16);
+                const uint32_t p = threadIdx.x + (uint32_t)i * kThreads, key = p / (D / 16);
+                if ((int32_t)(st * kKeys + key) >= sh.len || (odd_pages >> (key / 16 % G) & 1u)) kc[i] = u32x4_t{0u, 0u, 0u, 0u};
+                const int32_t have = odd_pages >> (p % G) & 1u ? 0 : sh.len - (int32_t)(st * kKeys + p % G * 16);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int32_t b = have - 4 * j;
@@ -552,17 +596,17 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
         }
 #pragma unroll
         for (int i = 0; i < kPieces; i++) {
-            const uint32_t p = threadIdx.x + (uint32_t)i * kAttnThreads;
-            if (kStep * D / 16 % kAttnThreads != 0 && p >= kStep * D / 16) break;
-            const uint32_t key = p / (D / 16), at = (key & ~12u) | (key & 4u) << 1 | (key & 8u) >> 1;
-            f16x8_t *kd = (f16x8_t *)&sh_k[buf][at][p % (D / 16) * 16];
+            const uint32_t p = threadIdx.x + (uint32_t)i * kThreads;
+            if (kUneven && p >= kKeys * D / 16) break;
+            const uint32_t key = p / (D / 16);
+            f16x8_t *kd = (f16x8_t *)&sh_k[buf][Sh::row_of_key(key)][p % (D / 16) * 16];
             kd[0] = codes_f16(u32x2_t{kc[i][0], kc[i][1]});
             kd[1] = codes_f16(u32x2_t{kc[i][2], kc[i][3]});
-            f16x8_t *vd = (f16x8_t *)&sh_v[buf][p / 4][p % 4 * 16];
+            f16x8_t *vd = (f16x8_t *)&sh_v[buf][p / G][p % G * 16];
             vd[0] = codes_f16(u32x2_t{vc[i][0], vc[i][1]});
             vd[1] = codes_f16(u32x2_t{vc[i][2], vc[i][3]});
         }
-        if (threadIdx.x < 4) {
+        if (threadIdx.x < G) {
             // A hole's weights are 2^-inf of codes that are zeros.  A scale that is not a number makes its keys' scores NaN.
             const bool hole = vs == 0.f, odd = !(vs == vs);
             const int ev = odd || hole ? 0 : (int)(__builtin_bit_cast(uint32_t, vs) >> 23 & 0xFFu) - 127;
@@ -572,11 +616,9 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
         }
     };
 
-    f32x16_t acc[NK];
+    typename Sh::Acc acc[DT];
 #pragma unroll
-    for (int i = 0; i < NK; i++)
-#pragma unroll
-        for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
+    for (int i = 0; i < DT; i++) acc[i] = 0.f;
     float M = kNoMax, L = 0.f;
     uint32_t buf = 0;
     uint32_t pages = ~0u;
@@ -594,98 +636,101 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 1 : 2) attention_tiles_
             load_step(step + 2, pages);
             pages = pages_of(step + 3);
         }
-        const int32_t key0 = (int32_t)(step * kStep);
-        if (key0 > any_hi || key0 + (int32_t)kStep <= any_lo) continue;  // (no row of this wavefront sees the step)
-        f32x16_t S[2], zero;
+        const int32_t key0 = (int32_t)(step * kKeys);
+        if (key0 > any_hi || key0 + (int32_t)kKeys <= any_lo) continue;  // (no row of this wavefront sees the step)
+        typename Sh::Acc S[ST], zero = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; j++) zero[j] = 0.f;
+        for (int k = 0; k < KD; k++) {
 #pragma unroll
-        for (int k = 0; k < 2 * NK; k++) {
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const f16x8_t ka = *(const f16x8_t *)&sh_k[buf][t * 32 + n][k * 16 + hi * 8];
-                S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qh[k], k ? S[t] : zero, 0, 0, 0);
-                if constexpr (PAIRS) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, ql[k], S[t], 0, 0, 0);
+            for (int t = 0; t < ST; t++) {
+                const f16x8_t ka = *(const f16x8_t *)&sh_k[buf][t * Sh::kTileKeys + n][k * Sh::kStepDims + hi * 8];
+                S[t] = Sh::mma(ka, qh[k], k ? S[t] : zero);
+                if constexpr (PAIRS) S[t] = Sh::mma(ka, ql[k], S[t]);
             }
         }
-        // x[c]: the 8 scores of group c of 16 keys, keys 16 c + 8 hi + j; their logarithm (base 2) with the value scale: x a + e
-        float a[4], e[4], unscale[4];
+        // x(c, j): the lane's 8 scores of k step c, keys kStepKeys c + 8 hi + j; their logarithm (base 2) with the value scale: x a + e
+        float a[KC], e[KC], unscale[KC];
 #pragma unroll
-        for (int c = 0; c < 4; c++) a[c] = factor * sh_s[buf][c][0], e[c] = sh_s[buf][c][1], unscale[c] = sh_s[buf][c][2];
-        const bool whole = key0 >= all_lo && key0 + (int32_t)kStep - 1 <= all_hi;
+        for (int c = 0; c < KC; c++) {
+            const uint32_t grp = Sh::group(c, hi);
+            a[c] = factor * sh_s[buf][grp][0], e[c] = sh_s[buf][grp][1], unscale[c] = sh_s[buf][grp][2];
+        }
+#define LARQL_X(c, j) S[Sh::tile(c, j)][Sh::reg(c, j)]
+        const bool whole = key0 >= all_lo && key0 + (int32_t)kKeys - 1 <= all_hi;
         if (CAP || !whole) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
+            for (int c = 0; c < KC; c++) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const float x = score<CAP>(A, S[c / 2][c % 2 * 8 + j], a[c], e[c]);
-                    const int32_t key = key0 + c * 16 + (int32_t)hi * 8 + j;
-                    S[c / 2][c % 2 * 8 + j] = !whole && (key > key_hi || key < key_lo) ? -__builtin_inff() : x;
+                    const float x = score<CAP>(A, LARQL_X(c, j), a[c], e[c]);
+                    const int32_t key = key0 + c * (int32_t)Sh::kStepKeys + (int32_t)hi * 8 + j;
+                    LARQL_X(c, j) = !whole && (key > key_hi || key < key_lo) ? -__builtin_inff() : x;
                 }
                 a[c] = 1.f, e[c] = 0.f;
             }
         }
         float top = kNoMax;
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            float m = S[c / 2][c % 2 * 8];
+        for (int c = 0; c < KC; c++) {
+            float m = LARQL_X(c, 0);
 #pragma unroll
-            for (int j = 1; j < 8; j++) m = fmaxf(m, S[c / 2][c % 2 * 8 + j]);
+            for (int j = 1; j < 8; j++) m = fmaxf(m, LARQL_X(c, j));
             top = fmaxf(top, fmaf(m, a[c], e[c]));
         }
         if (__ballot(top > M + kSlack)) {
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
+#pragma unroll
+            for (uint32_t d = Sh::kRows; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, (int)d, 64));
             const float next = top > M + kSlack ? top : M;
             const float f = __builtin_amdgcn_exp2f(M - next);
             M = next;
             L *= f;
 #pragma unroll
-            for (int i = 0; i < NK; i++) acc[i] *= f;
+            for (int i = 0; i < DT; i++) acc[i] *= f;
         }
-        f16x8_t ph[4], pl[4];
+        f16x8_t ph[KC], pl[KC];
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
+        for (int c = 0; c < KC; c++) {
             const float shift = e[c] - M + kBias;
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
-                const f32x2_t p = {__builtin_amdgcn_exp2f(fmaf(S[c / 2][c % 2 * 8 + j], a[c], shift)),
-                                   __builtin_amdgcn_exp2f(fmaf(S[c / 2][c % 2 * 8 + j + 1], a[c], shift))};
+                const f32x2_t p = {__builtin_amdgcn_exp2f(fmaf(LARQL_X(c, j), a[c], shift)), __builtin_amdgcn_exp2f(fmaf(LARQL_X(c, j + 1), a[c], shift))};
                 weights_f16<PAIRS>(p, ph[c], pl[c], j);
                 sum += p[0] + p[1];  // (the f32 weights: one of a block of small values may be nothing in f16, and counts here)
             }
             L = fmaf(sum, unscale[c], L);
         }
+#undef LARQL_X
 #pragma unroll
-        for (int c = 0; c < 4; c++)
+        for (int c = 0; c < KC; c++)
 #pragma unroll
-            for (int d = 0; d < NK; d++) {
-                const f16x8_t va = *(const f16x8_t *)&sh_v[buf][d * 32 + n][c * 16 + hi * 8];
-                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[c], acc[d], 0, 0, 0);
-                if constexpr (PAIRS) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[c], acc[d], 0, 0, 0);
+            for (int d = 0; d < DT; d++) {
+                const f16x8_t va = *(const f16x8_t *)&sh_v[buf][d * Sh::kRows + n][c * Sh::kStepKeys + hi * 8];
+                acc[d] = Sh::mma(va, ph[c], acc[d]);
+                if constexpr (PAIRS) acc[d] = Sh::mma(va, pl[c], acc[d]);
             }
     }
-    L += __shfl_xor(L, 32, 64);
+#pragma unroll
+    for (uint32_t d = Sh::kRows; d < 64; d *= 2) L += __shfl_xor(L, (int)d, 64);
     if (!live) return;
-    // acc[d][4 i + j]: channel 32 d + 8 i + 4 hi + j
+    // acc[d][4 i + j]: channel kRows d + 8 i + 4 hi + j
+    constexpr int QUADS = sizeof(typename Sh::Acc) / 16;
+    const auto quad = [&](int d, int i) { return f32x4_t{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]}; };
     if (it.pieces > 1) {
-        const size_t at = ((size_t)kvh * part.slots + it.slot + it.piece) * kTilesTile + wave * 32 + n;
+        const size_t at = ((size_t)kvh * part.slots + it.slot + it.piece) * kTilesTile + wave * Sh::kRows + n;
         if (hi == 0) part.ml[2 * at] = M, part.ml[2 * at + 1] = L;
 #pragma unroll
-        for (int d = 0; d < NK; d++)
+        for (int d = 0; d < DT; d++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                *(f32x4_t *)(part.acc + at * D + d * 32 + i * 8 + hi * 4) = f32x4_t{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+            for (int i = 0; i < QUADS; i++) *(f32x4_t *)(part.acc + at * D + d * Sh::kRows + i * 8 + hi * 4) = quad(d, i);
         return;
     }
     const float inv = inverse_sum(A, L, M, head);
 #pragma unroll
-    for (int d = 0; d < NK; d++)
+    for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const f32x4_t v = {acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv, acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv};
-            store4(A.out, A.out_type, (size_t)(sh.row + tok) * A.out_stride + (size_t)head * D + d * 32 + i * 8 + hi * 4, v);
-        }
+        for (int i = 0; i < QUADS; i++)
+            store4(A.out, A.out_type, (size_t)(sh.row + tok) * A.out_stride + (size_t)head * D + d * Sh::kRows + i * 8 + hi * 4, quad(d, i) * inv);
 }
 
 // One query row of a split tile: pieces p0, p0 + step, ... as one sum.  `at`: the row in the first piece.
@@ -721,15 +766,26 @@ __device__ __forceinline__ void join_pieces(const Partials &part, uint32_t tile,
     }
 }
 
-// The pieces of split rows as one: a workgroup for kJoinRows rows of a split tile, `share` of its wavefronts (1, 2, 4 or 8) for a row.
+// The pieces of split rows as one, of both kernels: a workgroup for kJoinRows rows of a split tile, `share` of its wavefronts (1, 2, 4 or 8)
+// for a row.
 constexpr uint32_t kJoinRows = 16, kJoinWaves = 8;
-__global__ void __launch_bounds__(kJoinWaves * 64) attention_join_kernel(AttentionArgs A, Plan P, Partials part, uint32_t share) {
+struct Join {
+    Plan plan[2];
+    Partials part[2];
+    uint32_t split_tiles[2];  // at most
+    uint32_t share;
+};
+__global__ void __launch_bounds__(kJoinWaves * 64) attention_join_kernel(AttentionArgs A, Join J) {
     __shared__ float sh_acc[kJoinWaves][256], sh_ml[kJoinWaves][2];
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, D = A.kv.head_dim, dim = min(lane * 4, D - 4);
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, D = A.kv.head_dim, dim = min(lane * 4, D - 4), share = J.share;
     const uint32_t kvh = blockIdx.y, group = A.q_heads / A.kv.kv_heads;
+    const bool second = blockIdx.x >= J.split_tiles[0];
+    const Plan P = second ? J.plan[1] : J.plan[0];
+    const Partials part = second ? J.part[1] : J.part[0];
+    if (blockIdx.z * kJoinRows >= P.tile) return;
     Item it;
-    if (!find_item(A, P, blockIdx.x, true, it)) return;
-    const Share sh = share_of(A, P, it.s, group);
+    Share sh;
+    if (!find_item(A, P, blockIdx.x - (second ? J.split_tiles[0] : 0u), true, it, sh)) return;
     const uint32_t row0 = (P.tile == kTilesTile ? sh.tiles - 1 - it.tile : it.tile) * P.tile;
     const size_t at = ((size_t)kvh * part.slots + it.slot) * P.tile;
     const uint32_t end = min((blockIdx.z + 1) * kJoinRows, min(P.tile, sh.n * group - row0));
@@ -775,7 +831,8 @@ size_t attention_workspace_bytes(const AttentionArgs &A) {
 }
 int attention_launches(const AttentionArgs &A) {
     const Plans p = plans_of(A);
-    return (p.use_rows ? 1 + (int)p.rows.split : 0) + (p.use_tiles ? 1 + (int)p.tiles.split : 0);
+    const bool join = (p.use_rows && p.rows.split) || (p.use_tiles && p.tiles.split);
+    return (int)p.use_rows + (int)p.use_tiles + (int)join;
 }
 
 template <int NK>
@@ -784,7 +841,7 @@ static void launch_dim(hipStream_t s, const AttentionArgs &A, const Plan &P, con
     const uint32_t items = (uint32_t)Plans::items(A, P);
 #define LARQL_ATTN(PR, C)                                                                                                             \
     do {                                                                                                                              \
-        if (tiles) hipLaunchKernelGGL((attention_tiles_kernel<NK, PR, C>), dim3(items * A.kv.kv_heads), dim3(kAttnThreads), 0, s, A, P, part); \
+        if (tiles) hipLaunchKernelGGL((attention_tiles_kernel<NK, PR, C>), dim3(items * A.kv.kv_heads), dim3(Shape<tiles_narrow(NK, PR)>::kWaves * 64), 0, s, A, P, part); \
         else hipLaunchKernelGGL((attention_rows_kernel<NK, PR, C>), dim3(items, A.kv.kv_heads), dim3(kAttnThreads), 0, s, A, P, part);  \
     } while (0)
     if (pairs && cap) LARQL_ATTN(true, true);
@@ -807,12 +864,6 @@ static hipError_t launch_plan(hipStream_t s, const AttentionArgs &A, const Plan 
     case 8: launch_dim<8>(s, A, P, part, tiles); break;
     default: return hipErrorInvalidValue;
     }
-    if (P.split) {
-        const uint32_t rows = (uint32_t)std::min<uint64_t>((uint64_t)A.kv.max_new * (A.q_heads / A.kv.kv_heads), P.tile);
-        const uint32_t share = rows <= 1 ? 8 : rows <= 2 ? 4 : rows <= 4 ? 2 : 1;
-        hipLaunchKernelGGL(attention_join_kernel, dim3((uint32_t)Plans::split_tiles(A, P), A.kv.kv_heads, (rows + kJoinRows - 1) / kJoinRows),
-                           dim3(kJoinWaves * 64), 0, s, A, P, part, share);
-    }
     return hipGetLastError();
 }
 
@@ -820,15 +871,24 @@ hipError_t attention_launch(hipStream_t s, const AttentionArgs &A, void *workspa
     const Plans p = plans_of(A);
     float *at = (float *)workspace;
     hipError_t e = hipSuccess;
-    if (p.use_tiles) {
-        const Partials part = partials_of(A, p.tiles, at, &at);
-        e = launch_plan(s, A, p.tiles, part, true);
-    }
-    if (p.use_rows && e == hipSuccess) {
-        const Partials part = partials_of(A, p.rows, at, &at);
-        e = launch_plan(s, A, p.rows, part, false);
-    }
-    return e;
+    Join J = {};
+    uint32_t rows = 0;  // of a split tile, at most
+    const auto run = [&](const Plan &P, bool tiles) {
+        const Partials part = partials_of(A, P, at, &at);
+        if (e == hipSuccess) e = launch_plan(s, A, P, part, tiles);
+        const int i = tiles ? 0 : 1;
+        J.plan[i] = P;
+        J.part[i] = part;
+        J.split_tiles[i] = (uint32_t)Plans::split_tiles(A, P);
+        if (P.split) rows = std::max(rows, (uint32_t)std::min<uint64_t>((uint64_t)A.kv.max_new * (A.q_heads / A.kv.kv_heads), P.tile));
+    };
+    if (p.use_tiles) run(p.tiles, true);
+    if (p.use_rows) run(p.rows, false);
+    const uint32_t split = J.split_tiles[0] + J.split_tiles[1];
+    if (e != hipSuccess || split == 0) return e;
+    J.share = rows <= 1 ? 8 : rows <= 2 ? 4 : rows <= 4 ? 2 : 1;
+    hipLaunchKernelGGL(attention_join_kernel, dim3(split, A.kv.kv_heads, (rows + kJoinRows - 1) / kJoinRows), dim3(kJoinWaves * 64), 0, s, A, J);
+    return hipGetLastError();
 }
 
 }  // namespace larql

@@ -847,11 +847,11 @@ _APP = [("app", "format", hip.FMT_Q4_K, L.UNSUPPORTED), ("app", "rot_dim", 72, L
         ("app", "inv_freq", None, L.E_ARG), ("app", "inv_freq", 66, L.REFUSED_SHAPE), ("app", "k", None, L.E_ARG), ("app", "v", None, L.E_ARG), ("app", "q_out", None, L.E_ARG),
         ("app", "k_stride", 127, L.REFUSED_SHAPE), ("app", "k_stride", 64, L.REFUSED_SHAPE), ("app", "v", 4104, L.REFUSED_SHAPE),
         ("app", "q_stride", 200, L.REFUSED_SHAPE), ("app", "q_out", 8200, L.REFUSED_SHAPE), ("app", "k_norm", 72, L.REFUSED_SHAPE),
-        ("app", "q_heads", 5, L.REFUSED_SHAPE)]
+        ("app", "q_heads", 5, L.REFUSED_SHAPE), ("app", "v_stride", 1 << 23, L.UNSUPPORTED), ("app", "q_out_stride", 1 << 23, L.UNSUPPORTED)]
 _ATT = [("att", "q_format", hip.FMT_Q8_0, L.UNSUPPORTED), ("att", "out_format", -1, L.UNSUPPORTED), ("att", "q_heads", 0, L.REFUSED_SHAPE),
         ("att", "q_heads", 3, L.REFUSED_SHAPE), ("att", "q", None, L.E_ARG), ("att", "out", None, L.E_ARG), ("att", "out_stride", 252, L.REFUSED_SHAPE),
         ("att", "q_stride", 258, L.REFUSED_SHAPE), ("att", "out", 8200, L.REFUSED_SHAPE), ("att", "softcap", -1.0, L.REFUSED_SHAPE),
-        ("att", "softcap", math.nan, L.REFUSED_SHAPE), ("att", "scale", math.inf, L.REFUSED_SHAPE), ("att", "window", 1 << 31, L.UNSUPPORTED),
+        ("att", "softcap", math.nan, L.REFUSED_SHAPE), ("att", "softcap", 1e-7, L.REFUSED_SHAPE), ("att", "scale", math.inf, L.REFUSED_SHAPE), ("att", "window", 1 << 31, L.UNSUPPORTED),
         ("att", "sinks", 66, L.REFUSED_SHAPE)]
 _NORM = [("norm", "hidden", 32769, L.UNSUPPORTED), ("norm", "block_format", hip.FMT_MXFP4, L.UNSUPPORTED), ("norm", "residual", None, L.E_ARG),
          ("norm", "residual_stride", 63, L.REFUSED_SHAPE), ("norm", "normed_stride", 1, L.REFUSED_SHAPE), ("norm", "residual", 4098, L.REFUSED_SHAPE),
