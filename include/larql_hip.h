@@ -574,7 +574,8 @@ typedef struct {
  * tokens of sequence s with the new ones; its new tokens are rows q_start[s] .. q_start[s+1] of the activations and the last
  * ones of the sequence.  block_table[s] lists its pages; an entry outside [0, num_pages) is a hole: nothing is written
  * there, and its tokens are masked.  A sequence whose rows do not fit (q_start falling, beyond `tokens`, or more than
- * max_new_tokens of them) is left out, its rows untouched. */
+ * max_new_tokens of them) is left out, its rows untouched.  Up to 2^20 sequences, 2^24 new tokens and tables of 2^30 tokens
+ * (more: LARQL_UNSUPPORTED). */
 typedef struct {
     const int32_t *kv_len;         /* [sequences] */
     const int32_t *block_table;    /* [sequences, table_width] */
@@ -616,8 +617,9 @@ int larql_hip_dev_kv_append(larql_hip_ctx *ctx, const larql_hip_kv_cache *cache,
  * > p - window (window > 0); `sinks` [q_heads] (or NULL) adds exp(sink) to the sum of the weights.  A query that sees
  * nothing gives zeros.  Sums are f32; where `out` is f32 queries and weights enter the matrix instructions as f16 pairs
  * (about 22 bits), otherwise as one f16 each.  Results may differ in their last bits with the batch around a sequence: long
- * rows are split by the work that there is.  workspace: larql_hip_attention_workspace_bytes(...) of device memory, 16-byte
- * aligned, not shared with a call that may run at the same time. */
+ * rows are split by the work that there is.  workspace: larql_hip_attention_workspace_bytes(...) (0: a call that is refused or
+ * has nothing to do) of device memory, 16-byte aligned, not shared with a call that may run at the same time; it depends on
+ * the batch's sizes, not on what the device memory holds. */
 typedef struct {
     const void *q;
     size_t q_stride;

@@ -2610,7 +2610,7 @@ static int check_kv(larql_hip_ctx *c, const char *what, const larql_hip_kv_cache
     *empty = b->sequences == 0 || b->tokens == 0 || b->max_new_tokens == 0;
     if (*empty) return LARQL_OK;
     if (k->num_pages == 0 || b->table_width == 0) return fail(c, LARQL_REFUSED_SHAPE, "%s: a cache without pages", what);
-    if (k->num_pages > 0x7FFFFFFFull || b->sequences > (1u << 20) || b->table_width > 0x7FFFFFFFull || b->tokens > (1u << 24))
+    if (k->num_pages > 0x7FFFFFFFull || b->sequences > (1u << 20) || b->table_width > (1u << 30) / k->page_tokens || b->tokens > (1u << 24))
         return fail(c, LARQL_UNSUPPORTED, "%s: too large", what);
     if (!k->k_codes || !k->v_codes || !k->k_scales || !k->v_scales || !b->kv_len || !b->block_table || !b->q_start) return LARQL_E_ARG;
     if (((uintptr_t)k->k_codes | (uintptr_t)k->v_codes) & 15) return fail(c, LARQL_REFUSED_SHAPE, "%s: codes must be 16-byte aligned", what);

@@ -27,9 +27,10 @@ constexpr uint32_t kRowsTile = 16;      // query rows of a workgroup of the kern
 constexpr uint32_t kTilesTile = 128;    // ... for many, 32 a wavefront
 constexpr uint32_t kFewRows = 32;       // a sequence with at most this many rows for each key/value head goes through the former
 constexpr float kLog2E = 1.44269504088896341f;
-// Weights are held as 2^(t + e - M + 12) with t + e - M <= 3, so that the f16 pair of an f32 weight keeps 22 bits down to 2^-15 of the
-// largest and 2^-37 of it beyond; M only moves where a score leaves that range.
-constexpr float kBias = 12.f, kSlack = 3.f;
+// Weights are held as 2^(t + e - M + 7) with t + e - M <= 3; M is whole and only moves where a score leaves that range, so it brings no
+// rounding, and the one of the exponent is that of a number of at most 10.  The f16 pair of an f32 weight keeps 22 bits down to 2^-10 of the
+// largest and 2^-32 of it beyond (131072 equal weights 2^-17 of one that weighs as much as they all: 2^-15 each, at random).
+constexpr float kBias = 7.f, kSlack = 3.f;
 constexpr float kNoMax = -1e30f;
 
 // How one of the two kernels shares its work out.
@@ -177,18 +178,30 @@ struct Partials {
 
 // A result row's end: the sink, the quotient.
 __device__ __forceinline__ float inverse_sum(const AttentionArgs &A, float l, float top, uint32_t head) {
-    if (A.sinks && l != 0.f) l += __builtin_amdgcn_exp2f(A.sinks[head] * kLog2E - top + kBias);
+    if (A.sinks && l != 0.f) l += __builtin_amdgcn_exp2f(fmaf(A.sinks[head], kLog2E, kBias - top));
     return l == 0.f ? 0.f : 1.f / l;
 }
 
-// The logarithm (base 2) of a score's weight, plus e: s a + e, or with the cap in between.
-template <bool CAP>
-__device__ __forceinline__ float score(const AttentionArgs &A, float s, float a, float e) {
-    if constexpr (!CAP) return fmaf(s, a, e);
-    // cap * tanh(s / cap) = cap - 2 cap / (exp(2 s / cap) + 1), `a` with the factor 2 log2(e) / cap (query_f16)
+// The logarithm (base 2) of a capped score's weight, plus e: cap * tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1), where s a is the
+// exponent of that as a power of two (query_f16).
+__device__ __forceinline__ float capped(const AttentionArgs &A, float s, float a, float e) {
     const float c = A.softcap * kLog2E;
     return fmaf(-2.f * c, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a) + 1.f), c + e);
 }
+
+// Scores s of a step with hidden keys, whose logarithms are s a + e: a hidden one is -inf, times a factor that is positive; a factor that is
+// not (a scale of 0, a block that is no number) goes into the scores that are seen.
+struct Seen {
+    float factor, offset;
+    bool keep;
+    __device__ __forceinline__ Seen(float a, float e) : factor(a), offset(e), keep(a > 0.f) {}
+    __device__ __forceinline__ float operator()(float s, int hidden) const {
+        const float x = keep ? s : fmaf(s, factor, offset);
+        return hidden ? -__builtin_inff() : x;
+    }
+    __device__ __forceinline__ float a() const { return keep ? factor : 1.f; }
+    __device__ __forceinline__ float e() const { return keep ? offset : 0.f; }
+};
 
 // A query row's elements (spread over lanes 32 apart, and 16 apart where QUARTERS) as f16 or f16 pairs after a power-of-two scale that brings
 // the largest to [2^14, 2^15); returns what scores are multiplied by.  A row that is not finite gets NaN there.
@@ -332,7 +345,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(Attenti
         const int32_t key0 = (int32_t)(step * kStep);
         const bool hole = page_v == ~0u;
         const uint8_t *vp = v_head + (uint64_t)(hole ? 0u : page_v) * page_bytes + ((n << kv.page_shift) + (((uint32_t)key0 + g * 16) & page_mask));
-        f32x4_t S[4];
+        f32x4_t S[4], odd[PAIRS ? 4 : 1] = {}, low[PAIRS ? 4 : 1] = {};  // (pairs: three sums, each of a third of the roundings)
 #pragma unroll
         for (int p = 0; p < NP; p++) {
 #pragma unroll
@@ -342,8 +355,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(Attenti
                 for (int t = 0; t < 4; t++) {
                     const u32x4_t c = ring[p][t];
                     const f16x8_t ka = codes_f16(k % 2 ? u32x2_t{c[2], c[3]} : u32x2_t{c[0], c[1]});
-                    S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh, k ? S[t] : f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                    if constexpr (PAIRS) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql, S[t], 0, 0, 0);
+                    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+                    f32x4_t &sum = PAIRS && k % 2 ? odd[t] : S[t];
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh, k < (PAIRS ? 2 : 1) ? zero : sum, 0, 0, 0);
+                    if constexpr (PAIRS) low[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql, k ? low[t] : zero, 0, 0, 0);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -351,31 +366,37 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(Attenti
             for (int d = 4 * p; d < (4 * p + 4 < 2 * NK ? 4 * p + 4 : 2 * NK); d++) ring[p][d % 4] = *(const u32x4_t *)(vp + ((size_t)(16 * d) << kv.page_shift));
             __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (PAIRS)
+#pragma unroll
+            for (int t = 0; t < 4; t++) S[t] += odd[t] + low[t];
         // Logarithms (base 2) of the weights times the value scale.  A scale that is not a number makes its tokens' scores NaN.
-        const bool odd = !(vs == vs);
-        const int ev = odd || hole ? 0 : (int)(__builtin_bit_cast(uint32_t, vs) >> 23 & 0xFFu) - 127;
+        const bool none = !(vs == vs);
+        const int ev = none || hole ? 0 : (int)(__builtin_bit_cast(uint32_t, vs) >> 23 & 0xFFu) - 127;
         const float unscale = __builtin_bit_cast(float, (uint32_t)(127 - ev) << 23);
-        const float a = factor * (odd ? __builtin_nanf("") : ks);
-        float x[16];
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) x[4 * t + r] = score<CAP>(A, S[t][r], a, (float)ev);
+        float a = factor * (none ? __builtin_nanf("") : ks), e = (float)ev;
         const bool plain = key0 >= all_lo && key0 + (int32_t)kStep - 1 <= all_hi && __ballot(hole) == 0;
+        if constexpr (CAP) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) S[i / 4][i % 4] = capped(A, S[i / 4][i % 4], a, e);
+            a = 1.f, e = 0.f;
+        }
         if (!plain) {
+            const Seen see(a, e);
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const int32_t key = key0 + (int32_t)g * 16 + i;
-                if (hole || key > key_hi || key < key_lo) x[i] = -__builtin_inff();
+                S[i / 4][i % 4] = see(S[i / 4][i % 4], (int)hole | (int)(key > key_hi) | (int)(key < key_lo));
             }
+            a = see.a(), e = see.e();
         }
-        float top = x[0];
+        float top = S[0][0];
 #pragma unroll
-        for (int i = 1; i < 16; i++) top = fmaxf(top, x[i]);
+        for (int i = 1; i < 16; i++) top = fmaxf(top, S[i / 4][i % 4]);
+        top = fmaf(top, a, e);
         if (__ballot(top > M + kSlack)) {
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float next = top > M + kSlack ? top : M;
+            const float next = top > M + kSlack ? ceilf(top) : M;
             const float f = __builtin_amdgcn_exp2f(M - next);
             M = next;
             L *= f;
@@ -384,9 +405,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(Attenti
         }
         f16x8_t ph[2], pl[2];
         float sum = 0.f;
+        const float shift = e - M + kBias;
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-            const f32x2_t p = {__builtin_amdgcn_exp2f(x[i] - M + kBias), __builtin_amdgcn_exp2f(x[i + 1] - M + kBias)};
+            const f32x2_t p = {__builtin_amdgcn_exp2f(fmaf(S[i / 4][i % 4], a, shift)), __builtin_amdgcn_exp2f(fmaf(S[i / 4][i % 4 + 1], a, shift))};
             weights_f16<PAIRS>(p, ph[i / 8], pl[i / 8], i % 8);
             sum += p[0] + p[1];  // (the f32 weights: one of a block of small values may be nothing in f16, and counts here)
         }
@@ -657,16 +679,24 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
         }
 #define LARQL_X(c, j) S[Sh::tile(c, j)][Sh::reg(c, j)]
         const bool whole = key0 >= all_lo && key0 + (int32_t)kKeys - 1 <= all_hi;
-        if (CAP || !whole) {
+        if constexpr (CAP) {
 #pragma unroll
             for (int c = 0; c < KC; c++) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float x = score<CAP>(A, LARQL_X(c, j), a[c], e[c]);
-                    const int32_t key = key0 + c * (int32_t)Sh::kStepKeys + (int32_t)hi * 8 + j;
-                    LARQL_X(c, j) = !whole && (key > key_hi || key < key_lo) ? -__builtin_inff() : x;
-                }
+                for (int j = 0; j < 8; j++) LARQL_X(c, j) = capped(A, LARQL_X(c, j), a[c], e[c]);
                 a[c] = 1.f, e[c] = 0.f;
+            }
+        }
+        if (!whole) {
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                const Seen see(a[c], e[c]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int32_t key = key0 + c * (int32_t)Sh::kStepKeys + (int32_t)hi * 8 + j;
+                    LARQL_X(c, j) = see(LARQL_X(c, j), (int)(key > key_hi) | (int)(key < key_lo));
+                }
+                a[c] = see.a(), e[c] = see.e();
             }
         }
         float top = kNoMax;
@@ -680,7 +710,7 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
         if (__ballot(top > M + kSlack)) {
 #pragma unroll
             for (uint32_t d = Sh::kRows; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, (int)d, 64));
-            const float next = top > M + kSlack ? top : M;
+            const float next = top > M + kSlack ? ceilf(top) : M;
             const float f = __builtin_amdgcn_exp2f(M - next);
             M = next;
             L *= f;

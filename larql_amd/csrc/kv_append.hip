@@ -430,6 +430,7 @@ hipError_t kv_append_launch(hipStream_t s, const KvAppendArgs &A) {
     if (kv.max_new == 1) {
         const uint32_t lanes = groups <= 4 ? 4 : groups <= 8 ? 8 : groups <= 16 ? 16 : 32;
         const uint32_t blocks = ((2 * kv.kv_heads + (A.q ? A.q_heads : 0)) * lanes + kAppendThreads - 1) / kAppendThreads;
+        if ((uint64_t)kv.sequences * blocks > 0x7FFFFFFFull) return hipErrorInvalidValue;
         const dim3 one(kv.sequences * blocks), threads(kAppendThreads);
         if (lanes == 4) hipLaunchKernelGGL(kv_append_one_kernel<4>, one, threads, 0, s, A, blocks);
         else if (lanes == 8) hipLaunchKernelGGL(kv_append_one_kernel<8>, one, threads, 0, s, A, blocks);

@@ -840,7 +840,7 @@ _KV = [("cache", "head_dim", 0, L.REFUSED_SHAPE), ("cache", "head_dim", 48, L.RE
        ("cache", "page_tokens", 0, L.REFUSED_SHAPE), ("cache", "page_tokens", 24, L.REFUSED_SHAPE), ("cache", "page_tokens", 256, L.REFUSED_SHAPE),
        ("cache", "kv_heads", 0, L.REFUSED_SHAPE), ("cache", "kv_heads", 5000, L.REFUSED_SHAPE), ("cache", "num_pages", 0, L.REFUSED_SHAPE),
        ("cache", "num_pages", 1 << 31, L.UNSUPPORTED), ("cache", "k_codes", 4104, L.REFUSED_SHAPE), ("cache", "v_codes", None, L.E_ARG),
-       ("cache", "k_scales", 66, L.REFUSED_SHAPE), ("batch", "table_width", 0, L.REFUSED_SHAPE), ("batch", "sequences", 1 << 21, L.UNSUPPORTED),
+       ("cache", "k_scales", 66, L.REFUSED_SHAPE), ("batch", "table_width", 0, L.REFUSED_SHAPE), ("batch", "table_width", (1 << 26) + 1, L.UNSUPPORTED), ("batch", "sequences", 1 << 21, L.UNSUPPORTED),
        ("batch", "tokens", 1 << 25, L.UNSUPPORTED), ("batch", "q_start", None, L.E_ARG), ("batch", "block_table", 66, L.REFUSED_SHAPE),
        ("batch", "kv_len", None, L.E_ARG)]
 _APP = [("app", "format", hip.FMT_Q4_K, L.UNSUPPORTED), ("app", "rot_dim", 72, L.REFUSED_SHAPE), ("app", "rot_dim", 12, L.REFUSED_SHAPE),
