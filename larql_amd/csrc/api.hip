@@ -2678,6 +2678,7 @@ static int check_attention(larql_hip_ctx *c, const larql_hip_kv_cache *k, const 
     if ((uintptr_t)a->sinks & 3) return fail(c, LARQL_REFUSED_SHAPE, "attention: sinks must be 4-byte aligned");
     A.q = a->q; A.out = a->out; A.q_stride = a->q_stride; A.out_stride = a->out_stride; A.sinks = a->sinks;
     A.q_heads = (uint32_t)a->q_heads; A.window = (uint32_t)a->window; A.causal = a->causal != 0;
+    A.group = Divisor::by(A.q_heads / A.kv.kv_heads);
     A.scale = a->scale; A.softcap = a->softcap;
     return LARQL_OK;
 }

@@ -49,17 +49,17 @@ struct Share {
     int32_t len, first;   // keys, position of the first new token
     uint32_t tiles, steps;
 };
-__device__ __forceinline__ Share share_of(const AttentionArgs &A, const Plan &P, uint32_t s, uint32_t group) {
+__device__ __forceinline__ Share share_of(const AttentionArgs &A, const Plan &P, uint32_t s) {
     const NewTokens t = new_tokens(A.kv, s);
     Share h;
     h.row = t.row;
     h.n = t.n;
     h.len = (int32_t)min((uint64_t)t.len, (uint64_t)A.kv.table_width << A.kv.page_shift);
     h.first = t.len - (int32_t)t.n;
-    const uint32_t rows = t.n * group;
+    const uint32_t rows = t.n * A.group.d;
     h.tiles = rows < P.rows_min || rows > P.rows_max ? 0u : (rows + P.tile - 1) / P.tile;
     h.steps = h.tiles ? ((uint32_t)h.len + kStep - 1) / kStep : 0;
-    if (A.window) h.steps = min((uint64_t)h.steps, ((uint64_t)A.window + P.tile / group + 1) / kStep + 2);  // (a tile's tokens may straddle)
+    if (A.window) h.steps = min((uint64_t)h.steps, ((uint64_t)A.window + A.group.of(P.tile) + 1) / kStep + 2);  // (a tile's tokens may straddle)
     return h;
 }
 
@@ -75,8 +75,8 @@ struct Item {
     }
 };
 __device__ __forceinline__ bool find_item(const AttentionArgs &A, const Plan &P, uint32_t item, bool split_tiles, Item &it, Share &sh) {
-    const uint32_t lane = threadIdx.x % 64, group = A.q_heads / A.kv.kv_heads;
-    const auto share_at = [&](uint32_t s) { return s < A.kv.sequences ? share_of(A, P, s, group) : Share{}; };
+    const uint32_t lane = threadIdx.x % 64;
+    const auto share_at = [&](uint32_t s) { return s < A.kv.sequences ? share_of(A, P, s) : Share{}; };
     const auto pieces_of = [](const Share &h, uint32_t chunk) { return max(h.steps / chunk + (h.steps % chunk ? 1u : 0u), 1u); };
     const Share first = share_at(lane);  // (read once where 64 sequences are all)
     const auto sum_of = [&](auto f) {  // over the sequences; a sum that need not be exact
@@ -124,15 +124,15 @@ struct Plans {
     Plan rows, tiles;
     bool use_rows, use_tiles;
     static uint64_t items(const AttentionArgs &A, const Plan &P) {
-        return A.kv.tokens * (uint64_t)(A.q_heads / A.kv.kv_heads) / P.tile + A.kv.sequences + (P.split ? P.target + 1 : 0);
+        return A.kv.tokens * (uint64_t)A.group.d / P.tile + A.kv.sequences + (P.split ? P.target + 1 : 0);
     }
     static uint64_t slots(const Plan &P) { return P.split ? 2 * P.target + 2 : 0; }
     static uint64_t split_tiles(const AttentionArgs &A, const Plan &P) {
-        return P.split ? std::min<uint64_t>(P.target + 1, A.kv.tokens * (uint64_t)(A.q_heads / A.kv.kv_heads) / P.tile + A.kv.sequences) : 0;
+        return P.split ? std::min<uint64_t>(P.target + 1, A.kv.tokens * (uint64_t)A.group.d / P.tile + A.kv.sequences) : 0;
     }
 };
 static Plans plans_of(const AttentionArgs &A) {
-    const uint64_t group = A.q_heads / A.kv.kv_heads, most = A.kv.max_new * group;
+    const uint64_t group = A.group.d, most = A.kv.max_new * group;
     const uint64_t steps = (((uint64_t)A.kv.table_width << A.kv.page_shift) + kStep - 1) / kStep;
     const uint32_t cus = 256;
     Plans p;
@@ -203,10 +203,13 @@ struct Seen {
     __device__ __forceinline__ float e() const { return keep ? offset : 0.f; }
 };
 
-// A query row's elements (spread over lanes 32 apart, and 16 apart where QUARTERS) as f16 or f16 pairs after a power-of-two scale that brings
-// the largest to [2^14, 2^15); returns what scores are multiplied by.  A row that is not finite gets NaN there.
-template <int N, bool PAIRS, bool CAP, bool QUARTERS>
-__device__ __forceinline__ float query_f16(const AttentionArgs &A, const Eight (&q)[N], f16x8_t (&qh)[N], f16x8_t (&ql)[PAIRS ? N : 1]) {
+// A query row's elements (spread over lanes 32 apart, and 16 apart where QUARTERS) enter as f16 or f16 pairs after a power-of-two scale that
+// brings the largest to [2^14, 2^15): what they are multiplied by, and what scores are.  A row that is not finite gets NaN there.
+struct QueryScale {
+    float mul, factor;
+};
+template <int N, bool CAP, bool QUARTERS>
+__device__ __forceinline__ QueryScale query_scale(const AttentionArgs &A, const Eight (&q)[N]) {
     uint32_t amax = 0;
 #pragma unroll
     for (int k = 0; k < N; k++)
@@ -217,18 +220,15 @@ __device__ __forceinline__ float query_f16(const AttentionArgs &A, const Eight (
     const bool finite = amax < 0x7F800000u;
     const int e = min(max((int)(amax >> 23) - 127 - 14, -114), 114);
     const float inv = finite ? __builtin_bit_cast(float, (uint32_t)(127 - e) << 23) : 0.f;
-    // (the scale's sign goes into the query: factors of scores are not negative)
-    const float sign = A.scale < 0.f ? -inv : inv;
-#pragma unroll
-    for (int k = 0; k < N; k++)
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            const f32x2_t x = {finite ? q[k][i] * sign : 0.f, finite ? q[k][i + 1] * sign : 0.f};
-            f16x8_t rest;
-            weights_f16<PAIRS>(x, qh[k], PAIRS ? ql[PAIRS ? k : 0] : rest, i);
-        }
     const float factor = fabsf(A.scale) * (CAP ? 2.f * kLog2E / A.softcap : kLog2E) * __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
-    return finite ? factor : __builtin_nanf("");
+    // (the scale's sign goes into the query: factors of scores are not negative)
+    return {A.scale < 0.f ? -inv : inv, finite ? factor : __builtin_nanf("")};
+}
+template <bool PAIRS>
+__device__ __forceinline__ void query_f16(const Eight &q, float mul, f16x8_t &h, f16x8_t &l) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2)
+        weights_f16<PAIRS>(f32x2_t{mul == 0.f ? 0.f : q[i] * mul, mul == 0.f ? 0.f : q[i + 1] * mul}, h, l, i);
 }
 
 // ---- few query rows --------------------------------------------------------------------------------------------------
@@ -254,18 +254,18 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(Attenti
     Sums &ss = *(Sums *)shared;
     const KvArgs &kv = A.kv;
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = lane % 16, g = lane / 16;
-    const uint32_t kvh = blockIdx.y, group = A.q_heads / kv.kv_heads;
+    const uint32_t kvh = blockIdx.y, group = A.group.d;
     Item it;
     Share sh;
     if (!find_item(A, P, blockIdx.x, false, it, sh)) return;
     const uint32_t rows = sh.n * group;
 
     // The lane's query row: token and head, what it sees.  What all and any of the rows see: the first and the last say it.
-    const uint32_t row0 = it.tile * kRowsTile, row = row0 + n, tok = row / group;
+    const uint32_t row0 = it.tile * kRowsTile, row = row0 + n, tok = A.group.of(row);
     const bool live = row < rows;
-    const auto hi_of = [&](uint32_t r) { return A.causal ? min(sh.first + (int32_t)(r / group), sh.len - 1) : sh.len - 1; };
+    const auto hi_of = [&](uint32_t r) { return A.causal ? min(sh.first + (int32_t)A.group.of(r), sh.len - 1) : sh.len - 1; };
     const auto lo_of = [&](uint32_t r) {
-        return A.window ? (int32_t)max((int64_t)sh.first + (int64_t)(r / group) - (int64_t)A.window + 1, (int64_t)0) : 0;
+        return A.window ? (int32_t)max((int64_t)sh.first + (int64_t)A.group.of(r) - (int64_t)A.window + 1, (int64_t)0) : 0;
     };
     const int32_t key_hi = live ? hi_of(row) : -1, key_lo = lo_of(row);
     const uint32_t last_row = min(row0 + kRowsTile - 1, rows - 1);
@@ -308,6 +308,16 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(Attenti
         vs = kv.v_scales[at];
     };
     uint32_t page_k = page_of(step, gk), page_v = page_of(step, g);
+    __builtin_amdgcn_sched_barrier(0);
+    // The queries' elements are on their way before the keys'.  Channels of the lane's operand k: two operands' lie in one 16-byte piece of
+    // a key's row.
+    Eight q[NK];
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+        const uint32_t d = (k | 1) < NK ? (uint32_t)(k & ~1) * 32 + g * 16 + (uint32_t)(k & 1) * 8 : (uint32_t)k * 32 + g * 8;
+        q[k] = load8(A.q, A.q_type, (size_t)(sh.row + (live ? tok : A.group.of(last_row))) * A.q_stride + (size_t)(kvh * group + A.group.rest(live ? row : last_row)) * D + d);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     if (step < end) {
         const uint8_t *kp = keys_at(step, page_k);
 #pragma unroll
@@ -316,24 +326,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(Attenti
     }
     uint32_t next_k = page_of(step + kAttnWaves, gk), next_v = page_of(step + kAttnWaves, g);
 
-    // channel d of the lane's operand k: 64 channels of two operands lie in one 16-byte piece of a key's row
-    if (wave == 0) {
-        Eight q[NK];
+    // (every wavefront scales the rows, each converts a quarter of the operands)
+    const QueryScale f = query_scale<NK, CAP, true>(A, q);
+    if (wave == 0 && g == 0) sq.factor[n] = f.factor;
 #pragma unroll
-        for (int k = 0; k < NK; k++) {
-            const uint32_t d = (k | 1) < NK ? (uint32_t)(k & ~1) * 32 + g * 16 + (uint32_t)(k & 1) * 8 : (uint32_t)k * 32 + g * 8;
-            q[k] = {};
-            if (live) q[k] = load8(A.q, A.q_type, (size_t)(sh.row + tok) * A.q_stride + (size_t)(kvh * group + row % group) * D + d);
+    for (int k = 0; k < NK; k++)
+        if ((uint32_t)k % kAttnWaves == wave) {
+            f16x8_t h, l;
+            query_f16<PAIRS>(q[k], f.mul, h, l);
+            sq.q[0][k][lane] = h;
+            if constexpr (PAIRS) sq.q[PAIRS ? 1 : 0][k][lane] = l;
         }
-        f16x8_t qh[NK], ql[PAIRS ? NK : 1];
-        const float f = query_f16<NK, PAIRS, CAP, true>(A, q, qh, ql);
-        if (g == 0) sq.factor[n] = f;
-#pragma unroll
-        for (int k = 0; k < NK; k++) {
-            sq.q[0][k][lane] = qh[k];
-            if constexpr (PAIRS) sq.q[PAIRS ? 1 : 0][k][lane] = ql[k];
-        }
-    }
     __syncthreads();
     const float factor = sq.factor[n];
 
@@ -474,10 +477,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(Attenti
             if (d == 0) part.ml[(slot * kRowsTile + r) * 2] = top, part.ml[(slot * kRowsTile + r) * 2 + 1] = l;
             continue;
         }
-        const uint32_t h = kvh * group + q % group;
+        const uint32_t h = kvh * group + A.group.rest(q);
         const float inv = inverse_sum(A, l, top, h);
         const f32x4_t v = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-        store4(A.out, A.out_type, (size_t)(sh.row + q / group) * A.out_stride + (size_t)h * D + d, v);
+        store4(A.out, A.out_type, (size_t)(sh.row + A.group.of(q)) * A.out_stride + (size_t)h * D + d, v);
     }
 }
 
@@ -530,14 +533,14 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
     __shared__ float sh_s[2][G][4];  // of each group of 16 keys: key scale, log2 of the value scale, and one over it
     const KvArgs &kv = A.kv;
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = lane % Sh::kRows, hi = lane / Sh::kRows;  // column; part of a k step
-    const uint32_t kvh = blockIdx.x % kv.kv_heads, group = A.q_heads / kv.kv_heads;  // (neighbours: the heads, one for each XCD's cache)
+    const uint32_t kvh = blockIdx.x % kv.kv_heads, group = A.group.d;  // (neighbours: the heads, one for each XCD's cache)
     Item it;
     Share sh;
     if (!find_item(A, P, blockIdx.x / kv.kv_heads, false, it, sh)) return;
     const uint32_t rows = sh.n * group;
     const uint32_t tile = sh.tiles - 1 - it.tile;  // (the last rows see the most keys: first)
 
-    const uint32_t row = tile * kTilesTile + wave * Sh::kRows + n, tok = row / group, head = kvh * group + row % group;
+    const uint32_t row = tile * kTilesTile + wave * Sh::kRows + n, tok = A.group.of(row), head = kvh * group + A.group.rest(row);
     const bool live = row < rows;
     const int32_t pos = sh.first + (int32_t)tok;
     const int32_t key_hi = !live ? -1 : (A.causal ? min(pos, sh.len - 1) : sh.len - 1);
@@ -551,14 +554,17 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
             q[k] = {};
             if (live) q[k] = load8(A.q, A.q_type, (size_t)(sh.row + tok) * A.q_stride + (size_t)head * D + (uint32_t)k * Sh::kStepDims + hi * 8);
         }
-        factor = query_f16<KD, PAIRS, CAP, tiles_narrow(NK, PAIRS)>(A, q, qh, ql);
+        const QueryScale f = query_scale<KD, CAP, tiles_narrow(NK, PAIRS)>(A, q);
+        factor = f.factor;
+#pragma unroll
+        for (int k = 0; k < KD; k++) query_f16<PAIRS>(q[k], f.mul, qh[k], ql[PAIRS ? k : 0]);
     }
     // what all and any of the wavefront's rows see (whole rows of lanes: the first and the last live one say it)
     const uint32_t first_row = tile * kTilesTile + wave * Sh::kRows, last_row = min(first_row + Sh::kRows - 1, rows - 1);
     const bool any_live = first_row < rows;
-    const auto hi_of = [&](uint32_t r) { return A.causal ? min(sh.first + (int32_t)(r / group), sh.len - 1) : sh.len - 1; };
+    const auto hi_of = [&](uint32_t r) { return A.causal ? min(sh.first + (int32_t)A.group.of(r), sh.len - 1) : sh.len - 1; };
     const auto lo_of = [&](uint32_t r) {
-        return A.window ? (int32_t)max((int64_t)sh.first + (int64_t)(r / group) - (int64_t)A.window + 1, (int64_t)0) : 0;
+        return A.window ? (int32_t)max((int64_t)sh.first + (int64_t)A.group.of(r) - (int64_t)A.window + 1, (int64_t)0) : 0;
     };
     const int32_t all_hi = hi_of(first_row), any_hi = any_live ? hi_of(last_row) : -1;
     const int32_t any_lo = lo_of(first_row), all_lo = lo_of(any_live ? last_row : first_row);
@@ -808,7 +814,7 @@ struct Join {
 __global__ void __launch_bounds__(kJoinWaves * 64) attention_join_kernel(AttentionArgs A, Join J) {
     __shared__ float sh_acc[kJoinWaves][256], sh_ml[kJoinWaves][2];
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, D = A.kv.head_dim, dim = min(lane * 4, D - 4), share = J.share;
-    const uint32_t kvh = blockIdx.y, group = A.q_heads / A.kv.kv_heads;
+    const uint32_t kvh = blockIdx.y, group = A.group.d;
     const bool second = blockIdx.x >= J.split_tiles[0];
     const Plan P = second ? J.plan[1] : J.plan[0];
     const Partials part = second ? J.part[1] : J.part[0];
@@ -840,10 +846,10 @@ __global__ void __launch_bounds__(kJoinWaves * 64) attention_join_kernel(Attenti
             }
         }
         if (r >= end || lane * 4 >= D) continue;
-        const uint32_t q = row0 + r, h = kvh * group + q % group;
+        const uint32_t q = row0 + r, h = kvh * group + A.group.rest(q);
         const float inv = inverse_sum(A, l, top, h);
         const f32x4_t v = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-        store4(A.out, A.out_type, (size_t)(sh.row + q / group) * A.out_stride + (size_t)h * D + lane * 4, v);
+        store4(A.out, A.out_type, (size_t)(sh.row + A.group.of(q)) * A.out_stride + (size_t)h * D + lane * 4, v);
     }
 }
 
@@ -910,7 +916,7 @@ hipError_t attention_launch(hipStream_t s, const AttentionArgs &A, void *workspa
         J.plan[i] = P;
         J.part[i] = part;
         J.split_tiles[i] = (uint32_t)Plans::split_tiles(A, P);
-        if (P.split) rows = std::max(rows, (uint32_t)std::min<uint64_t>((uint64_t)A.kv.max_new * (A.q_heads / A.kv.kv_heads), P.tile));
+        if (P.split) rows = std::max(rows, (uint32_t)std::min<uint64_t>((uint64_t)A.kv.max_new * A.group.d, P.tile));
     };
     if (p.use_tiles) run(p.tiles, true);
     if (p.use_rows) run(p.rows, false);

@@ -47,6 +47,18 @@ struct KvAppendArgs {
 constexpr size_t kMaxRowStride = 1u << 22;  // elements between tokens
 hipError_t kv_append_launch(hipStream_t s, const KvAppendArgs &A);
 
+// Division by a number that the host knows: (n * mul / 2^32 + n) / 2^shift, exact for every n below 2^31.
+struct Divisor {
+    uint32_t d, mul, shift;
+    static Divisor by(uint32_t d) {
+        uint32_t shift = 0;
+        while (((uint64_t)1 << shift) < d) shift++;
+        return {d, (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1), shift};
+    }
+    __host__ __device__ uint32_t of(uint32_t n) const { return ((uint32_t)(((uint64_t)n * mul) >> 32) + n) >> shift; }
+    __host__ __device__ uint32_t rest(uint32_t n) const { return n - of(n) * d; }
+};
+
 struct AttentionArgs {
     KvArgs kv;
     const void *q;
@@ -55,6 +67,7 @@ struct AttentionArgs {
     const float *sinks;
     int32_t q_type, out_type;
     uint32_t q_heads, window, causal;
+    Divisor group;  // query heads of a key/value head
     float scale, softcap;
 };
 size_t attention_workspace_bytes(const AttentionArgs &A);
