@@ -809,23 +809,25 @@ struct Join {
     Plan plan[2];
     Partials part[2];
     uint32_t split_tiles[2];  // at most
+    uint32_t parts[2];        // workgroups of a tile
     uint32_t share;
 };
 __global__ void __launch_bounds__(kJoinWaves * 64) attention_join_kernel(AttentionArgs A, Join J) {
     __shared__ float sh_acc[kJoinWaves][256], sh_ml[kJoinWaves][2];
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, D = A.kv.head_dim, dim = min(lane * 4, D - 4), share = J.share;
     const uint32_t kvh = blockIdx.y, group = A.group.d;
-    const bool second = blockIdx.x >= J.split_tiles[0];
+    const uint32_t of_first = J.split_tiles[0] * J.parts[0];
+    const bool second = blockIdx.x >= of_first;
     const Plan P = second ? J.plan[1] : J.plan[0];
     const Partials part = second ? J.part[1] : J.part[0];
-    if (blockIdx.z * kJoinRows >= P.tile) return;
+    const uint32_t at_tile = second ? blockIdx.x - of_first : blockIdx.x, parts = second ? J.parts[1] : J.parts[0], part_of = at_tile % parts;
     Item it;
     Share sh;
-    if (!find_item(A, P, blockIdx.x - (second ? J.split_tiles[0] : 0u), true, it, sh)) return;
+    if (!find_item(A, P, at_tile / parts, true, it, sh)) return;
     const uint32_t row0 = (P.tile == kTilesTile ? sh.tiles - 1 - it.tile : it.tile) * P.tile;
     const size_t at = ((size_t)kvh * part.slots + it.slot) * P.tile;
-    const uint32_t end = min((blockIdx.z + 1) * kJoinRows, min(P.tile, sh.n * group - row0));
-    for (uint32_t r0 = blockIdx.z * kJoinRows; r0 < end; r0 += kJoinWaves / share) {
+    const uint32_t end = min((part_of + 1) * kJoinRows, min(P.tile, sh.n * group - row0));
+    for (uint32_t r0 = part_of * kJoinRows; r0 < end; r0 += kJoinWaves / share) {
         const uint32_t r = r0 + wave / share;
         float top = kNoMax, l = 0.f;
         f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -916,14 +918,16 @@ hipError_t attention_launch(hipStream_t s, const AttentionArgs &A, void *workspa
         J.plan[i] = P;
         J.part[i] = part;
         J.split_tiles[i] = (uint32_t)Plans::split_tiles(A, P);
-        if (P.split) rows = std::max(rows, (uint32_t)std::min<uint64_t>((uint64_t)A.kv.max_new * A.group.d, P.tile));
+        const uint32_t most = (uint32_t)std::min<uint64_t>((uint64_t)A.kv.max_new * A.group.d, P.tile);
+        J.parts[i] = (most + kJoinRows - 1) / kJoinRows;
+        if (P.split) rows = std::max(rows, most);
     };
     if (p.use_tiles) run(p.tiles, true);
     if (p.use_rows) run(p.rows, false);
-    const uint32_t split = J.split_tiles[0] + J.split_tiles[1];
-    if (e != hipSuccess || split == 0) return e;
+    const uint32_t groups = J.split_tiles[0] * J.parts[0] + J.split_tiles[1] * J.parts[1];
+    if (e != hipSuccess || groups == 0) return e;
     J.share = rows <= 1 ? 8 : rows <= 2 ? 4 : rows <= 4 ? 2 : 1;
-    hipLaunchKernelGGL(attention_join_kernel, dim3(split, A.kv.kv_heads, (rows + kJoinRows - 1) / kJoinRows), dim3(kJoinWaves * 64), 0, s, A, J);
+    hipLaunchKernelGGL(attention_join_kernel, dim3(groups, A.kv.kv_heads), dim3(kJoinWaves * 64), 0, s, A, J);
     return hipGetLastError();
 }
 
