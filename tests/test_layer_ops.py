@@ -489,6 +489,8 @@ def attention_case(be, seqs, kv_heads=2, group=2, head_dim=64, page=16, t="f32",
         for s, (_, length) in enumerate(seqs):
             for j in range(-(-length // page)):
                 pg, n = c.table[s, j], min(page, length - j * page)
+                if not 0 <= pg < c.pages:
+                    continue
                 used.add(int(pg))
                 c.k[pg][:, n:], c.v[pg][:, :, n:] = 0x7F, 0xFF
         for pg in set(range(c.pages)) - used:
@@ -565,6 +567,17 @@ def test_attention_ways(be, how, out):
 @pytest.mark.parametrize("seqs", [[(1, 20000)], [(2, 9001), (1, 3), (1, 4097)], [(33, 5000)], [(1, 1 + 97 * i) for i in range(70)]])
 def test_attention_long_rows_in_pieces(be, t, out, seqs):
     attention_case(be, seqs, kv_heads=1, group=4, head_dim=64, page=64, t=t, out=out, spoil_tail=True)
+
+
+@gpu
+@pytest.mark.parametrize("t,out", [("f32", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("how", [{}, {"window": 900}, {"causal": False, "window": 2000}, {"softcap": 20.0}, {"sinks": [1.0, -1.0]},
+                                 {"holes": [(0, 3), (0, 40), (1, 0), (2, 17)]}])
+@pytest.mark.parametrize("head_dim", [64, 192])
+def test_attention_of_rows_in_pieces_beside_whole_ones(be, t, out, how, head_dim):
+    """Few and many rows, long and short, in one batch: both kernels, and the joining of both."""
+    attention_case(be, [(40, 3000), (1, 2500), (130, 1500), (2, 64), (20, 20), (5, 4100)], kv_heads=1, group=3, head_dim=head_dim, page=64, t=t,
+                   out=out, spoil_tail=True, **how)
 
 
 @gpu
