@@ -517,6 +517,17 @@ template <> struct Shape<true> {
     static __device__ __forceinline__ uint32_t group(uint32_t c, uint32_t part) { return 2 * c + part / 2; }
 };
 constexpr bool tiles_narrow(int nk, bool pairs) { return pairs || nk > 4; }
+// A narrow product's order in a wavefront: four reads from LDS ahead of the matrix instructions that use them, `per` for each.
+template <int READS, int PER>
+__device__ __forceinline__ void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < READS - 4; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, PER, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, 4 * PER, 0);
+}
 
 template <int NK, bool PAIRS, bool CAP>
 __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, NK > 4 && !tiles_narrow(NK, PAIRS) ? 1 : 2)
@@ -676,6 +687,7 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
                 if constexpr (PAIRS) S[t] = Sh::mma(ka, ql[k], S[t]);
             }
         }
+        if constexpr (tiles_narrow(NK, PAIRS)) reads_ahead<KD * ST, PAIRS ? 2 : 1>();
         // x(c, j): the lane's 8 scores of k step c, keys kStepKeys c + 8 hi + j; their logarithm (base 2) with the value scale: x a + e
         float a[KC], e[KC], unscale[KC];
 #pragma unroll
@@ -745,6 +757,7 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
                 acc[d] = Sh::mma(va, ph[c], acc[d]);
                 if constexpr (PAIRS) acc[d] = Sh::mma(va, pl[c], acc[d]);
             }
+        if constexpr (tiles_narrow(NK, PAIRS)) reads_ahead<KC * DT, PAIRS ? 2 : 1>();
     }
 #pragma unroll
     for (uint32_t d = Sh::kRows; d < 64; d *= 2) L += __shfl_xor(L, (int)d, 64);
