@@ -25,7 +25,9 @@ constexpr uint32_t kAttnThreads = 256;
 constexpr uint32_t kAttnWaves = kAttnThreads / 64;
 constexpr uint32_t kRowsTile = 16;      // query rows of a workgroup of the kernel for few rows
 constexpr uint32_t kTilesTile = 128;    // ... for many, 32 a wavefront
-constexpr uint32_t kFewRows = 32;       // a sequence with at most this many rows for each key/value head goes through the former
+// A sequence with at most this many rows for each key/value head goes through the former.  16 sequences of 4000 keys, us through it / through the
+// latter: 24 rows 51 / 53 (128 channels, bf16), 86 / 98 (256, f32); 32 rows 51 / 54, 87 / 101; 56 rows 93 / 62, 156 / 111.
+constexpr uint32_t kFewRows = 32;
 constexpr float kLog2E = 1.44269504088896341f;
 // Weights are held as 2^(t + e - M + 7) with t + e - M <= 3; M is whole and only moves where a score leaves that range, so it brings no
 // rounding, and the one of the exponent is that of a number of at most 10.  The f16 pair of an f32 weight keeps 22 bits down to 2^-10 of the
@@ -140,8 +142,11 @@ static Plans plans_of(const AttentionArgs &A) {
     // them: 148, 103, 125, 110, joining included), 3 below (64 sequences, 64 channels: 44, 37, 33, 37); a wavefront's step each at least.
     p.rows = {kRowsTile, 1, kFewRows, std::max((A.kv.head_dim > 128 ? 2 : 3) * cus / A.kv.kv_heads, 1u), kAttnWaves, 1, 0};
     p.rows.split = steps > p.rows.min_steps;
+    // Many rows: as many as are resident, unless the tiles by themselves (of which a sequence's last is half full, say) are as many: splitting
+    // then is a launch more for nothing (2048 tokens of 32/8 heads of 128: 76 us whole, 88 with it; 16 sequences of 32 tokens, 256 channels,
+    // f32: 239 and 165).
     p.tiles = {kTilesTile, kFewRows + 1, 0xFFFFFFFFu, std::max((A.kv.head_dim > 128 ? 1 : 2) * cus / A.kv.kv_heads, 1u), 8, 1, 6};
-    p.tiles.split = steps > p.tiles.min_steps && A.kv.tokens * group / p.tiles.tile + A.kv.sequences < p.tiles.target;
+    p.tiles.split = steps > p.tiles.min_steps && A.kv.tokens * group / p.tiles.tile + A.kv.sequences / 2 < p.tiles.target;
     p.use_tiles = most > kFewRows;
     p.use_rows = !p.use_tiles || A.kv.sequences > 1;
     if (!p.use_rows) p.tiles.rows_min = 1;  // one sequence: one kernel, whatever its number of new tokens turns out to be
