@@ -242,9 +242,9 @@ __device__ __forceinline__ void query_f16(const Eight &q, float mul, f16x8_t &h,
 // end.  A wavefront reads its step's codes straight into the registers that the matrix instructions' operands are converted
 // from, 64 x head_dim bytes of K and then of V through ONE set of registers: as a part of the keys is multiplied its registers take a part
 // of the step's values, and as that is multiplied a part of the next step's keys, so about 64 x head_dim bytes are always in flight and
-// two wavefronts fit a SIMD at every head_dim.  The queries' operands are read from LDS.
+// two wavefronts fit a SIMD above 128 channels and three below.  The queries' operands are read from LDS.
 template <int NK, bool PAIRS, bool CAP>
-__global__ void __launch_bounds__(kAttnThreads, 2) attention_rows_kernel(AttentionArgs A, Plan P, Partials part) {
+__global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_kernel(AttentionArgs A, Plan P, Partials part) {
     constexpr uint32_t D = NK * 32, kPad = D + 4;
     constexpr int NP = (NK + 1) / 2;  // parts: 64 channels of the keys, 64 channels of the values
     struct Queries {
