@@ -29,10 +29,12 @@ constexpr uint32_t kTilesTile = 128;    // ... for many, 32 a wavefront
 // latter: 24 rows 51 / 53 (128 channels, bf16), 86 / 98 (256, f32); 32 rows 51 / 54, 87 / 101; 56 rows 93 / 62, 156 / 111.
 constexpr uint32_t kFewRows = 32;
 constexpr float kLog2E = 1.44269504088896341f;
-// Weights are held as 2^(t + e - M + 7) with t + e - M <= 3; M is whole and only moves where a score leaves that range, so it brings no
-// rounding, and the one of the exponent is that of a number of at most 10.  The f16 pair of an f32 weight keeps 22 bits down to 2^-10 of the
-// largest and 2^-32 of it beyond (131072 equal weights 2^-17 of one that weighs as much as they all: 2^-15 each, at random).
-constexpr float kBias = 7.f, kSlack = 3.f;
+// Weights are held as 2^(t + e - M + bias) with t + e - M <= 3; M is whole and only moves where a score leaves that range, so it brings no
+// rounding.  f16 pairs: the bias is small, for the exponent is rounded as a number of its size; a pair keeps 22 bits down to 2^-10 of the
+// largest and 2^-32 of it beyond (131072 equal weights 2^-17 of one that weighs as much as they all: 2^-15 each, at random).  One f16: as
+// large as fits, 11 bits down to 2^-26 of the largest.
+constexpr float kPairsBias = 7.f, kOneBias = 12.f, kSlack = 3.f;
+__device__ __forceinline__ float weight_bias(bool pairs) { return pairs ? kPairsBias : kOneBias; }
 constexpr float kNoMax = -1e30f;
 
 // How one of the two kernels shares its work out.
@@ -175,6 +177,18 @@ __device__ __forceinline__ void weights_f16(f32x2_t p, f16x8_t &h, f16x8_t &l, i
     }
 }
 
+// Weights of one f16 are summed as they enter the matrix instructions, so that a rounding moves numerator and sum alike, unless the value
+// scale of one of the wavefront's blocks is so far (kFar) below the largest met that its weights may be nothing in f16 and still count: those are
+// summed in f32.
+constexpr int kFar = 8;
+__device__ __forceinline__ float weights_sum(const f16x8_t &h) {
+    const f16x2_t one = {(_Float16)1.f, (_Float16)1.f};
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) sum = __builtin_amdgcn_fdot2(f16x2_t{h[j], h[j + 1]}, one, sum, false);
+    return sum;
+}
+
 // Partial results of pieces: [kv_heads][slots][tile][head_dim] weighted sums, and [kv_heads][slots][tile] maxima and sums of weights.
 struct Partials {
     float *acc, *ml;
@@ -183,7 +197,7 @@ struct Partials {
 
 // A result row's end: the sink, the quotient.
 __device__ __forceinline__ float inverse_sum(const AttentionArgs &A, float l, float top, uint32_t head) {
-    if (A.sinks && l != 0.f) l += __builtin_amdgcn_exp2f(fmaf(A.sinks[head], kLog2E, kBias - top));
+    if (A.sinks && l != 0.f) l += __builtin_amdgcn_exp2f(fmaf(A.sinks[head], kLog2E, weight_bias(A.out_type == ELEM_F32) - top));
     return l == 0.f ? 0.f : 1.f / l;
 }
 
@@ -349,6 +363,7 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
 #pragma unroll
     for (int i = 0; i < 2 * NK; i++) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float M = kNoMax, L = 0.f;
+    int e_top = -1000;  // the largest logarithm of a value scale met
     for (; step < end; step += kAttnWaves) {
         const int32_t key0 = (int32_t)(step * kStep);
         const bool hole = page_v == ~0u;
@@ -413,13 +428,23 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
         }
         f16x8_t ph[2], pl[2];
         float sum = 0.f;
-        const float shift = e - M + kBias;
+        const float shift = e - M + weight_bias(PAIRS);
+        const bool far = !PAIRS && __ballot(ev < e_top - kFar && !hole) != 0;
+        e_top = hole ? e_top : max(e_top, ev);
+        float far_sum = 0.f;
+        if (far) {
+            float shift_of = shift;
+            asm volatile("" : "+v"(shift_of));  // (exponentials of its own: those below are to mix with the matrix instructions)
+#pragma unroll
+            for (int i = 0; i < 16; i++) far_sum += __builtin_amdgcn_exp2f(fmaf(S[i / 4][i % 4], a, shift_of));
+        }
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
             const f32x2_t p = {__builtin_amdgcn_exp2f(fmaf(S[i / 4][i % 4], a, shift)), __builtin_amdgcn_exp2f(fmaf(S[i / 4][i % 4 + 1], a, shift))};
             weights_f16<PAIRS>(p, ph[i / 8], pl[i / 8], i % 8);
-            sum += p[0] + p[1];  // (the f32 weights: one of a block of small values may be nothing in f16, and counts here)
+            if constexpr (PAIRS) sum += p[0] + p[1];
         }
+        if constexpr (!PAIRS) sum = far ? far_sum : weights_sum(ph[0]) + weights_sum(ph[1]);
         L = fmaf(sum, unscale, L);
         if (!plain) {  // bytes behind the last key may be anything
             const int32_t have = hole ? 0 : sh.len - key0 - (int32_t)g * 16;
@@ -546,7 +571,7 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
     static_assert(Sh::kRows * Sh::kWaves == kTilesTile, "a workgroup's rows");
     __shared__ __align__(16) _Float16 sh_k[2][kKeys][kKeyPad];
     __shared__ __align__(16) _Float16 sh_v[2][D][kValPad];
-    __shared__ float sh_s[2][G][4];  // of each group of 16 keys: key scale, log2 of the value scale, and one over it
+    __shared__ float sh_s[2][G][4];  // of each group of 16 keys: key scale, log2 of the value scale, one over it, and whether the turn has a far one
     const KvArgs &kv = A.kv;
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = lane % Sh::kRows, hi = lane / Sh::kRows;  // column; part of a k step
     const uint32_t kvh = blockIdx.x % kv.kv_heads, group = A.group.d;  // (neighbours: the heads, one for each XCD's cache)
@@ -596,6 +621,7 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
     // Staging: a piece is 16 channels of a key's row, or 16 keys of a value channel's.
     u32x4_t kc[kPieces], vc[kPieces];
     float ks = 0.f, vs = 0.f;
+    int e_top = -1000;  // the largest logarithm of a value scale met
     // The pages of a step, that of group lane % 4 in a lane: read one step before its codes.
     const auto pages_of = [&](uint32_t st) -> uint32_t {
         const uint32_t key = st * kKeys + lane % G * 16;
@@ -657,6 +683,13 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
             sh_s[buf][threadIdx.x][0] = odd ? __builtin_nanf("") : ks;
             sh_s[buf][threadIdx.x][1] = hole ? -__builtin_inff() : (float)ev;
             sh_s[buf][threadIdx.x][2] = hole ? 0.f : __builtin_bit_cast(float, (uint32_t)(127 - ev) << 23);
+            if constexpr (!PAIRS) {  // whether one of the turn's blocks is far below the largest met (weights_sum)
+                int low = hole ? 0x7FFFFFFF : ev;
+                e_top = max(e_top, hole ? -1000 : ev);
+#pragma unroll
+                for (int m = 1; m < (int)G; m *= 2) low = min(low, __shfl_xor(low, m, 64)), e_top = max(e_top, __shfl_xor(e_top, m, 64));
+                sh_s[buf][threadIdx.x][3] = low < e_top - kFar ? 1.f : 0.f;
+            }
         }
     };
 
@@ -695,6 +728,7 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
         if constexpr (tiles_narrow(NK, PAIRS)) reads_ahead<KD * ST, PAIRS ? 2 : 1>();
         // x(c, j): the lane's 8 scores of k step c, keys kStepKeys c + 8 hi + j; their logarithm (base 2) with the value scale: x a + e
         float a[KC], e[KC], unscale[KC];
+        const bool far = !PAIRS && __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sh_s[buf][0][3])) != 0;
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             const uint32_t grp = Sh::group(c, hi);
@@ -730,7 +764,8 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
             for (int j = 1; j < 8; j++) m = fmaxf(m, LARQL_X(c, j));
             top = fmaxf(top, fmaf(m, a[c], e[c]));
         }
-        if (__ballot(top > M + kSlack)) {
+        float far_sum = 0.f;
+        if (far || __ballot(top > M + kSlack)) {
 #pragma unroll
             for (uint32_t d = Sh::kRows; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, (int)d, 64));
             const float next = top > M + kSlack ? ceilf(top) : M;
@@ -739,20 +774,34 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
             L *= f;
 #pragma unroll
             for (int i = 0; i < DT; i++) acc[i] *= f;
+            if (far) {  // (exponentials of its own, hidden from the compiler: those below are to mix with the matrix instructions)
+                float top_of = M;
+                asm volatile("" : "+v"(top_of));
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) sum += __builtin_amdgcn_exp2f(fmaf(LARQL_X(c, j), a[c], e[c] - top_of + weight_bias(PAIRS)));
+                    far_sum = fmaf(sum, unscale[c], far_sum);
+                }
+            }
         }
         f16x8_t ph[KC], pl[KC];
+        float near_sum = 0.f;
 #pragma unroll
         for (int c = 0; c < KC; c++) {
-            const float shift = e[c] - M + kBias;
+            const float shift = e[c] - M + weight_bias(PAIRS);
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 const f32x2_t p = {__builtin_amdgcn_exp2f(fmaf(LARQL_X(c, j), a[c], shift)), __builtin_amdgcn_exp2f(fmaf(LARQL_X(c, j + 1), a[c], shift))};
                 weights_f16<PAIRS>(p, ph[c], pl[c], j);
-                sum += p[0] + p[1];  // (the f32 weights: one of a block of small values may be nothing in f16, and counts here)
+                if constexpr (PAIRS) sum += p[0] + p[1];
             }
-            L = fmaf(sum, unscale[c], L);
+            if constexpr (!PAIRS) sum = weights_sum(ph[c]);
+            near_sum = fmaf(sum, unscale[c], near_sum);
         }
+        L += far ? far_sum : near_sum;
 #undef LARQL_X
 #pragma unroll
         for (int c = 0; c < KC; c++)
