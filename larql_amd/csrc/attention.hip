@@ -429,8 +429,17 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
         f16x8_t ph[2], pl[2];
         float sum = 0.f;
         const float shift = e - M + weight_bias(PAIRS);
-        const bool far = !PAIRS && __ballot(ev < e_top - kFar && !hole) != 0;
-        e_top = hole ? e_top : max(e_top, ev);
+        bool far = false;
+        if constexpr (!PAIRS) {  // (a row's weights lie in all four groups' lanes)
+            int low = 0x7FFFFFFF;
+#pragma unroll
+            for (int grp = 0; grp < 4; grp++) {
+                const int of_group = __builtin_amdgcn_readlane(hole ? 0x7FFFFFFF : ev, 16 * grp);
+                low = min(low, of_group);
+                e_top = max(e_top, of_group == 0x7FFFFFFF ? e_top : of_group);
+            }
+            far = low < e_top - kFar;
+        }
         float far_sum = 0.f;
         if (far) {
             float shift_of = shift;

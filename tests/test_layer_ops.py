@@ -597,16 +597,23 @@ def test_attention_prompts_of_every_head_dim(be, head_dim, t, out):
 
 
 @gpu
-def test_attention_weighs_blocks_of_very_different_scales(be):
+@pytest.mark.parametrize("head_dim", [64, 256])
+@pytest.mark.parametrize("out", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("seqs", [[(1, 200), (4, 130)], [(70, 200), (64, 64)]])
+def test_attention_weighs_blocks_of_very_different_scales(be, seqs, out, head_dim):
     rng = np.random.default_rng(9)
-    seqs = [(1, 200), (4, 130)]
-    c = Cache(rng, seqs, 2, 64, 16)
-    # value blocks 2^-40 .. 2^60 apart from each other in one row, the large ones on keys that weigh little
-    c.vs[:] = np.exp2(rng.integers(-40, 61, c.vs.shape)).astype(np.float32)
-    attention_case(be, seqs, cache=c)
-    c = Cache(rng, seqs, 2, 64, 16)
-    c.vs[:] = np.exp2(rng.integers(-12, 8, c.vs.shape)).astype(np.float32)
-    attention_case(be, seqs, cache=c, q_sigma=6.0)
+    t = "f32" if out == "f32" else "f16"
+    if out != "f16":  # value blocks 2^-40 .. 2^60 apart from each other in one row, the large ones on keys that weigh little
+        c = Cache(rng, seqs, 2, head_dim, 16)
+        c.vs[:] = np.exp2(rng.integers(-40, 61, c.vs.shape)).astype(np.float32)
+        attention_case(be, seqs, cache=c, head_dim=head_dim, t=t, out=out)
+    c = Cache(rng, seqs, 2, head_dim, 16)
+    c.vs[:] = np.exp2(rng.integers(-12, 4, c.vs.shape)).astype(np.float32)
+    attention_case(be, seqs, cache=c, head_dim=head_dim, t=t, out=out, q_sigma=6.0)
+    # and those of one row that its weights all but leave out
+    c.vs[:] = 2.0 ** -20
+    c.vs[::3] = 1.0
+    attention_case(be, seqs, cache=c, head_dim=head_dim, t=t, out=out, q_sigma=3.0)
 
 
 @gpu
