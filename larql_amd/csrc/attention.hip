@@ -9,6 +9,10 @@
 // Codes are exact in f16.  The key scale enters the scores' factor and the value scale, a power of two 2^e, the exponent:
 //   weight 2^(t + e - M), M the running maximum of t + e, times the bare code;  sum of weights: 2^(t + e - M) * 2^-e.
 // So neither costs an instruction for each element, and numerators keep their precision whatever the blocks' scales.
+//
+// Measured: one token over 131072 keys of 16/8 heads of 256, f32: 95 us, 5.7 TB/s of codes (reads reach 6.5), and 7 of joining; 32 sequences of 4000
+// keys of 32/8 heads of 128: 49 us, 5.3 TB/s.  A prompt of 8192 tokens, causal: 32/8 heads of 128, bf16, 640-700 us, 0.79-0.86 PFLOP/s at a clock of
+// 1.95 GHz (a large bf16 product of the library: 1.24); 8/4 heads of 256: bf16 400 us, f32 (twice the matrix instructions) 457.
 #include <algorithm>
 
 #include "kernels.h"

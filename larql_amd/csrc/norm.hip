@@ -1,6 +1,8 @@
 // norm.hip — the residual between two blocks and the norms around it:
 //   h' = h + s * g . rms(b; w_post),  n = rms(h'; w_pre),  rms(x; w) = x / sqrt(mean(x^2) + eps) * (offset + w)
-// A row is read once and kept in registers over both reductions.
+// A row is read once and kept in registers over both reductions, so many rows are bound by memory: 4096 of 3840 (f32 block and stream, bf16
+// result) take 39.4 us, 5.6 TB/s of reads and writes (a large copy: 5.0).  A single row is bound by its chain of launch, load and two sums:
+// 2.8 us at 2560, of which an empty launch is about 2.  A thread holds 8 elements where the row's threads allow it (fewer waits a row), at most 32.
 #include "kernels.h"
 #include "layer.h"
 
