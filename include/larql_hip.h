@@ -534,7 +534,8 @@ int  larql_hip_dev_moe_layer_forward(larql_hip_ctx *ctx, larql_hip_moe_layer *la
  * and the norm before the next block in one pass.  Every part is optional: block NULL (h' = h), post_weight NULL (b as it
  * is), gate NULL (1), residual_out NULL (h' not wanted), normed NULL (n not wanted), pre_weight NULL (weights of n all
  * ones: norm_offset does not enter).  gate is f32 [hidden] for all rows (gate_stride 0) or one row for each.  n is taken
- * from h' before h' is rounded to its format.  residual_out may be residual, and normed may be block; no other overlap.
+ * from h' before h' is rounded to its format.  residual_out may be residual, and normed may be block (of the same element
+ * size and stride, else LARQL_REFUSED_SHAPE); no other overlap.
  * Strides are elements between rows, at least hidden.  hidden <= 32768 (else LARQL_UNSUPPORTED). */
 typedef struct {
     size_t rows, hidden;
@@ -574,7 +575,7 @@ typedef struct {
  * tokens of sequence s with the new ones; its new tokens are rows q_start[s] .. q_start[s+1] of the activations and the last
  * ones of the sequence.  block_table[s] lists its pages; an entry outside [0, num_pages) is a hole: nothing is written
  * there, and its tokens are masked.  A sequence whose rows do not fit (q_start falling, beyond `tokens`, or more than
- * max_new_tokens of them) is left out, its rows untouched.  Up to 2^20 sequences, 2^24 new tokens and tables of 2^30 tokens
+ * max_new_tokens of them) is left out, its rows untouched.  Up to 2^16 sequences, 2^24 new tokens and tables of 2^30 tokens
  * (more: LARQL_UNSUPPORTED). */
 typedef struct {
     const int32_t *kv_len;         /* [sequences] */
@@ -589,7 +590,8 @@ typedef struct {
  * the queries, normed (q_norm) and rotated alike, to q_out (q NULL: none).  Channel pairs (i, i + rot_dim/2), or
  * (2i, 2i+1) where `interleaved`, of the first rot_dim channels turn by position * inv_freq[i] (the angle is reduced in 64
  * bits) and are scaled by rope_scale; rot_dim 0: no rotation.  Positions count from the sequence's first token.  Rows are
- * [heads, head_dim], strides elements between tokens, at most 2^22 (k, v and q may be parts of one fused row); q_out may be q.
+ * [heads, head_dim], strides elements between tokens, at most 2^22 (k, v and q may be parts of one fused row); q_out may be q (with its
+ * stride, else LARQL_REFUSED_SHAPE).
  * Two sequences must not append to one page.  Appending the same tokens again changes nothing. */
 typedef struct {
     int format;                    /* of q, k, v and q_out */

@@ -2587,11 +2587,15 @@ static int check_residual_norm(larql_hip_ctx *c, const larql_hip_residual_norm *
     A.residual_scale = a->residual_scale; A.norm_offset = a->norm_offset; A.eps = a->eps;
     const size_t es = elem_bytes(A.residual_type), eb = elem_bytes(A.block_type), en = elem_bytes(A.normed_type);
     const auto whole = [&](const void *p, size_t stride, size_t item) { return !p || (((uintptr_t)p & 15) == 0 && stride * item % 16 == 0); };
+    const bool many = a->rows > 1;  // (one row: its stride is not used)
+    if ((A.residual_out == A.residual && many && A.residual_out_stride != A.residual_stride) ||
+        (A.normed && A.normed == A.block && (en != eb || (many && A.normed_stride != A.block_stride))))
+        return fail(c, LARQL_REFUSED_SHAPE, "residual_norm: a result in place of its operand has the same element size and row stride");
     const auto natural = [](const void *p, size_t item) { return ((uintptr_t)p & (item - 1)) == 0; };
     if (!natural(A.block, eb) || !natural(A.residual, es) || !natural(A.residual_out, es) || !natural(A.normed, en) || !natural(A.gate, 4) ||
         !natural(A.post_weight, 4) || !natural(A.pre_weight, 4))
         return fail(c, LARQL_REFUSED_SHAPE, "residual_norm: an operand is not aligned to its elements");
-    const size_t several = a->rows > 1;  // (one row: its stride is not used)
+    const size_t several = many;
     A.vec = a->hidden % 8 == 0 && whole(A.block, several * A.block_stride, eb) && whole(A.residual, several * A.residual_stride, es) &&
             whole(A.residual_out, several * A.residual_out_stride, es) && whole(A.normed, several * A.normed_stride, en) &&
             whole(A.gate, several * A.gate_stride, 4) && whole(A.post_weight, 0, 4) && whole(A.pre_weight, 0, 4);
@@ -2610,7 +2614,7 @@ static int check_kv(larql_hip_ctx *c, const char *what, const larql_hip_kv_cache
     *empty = b->sequences == 0 || b->tokens == 0 || b->max_new_tokens == 0;
     if (*empty) return LARQL_OK;
     if (k->num_pages == 0 || b->table_width == 0) return fail(c, LARQL_REFUSED_SHAPE, "%s: a cache without pages", what);
-    if (k->num_pages > 0x7FFFFFFFull || b->sequences > (1u << 20) || b->table_width > (1u << 30) / k->page_tokens || b->tokens > (1u << 24))
+    if (k->num_pages > 0x7FFFFFFFull || b->sequences > (1u << 16) || b->table_width > (1u << 30) / k->page_tokens || b->tokens > (1u << 24))
         return fail(c, LARQL_UNSUPPORTED, "%s: too large", what);
     if (!k->k_codes || !k->v_codes || !k->k_scales || !k->v_scales || !b->kv_len || !b->block_table || !b->q_start) return LARQL_E_ARG;
     if (((uintptr_t)k->k_codes | (uintptr_t)k->v_codes) & 15) return fail(c, LARQL_REFUSED_SHAPE, "%s: codes must be 16-byte aligned", what);
@@ -2648,6 +2652,8 @@ static int check_kv_append(larql_hip_ctx *c, const larql_hip_kv_cache *k, const 
         return fail(c, LARQL_REFUSED_SHAPE, "kv_append: rows must be 16-byte aligned and hold all heads");
     if (std::max(a->k_stride, a->v_stride) > kMaxRowStride || (with_q && std::max(a->q_stride, a->q_out_stride) > kMaxRowStride))
         return fail(c, LARQL_UNSUPPORTED, "kv_append: strides of more than 2^22 elements");
+    if (with_q && a->q_out == a->q && A.kv.tokens > 1 && a->q_out_stride != a->q_stride)
+        return fail(c, LARQL_REFUSED_SHAPE, "kv_append: queries in place have one row stride");
     if (((uintptr_t)a->q_norm | (uintptr_t)a->k_norm) & 15) return fail(c, LARQL_REFUSED_SHAPE, "kv_append: norm weights must be 16-byte aligned");
     if ((uintptr_t)a->inv_freq & 3) return fail(c, LARQL_REFUSED_SHAPE, "kv_append: inv_freq must be 4-byte aligned");
     A.q = with_q ? a->q : nullptr; A.k = a->k; A.v = a->v; A.q_out = a->q_out;

@@ -860,7 +860,7 @@ _KV = [("cache", "head_dim", 0, L.REFUSED_SHAPE), ("cache", "head_dim", 48, L.RE
        ("cache", "page_tokens", 0, L.REFUSED_SHAPE), ("cache", "page_tokens", 24, L.REFUSED_SHAPE), ("cache", "page_tokens", 256, L.REFUSED_SHAPE),
        ("cache", "kv_heads", 0, L.REFUSED_SHAPE), ("cache", "kv_heads", 5000, L.REFUSED_SHAPE), ("cache", "num_pages", 0, L.REFUSED_SHAPE),
        ("cache", "num_pages", 1 << 31, L.UNSUPPORTED), ("cache", "k_codes", 4104, L.REFUSED_SHAPE), ("cache", "v_codes", None, L.E_ARG),
-       ("cache", "k_scales", 66, L.REFUSED_SHAPE), ("batch", "table_width", 0, L.REFUSED_SHAPE), ("batch", "table_width", (1 << 26) + 1, L.UNSUPPORTED), ("batch", "sequences", 1 << 21, L.UNSUPPORTED),
+       ("cache", "k_scales", 66, L.REFUSED_SHAPE), ("batch", "table_width", 0, L.REFUSED_SHAPE), ("batch", "table_width", (1 << 26) + 1, L.UNSUPPORTED), ("batch", "sequences", (1 << 16) + 1, L.UNSUPPORTED),
        ("batch", "tokens", 1 << 25, L.UNSUPPORTED), ("batch", "q_start", None, L.E_ARG), ("batch", "block_table", 66, L.REFUSED_SHAPE),
        ("batch", "kv_len", None, L.E_ARG)]
 _APP = [("app", "format", hip.FMT_Q4_K, L.UNSUPPORTED), ("app", "rot_dim", 72, L.REFUSED_SHAPE), ("app", "rot_dim", 12, L.REFUSED_SHAPE),
@@ -886,6 +886,26 @@ def test_refusals(op, which, field, value, code):
     assert _call(op, s) == code
     if op == "att":
         assert L.lib.larql_hip_attention_workspace_bytes(ctypes.byref(s["cache"]), ctypes.byref(s["batch"]), ctypes.byref(s["att"])) == 0
+
+
+# A result in place of its operand: the same rows, or another row's elements are overwritten before they are read.
+@pytest.mark.parametrize("how,code", [({"normed": 4096, "normed_format": FMT["f32"]}, L.E_ARG), ({"normed": 4096}, L.REFUSED_SHAPE),
+                                      ({"normed": 4096, "normed_format": FMT["f32"], "normed_stride": 128}, L.REFUSED_SHAPE),
+                                      ({"normed": 4096, "normed_format": FMT["f32"], "normed_stride": 128, "rows": 1}, L.E_ARG),
+                                      ({"normed": 4096, "rows": 1}, L.REFUSED_SHAPE), ({"residual_out": 4096 + 4096, "residual": 8192}, L.E_ARG),
+                                      ({"residual": 8192, "residual_out_stride": 128}, L.REFUSED_SHAPE)])
+def test_a_norms_result_in_place_has_the_operands_rows(how, code):
+    s = _sound()
+    for field, value in how.items():
+        setattr(s["norm"], field, value)
+    assert _call("norm", s) == code
+
+
+@pytest.mark.parametrize("stride,tokens,code", [(256, 3, L.E_ARG), (512, 3, L.REFUSED_SHAPE), (512, 1, L.E_ARG)])
+def test_queries_rotated_in_place_have_the_same_rows(stride, tokens, code):
+    s = _sound()
+    s["app"].q_out, s["app"].q_out_stride, s["batch"].tokens = s["app"].q, stride, tokens
+    assert _call("app", s) == code
 
 
 def test_refusals_of_the_workspace_and_of_null_arguments():
