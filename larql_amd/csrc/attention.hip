@@ -28,7 +28,7 @@ constexpr uint32_t kStep = 64;          // keys of a step
 constexpr uint32_t kAttnThreads = 256;
 constexpr uint32_t kAttnWaves = kAttnThreads / 64;
 constexpr uint32_t kRowsTile = 16;      // query rows of a workgroup of the kernel for few rows
-constexpr uint32_t kTilesTile = 128;    // ... for many, 32 a wavefront
+constexpr uint32_t kTilesTile = 128;    // ... for many
 // A sequence with at most this many rows for each key/value head goes through the former.  16 sequences of 4000 keys, us through it / through the
 // latter: 24 rows 51 / 53 (128 channels, bf16), 86 / 98 (256, f32); 32 rows 51 / 54, 87 / 101; 56 rows 93 / 62, 156 / 111.
 constexpr uint32_t kFewRows = 32;
@@ -131,13 +131,13 @@ __device__ __forceinline__ bool find_item(const AttentionArgs &A, const Plan &P,
 struct Plans {
     Plan rows, tiles;
     bool use_rows, use_tiles;
-    static uint64_t items(const AttentionArgs &A, const Plan &P) {
-        return A.kv.tokens * (uint64_t)A.group.d / P.tile + A.kv.sequences + (P.split ? P.target + 1 : 0);
+    static uint64_t tiles_at_most(const AttentionArgs &A, const Plan &P) {
+        const uint64_t of_rows = A.kv.tokens * (uint64_t)A.group.d / P.tile + A.kv.sequences;  // (of few rows: a sequence's are few)
+        return std::min(of_rows, A.kv.sequences * (((uint64_t)P.rows_max + P.tile - 1) / P.tile));
     }
+    static uint64_t items(const AttentionArgs &A, const Plan &P) { return tiles_at_most(A, P) + (P.split ? P.target + 1 : 0); }
     static uint64_t slots(const Plan &P) { return P.split ? 2 * P.target + 2 : 0; }
-    static uint64_t split_tiles(const AttentionArgs &A, const Plan &P) {
-        return P.split ? std::min<uint64_t>(P.target + 1, A.kv.tokens * (uint64_t)A.group.d / P.tile + A.kv.sequences) : 0;
-    }
+    static uint64_t split_tiles(const AttentionArgs &A, const Plan &P) { return P.split ? std::min<uint64_t>(P.target + 1, tiles_at_most(A, P)) : 0; }
 };
 static Plans plans_of(const AttentionArgs &A) {
     const uint64_t group = A.group.d, most = A.kv.max_new * group;
@@ -206,12 +206,21 @@ __device__ __forceinline__ float inverse_sum(const AttentionArgs &A, float l, fl
 }
 
 // The logarithm (base 2) of a capped score's weight, plus e: cap * tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1), where s a is the
-// exponent of that as a power of two (query_f16).
+// exponent of that as a power of two (query_scale).  That is off by what 32 bits leave of the cap,
+// little beside the weights' own rounding for caps up to kLowCap.  SERIES: a score below 0.26 of its cap takes the series of tanh (next term
+// below 2e-8 of it), so that a cap far above the scores costs them nothing.  Many rows take it above kLowCap only (a causal prompt of 8192,
+// 32/8 heads of 128: 1001 us for 866), few rows, which wait for memory, always.
+constexpr float kLowCap = 64.f;
+template <bool SERIES>
 __device__ __forceinline__ float capped(const AttentionArgs &A, float s, float a, float e) {
-    const float c = A.softcap * kLog2E;
-    return fmaf(-2.f * c, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a) + 1.f), c + e);
+    const float c = A.softcap * kLog2E, z = s * a;
+    const float whole = fmaf(-2.f * c, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(z) + 1.f), c + e);
+    if constexpr (!SERIES) return whole;
+    constexpr float u2 = 0.120113253f;  // (ln 2 / 2)^2: x / cap = z ln 2 / 2
+    const float t = z * z;
+    const float series = fmaf(t, fmaf(t, fmaf(t, fmaf(t, u2 * u2 * u2 * u2 * 62.f / 2835.f, u2 * u2 * u2 * -17.f / 315.f), u2 * u2 * 2.f / 15.f), u2 / -3.f), 1.f);
+    return fabsf(z) < 0.75f ? fmaf(A.softcap * 0.5f * z, series, e) : whole;
 }
-
 // Scores s of a step with hidden keys, whose logarithms are s a + e: a hidden one is -inf, times a factor that is positive; a factor that is
 // not (a scale of 0, a block that is no number) goes into the scores that are seen.
 struct Seen {
@@ -283,8 +292,8 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
     if (!find_item(A, P, blockIdx.x, false, it, sh)) return;
     const uint32_t rows = sh.n * group;
 
-    // The lane's query row: token and head, what it sees.  What all and any of the rows see: the first and the last say it.
-    const uint32_t row0 = it.tile * kRowsTile, row = row0 + n, tok = A.group.of(row);
+    // The lane's query row, and what it sees.  What all and any of the rows see: the first and the last say it.
+    const uint32_t row0 = it.tile * kRowsTile, row = row0 + n;
     const bool live = row < rows;
     const auto hi_of = [&](uint32_t r) { return A.causal ? min(sh.first + (int32_t)A.group.of(r), sh.len - 1) : sh.len - 1; };
     const auto lo_of = [&](uint32_t r) {
@@ -335,10 +344,11 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
     // The queries' elements are on their way before the keys'.  Channels of the lane's operand k: two operands' lie in one 16-byte piece of
     // a key's row.
     Eight q[NK];
+    const uint32_t q_row = live ? row : last_row;
 #pragma unroll
     for (int k = 0; k < NK; k++) {
         const uint32_t d = (k | 1) < NK ? (uint32_t)(k & ~1) * 32 + g * 16 + (uint32_t)(k & 1) * 8 : (uint32_t)k * 32 + g * 8;
-        q[k] = load8(A.q, A.q_type, (size_t)(sh.row + (live ? tok : A.group.of(last_row))) * A.q_stride + (size_t)(kvh * group + A.group.rest(live ? row : last_row)) * D + d);
+        q[k] = load8(A.q, A.q_type, (size_t)(sh.row + A.group.of(q_row)) * A.q_stride + (size_t)(kvh * group + A.group.rest(q_row)) * D + d);
     }
     __builtin_amdgcn_sched_barrier(0);
     if (step < end) {
@@ -404,7 +414,7 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
         const bool plain = key0 >= all_lo && key0 + (int32_t)kStep - 1 <= all_hi && __ballot(hole) == 0;
         if constexpr (CAP) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) S[i / 4][i % 4] = capped(A, S[i / 4][i % 4], a, e);
+            for (int i = 0; i < 16; i++) S[i / 4][i % 4] = capped<true>(A, S[i / 4][i % 4], a, e);
             a = 1.f, e = 0.f;
         }
         if (!plain) {
@@ -435,14 +445,14 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
         const float shift = e - M + weight_bias(PAIRS);
         bool far = false;
         if constexpr (!PAIRS) {  // (a row's weights lie in all four groups' lanes)
-            int low = 0x7FFFFFFF;
+            int least = 0x7FFFFFFF;
 #pragma unroll
             for (int grp = 0; grp < 4; grp++) {
                 const int of_group = __builtin_amdgcn_readlane(hole ? 0x7FFFFFFF : ev, 16 * grp);
-                low = min(low, of_group);
+                least = min(least, of_group);
                 e_top = max(e_top, of_group == 0x7FFFFFFF ? e_top : of_group);
             }
-            far = low < e_top - kFar;
+            far = least < e_top - kFar;
         }
         float far_sum = 0.f;
         if (far) {
@@ -531,10 +541,9 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
 //
 // 128 query rows a workgroup as the columns of matrix instructions; a turn's codes (64 keys) are converted to f16 once and lie in LDS, two
 // turns' worth, rows padded by 16 bytes (an odd number of 16-byte pieces: consecutive rows in other banks).
-//   Wide: four wavefronts of 32 rows, v_mfma_f32_32x32x16_f16.  An operand read from LDS feeds 32 columns; above 128 channels the
-//     registers leave one wavefront a SIMD.
+//   Wide: four wavefronts of 32 rows, v_mfma_f32_32x32x16_f16.  An operand read from LDS feeds 32 columns.
 //   Narrow: eight wavefronts of 16 rows, v_mfma_f32_16x16x32_f16, two a SIMD at every head_dim, for twice the reads from LDS: where f16
-//     pairs double the multiplications anyway, above 128 channels.
+//     pairs double the multiplications anyway, and above 128 channels, where the wide shape's registers leave one.
 // The order of the keys in S^T's rows is free: they are laid out so that a lane holds the weights of 8 consecutive keys for each k step
 // of the second product, within one group of 16 keys, so a block's scales are the same for all of them.
 template <bool NARROW> struct Shape;
@@ -572,8 +581,9 @@ __device__ __forceinline__ void reads_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x8, 4 * PER, 0);
 }
 
-template <int NK, bool PAIRS, bool CAP>
-__global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, NK > 4 && !tiles_narrow(NK, PAIRS) ? 1 : 2)
+enum Cap { CAP_NONE, CAP_LOW, CAP_ANY };  // no cap, up to kLowCap, above
+template <int NK, bool PAIRS, Cap CAP>
+__global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, 2)
     attention_tiles_kernel(AttentionArgs A, Plan P, Partials part) {
     typedef Shape<tiles_narrow(NK, PAIRS)> Sh;
     constexpr uint32_t D = NK * 32, kKeys = kStep, kThreads = Sh::kWaves * 64, kKeyPad = D + 8, kValPad = kKeys + 8;
@@ -608,7 +618,7 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
             q[k] = {};
             if (live) q[k] = load8(A.q, A.q_type, (size_t)(sh.row + tok) * A.q_stride + (size_t)head * D + (uint32_t)k * Sh::kStepDims + hi * 8);
         }
-        const QueryScale f = query_scale<KD, CAP, tiles_narrow(NK, PAIRS)>(A, q);
+        const QueryScale f = query_scale<KD, CAP != CAP_NONE, tiles_narrow(NK, PAIRS)>(A, q);
         factor = f.factor;
 #pragma unroll
         for (int k = 0; k < KD; k++) query_f16<PAIRS>(q[k], f.mul, qh[k], ql[PAIRS ? k : 0]);
@@ -749,11 +759,11 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, N
         }
 #define LARQL_X(c, j) S[Sh::tile(c, j)][Sh::reg(c, j)]
         const bool whole = key0 >= all_lo && key0 + (int32_t)kKeys - 1 <= all_hi;
-        if constexpr (CAP) {
+        if constexpr (CAP != CAP_NONE) {
 #pragma unroll
             for (int c = 0; c < KC; c++) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) LARQL_X(c, j) = capped(A, LARQL_X(c, j), a[c], e[c]);
+                for (int j = 0; j < 8; j++) LARQL_X(c, j) = capped<CAP == CAP_ANY>(A, LARQL_X(c, j), a[c], e[c]);
                 a[c] = 1.f, e[c] = 0.f;
             }
         }
@@ -955,17 +965,19 @@ int attention_launches(const AttentionArgs &A) {
 
 template <int NK>
 static void launch_dim(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, bool tiles) {
-    const bool pairs = A.out_type == ELEM_F32, cap = A.softcap > 0.f;
+    const bool cap = A.softcap > 0.f;
     const uint32_t items = (uint32_t)Plans::items(A, P);
-#define LARQL_ATTN(PR, C)                                                                                                             \
-    do {                                                                                                                              \
-        if (tiles) hipLaunchKernelGGL((attention_tiles_kernel<NK, PR, C>), dim3(items * A.kv.kv_heads), dim3(Shape<tiles_narrow(NK, PR)>::kWaves * 64), 0, s, A, P, part); \
-        else hipLaunchKernelGGL((attention_rows_kernel<NK, PR, C>), dim3(items, A.kv.kv_heads), dim3(kAttnThreads), 0, s, A, P, part);  \
+#define LARQL_ATTN(PR)                                                                                                                                   \
+    do {                                                                                                                                                 \
+        const dim3 threads(Shape<tiles_narrow(NK, PR)>::kWaves * 64);                                                                                    \
+        if (!tiles && cap) hipLaunchKernelGGL((attention_rows_kernel<NK, PR, true>), dim3(items, A.kv.kv_heads), dim3(kAttnThreads), 0, s, A, P, part);  \
+        else if (!tiles) hipLaunchKernelGGL((attention_rows_kernel<NK, PR, false>), dim3(items, A.kv.kv_heads), dim3(kAttnThreads), 0, s, A, P, part);   \
+        else if (!cap) hipLaunchKernelGGL((attention_tiles_kernel<NK, PR, CAP_NONE>), dim3(items * A.kv.kv_heads), threads, 0, s, A, P, part);           \
+        else if (A.softcap <= kLowCap) hipLaunchKernelGGL((attention_tiles_kernel<NK, PR, CAP_LOW>), dim3(items * A.kv.kv_heads), threads, 0, s, A, P, part); \
+        else hipLaunchKernelGGL((attention_tiles_kernel<NK, PR, CAP_ANY>), dim3(items * A.kv.kv_heads), threads, 0, s, A, P, part);                      \
     } while (0)
-    if (pairs && cap) LARQL_ATTN(true, true);
-    else if (pairs) LARQL_ATTN(true, false);
-    else if (cap) LARQL_ATTN(false, true);
-    else LARQL_ATTN(false, false);
+    if (A.out_type == ELEM_F32) LARQL_ATTN(true);
+    else LARQL_ATTN(false);
 #undef LARQL_ATTN
 }
 

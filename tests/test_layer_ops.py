@@ -519,10 +519,10 @@ def attention_case(be, seqs, kv_heads=2, group=2, head_dim=64, page=16, t="f32",
     want, size, xmax, qk = ref_attention(c, q, scale, causal, window, softcap, sink_values)
     # Scores: sums of products with f16 pairs (2^-22 each, 2^-38 of the row's largest element) or, into 16 bits, one f16 of an f32
     # query (2^-11), and f32 sums; exponent and sums of weights in f32 (an exponent x ln 2 of at most xmax + 60: its rounding, and
-    # that of the cap); weights as f16 pairs or one f16 (2^-11).  A relative error e of the weights moves the result by 2 e size.
+    # that of the cap, which is as small as the scores where it is far above them); weights as f16 pairs or one f16 (2^-11).  A relative error e of the weights moves the result by 2 e size.
     one = out != "f32"
     e = 2.0 ** -20 * abs(scale) * qk + (2.0 ** -11 * abs(scale) * qk if one and t == "f32" else 0.0)
-    e = e + 32 * U * (60 + xmax + 2 * softcap) + (2.0 ** -11 if one else 2.0 ** -21)
+    e = e + 32 * U * (60 + xmax + 2 * np.minimum(softcap, 4 * xmax)) + (2.0 ** -11 if one else 2.0 ** -21)
     bound = (2 * e[..., None] * np.exp(np.minimum(e, 1))[..., None]) * size + HALF[out] * np.abs(want) + TINY[out]
     close(got[: c.tokens], want[: c.tokens], bound[: c.tokens])
     assert (got_bits[c.tokens:] == mark[c.tokens:]).all()
@@ -551,7 +551,7 @@ def test_attention_types_and_heads(be, t, out, kv_heads, group):
 
 @gpu
 @pytest.mark.parametrize("how", [{"window": 1}, {"window": 16}, {"window": 100}, {"causal": False}, {"causal": False, "window": 50},
-                                 {"softcap": 5.0, "q_sigma": 6.0}, {"softcap": 30.0, "window": 33}, {"sinks": [0.0, 3.0, -2.0, 60.0]},
+                                 {"softcap": 5.0, "q_sigma": 6.0}, {"softcap": 30.0, "window": 33}, {"softcap": 1e5}, {"sinks": [0.0, 3.0, -2.0, 60.0]},
                                  {"sinks": [-np.inf, -200.0]}, {"sinks": [1.0], "window": 20}, {"scale": -0.3}, {"scale": 0.0}, {"pad": 8},
                                  {"spoil_tail": True}, {"spoil_tail": True, "window": 40}, {"spoil_tail": True, "causal": False},
                                  {"holes": [(1, 0), (4, 3), (5, 8), (7, 1), (8, 6)]}, {"holes": [(4, j) for j in range(19)]},
