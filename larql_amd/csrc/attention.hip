@@ -51,6 +51,11 @@ struct Plan {
     int fits;                     // how often pieces are made longer to meet the target
 };
 
+// Steps of keys that the window lets a tile see, at most (its tokens may straddle).
+__host__ __device__ __forceinline__ uint64_t window_steps(const AttentionArgs &A, uint32_t tile) {
+    return A.window ? ((uint64_t)A.window + A.group.of(tile) + 1) / kStep + 2 : ~(uint64_t)0;
+}
+
 // A sequence's share of the work: its query rows in tiles, and at most how many steps of keys one of them sees.
 struct Share {
     uint32_t row, n;      // first row of the activations, new tokens
@@ -67,7 +72,7 @@ __device__ __forceinline__ Share share_of(const AttentionArgs &A, const Plan &P,
     const uint32_t rows = t.n * A.group.d;
     h.tiles = rows < P.rows_min || rows > P.rows_max ? 0u : (rows + P.tile - 1) / P.tile;
     h.steps = h.tiles ? ((uint32_t)h.len + kStep - 1) / kStep : 0;
-    if (A.window) h.steps = min((uint64_t)h.steps, ((uint64_t)A.window + A.group.of(P.tile) + 1) / kStep + 2);  // (a tile's tokens may straddle)
+    h.steps = min((uint64_t)h.steps, window_steps(A, P.tile));
     return h;
 }
 
@@ -141,18 +146,23 @@ struct Plans {
 };
 static Plans plans_of(const AttentionArgs &A) {
     const uint64_t group = A.group.d, most = A.kv.max_new * group;
-    const uint64_t steps = (((uint64_t)A.kv.table_width << A.kv.page_shift) + kStep - 1) / kStep;
+    const auto steps_of = [&](uint32_t tile) {
+        return std::min((((uint64_t)A.kv.table_width << A.kv.page_shift) + kStep - 1) / kStep, window_steps(A, tile));
+    };
     const uint32_t cus = 256;
     Plans p;
     // Pieces of few rows: as many as workgroups are resident, 2 a compute unit above 128 channels (131072 keys of 256, us with 1, 2, 3, 4 of
     // them: 148, 103, 125, 110, joining included), 3 below (64 sequences, 64 channels: 44, 37, 33, 37); a wavefront's step each at least.
     p.rows = {kRowsTile, 1, kFewRows, std::max((A.kv.head_dim > 128 ? 2 : 3) * cus / A.kv.kv_heads, 1u), kAttnWaves, 1, 0};
-    p.rows.split = steps > p.rows.min_steps;
+    // Rows so short that the launch of joining costs what it saves stay whole (1000 keys, us whole / split: 32/8 heads of 128 12.8 / 12.6, 16
+    // sequences of them 14.5 / 16.9, 64/8 of 64 9.6 / 10.9; 2000 of the first 17.6 / 12.8; 8/4 heads of 256, f32: 500 keys 13.5 / 15.1, 1000 19.5 /
+    // 15.2).
+    p.rows.split = steps_of(kRowsTile) > (A.kv.head_dim > 128 ? 8u : 16u);
     // Many rows: as many as are resident, unless the tiles by themselves (of which a sequence's last is half full, say) are as many: splitting
     // then is a launch more for nothing (2048 tokens of 32/8 heads of 128: 76 us whole, 88 with it; 16 sequences of 32 tokens, 256 channels,
     // f32: 239 and 165).
     p.tiles = {kTilesTile, kFewRows + 1, 0xFFFFFFFFu, std::max((A.kv.head_dim > 128 ? 1 : 2) * cus / A.kv.kv_heads, 1u), 8, 1, 6};
-    p.tiles.split = steps > p.tiles.min_steps && A.kv.tokens * group / p.tiles.tile + A.kv.sequences / 2 < p.tiles.target;
+    p.tiles.split = steps_of(kTilesTile) > p.tiles.min_steps && A.kv.tokens * group / p.tiles.tile + A.kv.sequences / 2 < p.tiles.target;
     p.use_tiles = most > kFewRows;
     p.use_rows = !p.use_tiles || A.kv.sequences > 1;
     if (!p.use_rows) p.tiles.rows_min = 1;  // one sequence: one kernel, whatever its number of new tokens turns out to be
