@@ -34,11 +34,11 @@ constexpr uint32_t kTilesTile = 128;    // ... for many
 constexpr uint32_t kFewRows = 32;
 constexpr float kLog2E = 1.44269504088896341f;
 // Weights are held as 2^(t + e - M + bias) with t + e - M <= 3; M is whole and only moves where a score leaves that range, so it brings no
-// rounding.  f16 pairs: the bias is small, for the exponent is rounded as a number of its size; a pair keeps 22 bits down to 2^-10 of the
-// largest and 2^-32 of it beyond (131072 equal weights 2^-17 of one that weighs as much as they all: 2^-15 each, at random).  One f16: as
-// large as fits, 11 bits down to 2^-26 of the largest.
-constexpr float kPairsBias = 7.f, kOneBias = 12.f, kSlack = 3.f;
-__device__ __forceinline__ float weight_bias(bool pairs) { return pairs ? kPairsBias : kOneBias; }
+// rounding.  f32 results: the bias is small, for the exponent is rounded as a number of its size; an f16 pair keeps 22 bits down to 2^-10 of the
+// largest and 2^-32 of it beyond (131072 equal weights 2^-17 of one that weighs as much as they all: 2^-15 each, at random).  16-bit results: as
+// large as fits; one f16 keeps 11 bits down to 2^-26 of the largest, 2^-37 of it beyond, a pair the same floor.
+constexpr float kLowBias = 7.f, kHighBias = 12.f, kSlack = 3.f;
+__device__ __forceinline__ float weight_bias(bool f32_result) { return f32_result ? kLowBias : kHighBias; }
 constexpr float kNoMax = -1e30f;
 
 // How one of the two kernels shares its work out.
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
         }
         f16x8_t ph[2], pl[2];
         float sum = 0.f;
-        const float shift = e - M + weight_bias(PAIRS);
+        const float shift = e - M + weight_bias(A.out_type == ELEM_F32);
         bool far = false;
         if constexpr (!PAIRS) {  // (a row's weights lie in all four groups' lanes)
             int least = 0x7FFFFFFF;
@@ -592,7 +592,7 @@ __device__ __forceinline__ void reads_ahead() {
 }
 
 enum Cap { CAP_NONE, CAP_LOW, CAP_ANY };  // no cap, up to kLowCap, above
-template <int NK, bool PAIRS, Cap CAP>
+template <int NK, bool QPAIRS, bool PAIRS, Cap CAP>  // f16 pairs: queries, weights
 __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, 2)
     attention_tiles_kernel(AttentionArgs A, Plan P, Partials part) {
     typedef Shape<tiles_narrow(NK, PAIRS)> Sh;
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, 2
     const int32_t pos = sh.first + (int32_t)tok;
     const int32_t key_hi = !live ? -1 : (A.causal ? min(pos, sh.len - 1) : sh.len - 1);
     const int32_t key_lo = A.window ? (int32_t)max((int64_t)pos - (int64_t)A.window + 1, (int64_t)0) : 0;
-    f16x8_t qh[KD], ql[PAIRS ? KD : 1];
+    f16x8_t qh[KD], ql[QPAIRS ? KD : 1];
     float factor;
     {
         Eight q[KD];
@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, 2
         const QueryScale f = query_scale<KD, CAP != CAP_NONE, tiles_narrow(NK, PAIRS)>(A, q);
         factor = f.factor;
 #pragma unroll
-        for (int k = 0; k < KD; k++) query_f16<PAIRS>(q[k], f.mul, qh[k], ql[PAIRS ? k : 0]);
+        for (int k = 0; k < KD; k++) query_f16<QPAIRS>(q[k], f.mul, qh[k], ql[QPAIRS ? k : 0]);
     }
     // what all and any of the wavefront's rows see (whole rows of lanes: the first and the last live one say it)
     const uint32_t first_row = tile * kTilesTile + wave * Sh::kRows, last_row = min(first_row + Sh::kRows - 1, rows - 1);
@@ -755,10 +755,10 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, 2
             for (int t = 0; t < ST; t++) {
                 const f16x8_t ka = *(const f16x8_t *)&sh_k[buf][t * Sh::kTileKeys + n][k * Sh::kStepDims + hi * 8];
                 S[t] = Sh::mma(ka, qh[k], k ? S[t] : zero);
-                if constexpr (PAIRS) S[t] = Sh::mma(ka, ql[k], S[t]);
+                if constexpr (QPAIRS) S[t] = Sh::mma(ka, ql[k], S[t]);
             }
         }
-        if constexpr (tiles_narrow(NK, PAIRS)) reads_ahead<KD * ST, PAIRS ? 2 : 1>();
+        if constexpr (tiles_narrow(NK, PAIRS)) reads_ahead<KD * ST, QPAIRS ? 2 : 1>();
         // x(c, j): the lane's 8 scores of k step c, keys kStepKeys c + 8 hi + j; their logarithm (base 2) with the value scale: x a + e
         float a[KC], e[KC], unscale[KC];
         const bool far = !PAIRS && __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sh_s[buf][0][3])) != 0;
@@ -973,22 +973,36 @@ int attention_launches(const AttentionArgs &A) {
     return (int)p.use_rows + (int)p.use_tiles + (int)join;
 }
 
+template <int NK, bool PAIRS>
+static void launch_rows(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, uint32_t items) {
+    const dim3 grid(items, A.kv.kv_heads), threads(kAttnThreads);
+    if (A.softcap > 0.f) hipLaunchKernelGGL((attention_rows_kernel<NK, PAIRS, true>), grid, threads, 0, s, A, P, part);
+    else hipLaunchKernelGGL((attention_rows_kernel<NK, PAIRS, false>), grid, threads, 0, s, A, P, part);
+}
+template <int NK, bool QPAIRS, bool PAIRS>
+static void launch_tiles(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, uint32_t items) {
+    const dim3 grid(items * A.kv.kv_heads), threads(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64);
+    if (A.softcap == 0.f) hipLaunchKernelGGL((attention_tiles_kernel<NK, QPAIRS, PAIRS, CAP_NONE>), grid, threads, 0, s, A, P, part);
+    else if (A.softcap <= kLowCap) hipLaunchKernelGGL((attention_tiles_kernel<NK, QPAIRS, PAIRS, CAP_LOW>), grid, threads, 0, s, A, P, part);
+    else hipLaunchKernelGGL((attention_tiles_kernel<NK, QPAIRS, PAIRS, CAP_ANY>), grid, threads, 0, s, A, P, part);
+}
+// One f16 holds a 16-bit query, but 11 of an f32 query's 24 bits, and what a score loses grows with the score: f32 queries enter as f16 pairs
+// whatever the result's type (a causal prompt of 4096 f32 queries, 32/8 heads of 128, into bf16: 242 us for 203; 8/4 of 256 into f16: 195 for 191, and
+// 2.6e-4 from 64 bits for 4.6e-4).  The kernel for few rows, which waits for memory, takes its weights as pairs with them.
 template <int NK>
 static void launch_dim(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, bool tiles) {
-    const bool cap = A.softcap > 0.f;
     const uint32_t items = (uint32_t)Plans::items(A, P);
-#define LARQL_ATTN(PR)                                                                                                                                   \
-    do {                                                                                                                                                 \
-        const dim3 threads(Shape<tiles_narrow(NK, PR)>::kWaves * 64);                                                                                    \
-        if (!tiles && cap) hipLaunchKernelGGL((attention_rows_kernel<NK, PR, true>), dim3(items, A.kv.kv_heads), dim3(kAttnThreads), 0, s, A, P, part);  \
-        else if (!tiles) hipLaunchKernelGGL((attention_rows_kernel<NK, PR, false>), dim3(items, A.kv.kv_heads), dim3(kAttnThreads), 0, s, A, P, part);   \
-        else if (!cap) hipLaunchKernelGGL((attention_tiles_kernel<NK, PR, CAP_NONE>), dim3(items * A.kv.kv_heads), threads, 0, s, A, P, part);           \
-        else if (A.softcap <= kLowCap) hipLaunchKernelGGL((attention_tiles_kernel<NK, PR, CAP_LOW>), dim3(items * A.kv.kv_heads), threads, 0, s, A, P, part); \
-        else hipLaunchKernelGGL((attention_tiles_kernel<NK, PR, CAP_ANY>), dim3(items * A.kv.kv_heads), threads, 0, s, A, P, part);                      \
-    } while (0)
-    if (A.out_type == ELEM_F32) LARQL_ATTN(true);
-    else LARQL_ATTN(false);
-#undef LARQL_ATTN
+    const bool f32_query = A.q_type == ELEM_F32, f32_result = A.out_type == ELEM_F32;
+    if (!tiles) {
+        if (f32_result || f32_query) launch_rows<NK, true>(s, A, P, part, items);
+        else launch_rows<NK, false>(s, A, P, part, items);
+    } else if (f32_result) {
+        launch_tiles<NK, true, true>(s, A, P, part, items);
+    } else if (f32_query) {
+        launch_tiles<NK, true, false>(s, A, P, part, items);
+    } else {
+        launch_tiles<NK, false, false>(s, A, P, part, items);
+    }
 }
 
 static hipError_t launch_plan(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, bool tiles) {

@@ -1,0 +1,48 @@
+"""The layer operators at the ends of what their documentation allows: precision where the plain bounds of test_layer_ops.py are
+wide, batches whose rows do not fit, launches of more workgroups than one grid dimension takes, recording."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import larql_amd as hip
+from larql_amd import _lib as L
+from test_layer_ops import FMT, HALF, ITEM, TINY, U, Cache, Dev, Layer, _call, _sound, close, e4m3, exponent, raw, ref_attention, values
+
+gpu = pytest.mark.gpu
+
+
+def attention(be, c, q, t, out, scale, causal=True, window=0, softcap=0.0):
+    """The results of queries q [tokens, heads, d] (values of type t) over the cache c."""
+    d = Dev(be)
+    rows, width = q.shape[0], q.shape[1] * q.shape[2]
+    cache, batch = c.upload(be)
+    p_out = d.put(np.zeros((rows, width), np.int32 if out == "f32" else np.int16))
+    args = hip.Attention(q=d.put(raw(q.reshape(rows, width), t)[0]), q_stride=width, q_format=FMT[t], out=p_out, out_stride=width, out_format=FMT[out],
+                         q_heads=q.shape[1], causal=int(causal), window=window, scale=scale, softcap=softcap)
+    n = be.attention_workspace_bytes(cache, batch, args)
+    assert be.dev_attention(cache, batch, args, be.malloc(n), n), be.last_error()
+    be.synchronize()
+    return values(be.d2h(p_out, (rows, width), np.int32 if out == "f32" else np.int16), out).reshape(q.shape)
+
+
+# ---- attention: precision ------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("head_dim", [64, 96, 256])
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("out", ["bf16", "f16"])
+def test_f32_queries_keep_their_bits_whatever_the_result(be, new, out, head_dim):
+    """Queries whose products with the keys are large and cancel: what is lost of a query's elements is large beside the scores."""
+    rng = np.random.default_rng(head_dim + new)
+    c = Cache(rng, [(new, 24)], 1, head_dim, 16, sigma=1.0)
+    keys, _, _ = c.keys_values(0, 24)
+    basis = np.linalg.qr(keys[0].T)[0]
+    q = rng.standard_normal((new, 1, head_dim)) * 50
+    q = (q - q @ basis @ basis.T + rng.standard_normal((new, 1, head_dim)) * 0.2).astype(np.float32)
+    got = attention(be, c, q, "f32", out, 1.0, causal=False)
+    want, size, xmax, qk = ref_attention(c, q.astype(np.float64), 1.0, False, 0, 0.0, None)
+    # queries as f16 pairs: 2^-22 of an element; f32 sums of at most 256 products: their roundings, 8 of them at a time and the parts, 2^-20 of the
+    # sum of |q k|; exponents of at most 60 + |x|; one f16 of a weight: 2^-11
+    e = 2.0 ** -20 * qk + 32 * U * (60 + xmax) + 2.0 ** -11
+    close(got, want, 2 * e[..., None] * size + HALF[out] * np.abs(want) + TINY[out])
