@@ -192,7 +192,7 @@ __device__ __forceinline__ void weights_f16(f32x2_t p, f16x8_t &h, f16x8_t &l, i
 }
 
 // Weights of one f16 are summed as they enter the matrix instructions, so that a rounding moves numerator and sum alike, unless the value
-// scale of one of the wavefront's blocks is so far (kFar) below the largest met that its weights may be nothing in f16 and still count: those are
+// scale of one of the turn's blocks is so far (kFar) below the largest met that its weights may be nothing in f16 and still count: those are
 // summed in f32.
 constexpr int kFar = 8;
 __device__ __forceinline__ float weights_sum(const f16x8_t &h) {
@@ -280,12 +280,14 @@ __device__ __forceinline__ void query_f16(const Eight &q, float mul, f16x8_t &h,
 // from, 64 x head_dim bytes of K and then of V through ONE set of registers: as a part of the keys is multiplied its registers take a part
 // of the step's values, and as that is multiplied a part of the next step's keys, so about 64 x head_dim bytes are always in flight and
 // two wavefronts fit a SIMD above 128 channels and three below.  The queries' operands are read from LDS.
-template <int NK, bool PAIRS, bool CAP>
+// Queries and weights are f16 pairs for every result: memory, not the matrix instructions, is waited for (one token of 131072 keys of 16/8 heads of
+// 128 into bf16, 52 us in pairs, 58 as one f16; 64 sequences of 64/8 heads of 64: 34.6, 33.3, of 500 keys each: 12, 11).
+template <int NK, bool CAP>
 __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_kernel(AttentionArgs A, Plan P, Partials part) {
     constexpr uint32_t D = NK * 32, kPad = D + 4;
     constexpr int NP = (NK + 1) / 2;  // parts: 64 channels of the keys, 64 channels of the values
     struct Queries {
-        f16x8_t q[PAIRS ? 2 : 1][NK][64];
+        f16x8_t q[2][NK][64];
         float factor[16];
     };
     struct Sums {
@@ -376,9 +378,9 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
     for (int k = 0; k < NK; k++)
         if ((uint32_t)k % kAttnWaves == wave) {
             f16x8_t h, l;
-            query_f16<PAIRS>(q[k], f.mul, h, l);
+            query_f16<true>(q[k], f.mul, h, l);
             sq.q[0][k][lane] = h;
-            if constexpr (PAIRS) sq.q[PAIRS ? 1 : 0][k][lane] = l;
+            sq.q[1][k][lane] = l;
         }
     __syncthreads();
     const float factor = sq.factor[n];
@@ -387,25 +389,24 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
 #pragma unroll
     for (int i = 0; i < 2 * NK; i++) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float M = kNoMax, L = 0.f;
-    int e_top = -1000;  // the largest logarithm of a value scale met
     for (; step < end; step += kAttnWaves) {
         const int32_t key0 = (int32_t)(step * kStep);
         const bool hole = page_v == ~0u;
         const uint8_t *vp = v_head + (uint64_t)(hole ? 0u : page_v) * page_bytes + ((n << kv.page_shift) + (((uint32_t)key0 + g * 16) & page_mask));
-        f32x4_t S[4], odd[PAIRS ? 4 : 1] = {}, low[PAIRS ? 4 : 1] = {};  // (pairs: three sums, each of a third of the roundings)
+        f32x4_t S[4], odd[4] = {}, low[4] = {};  // (three sums, each of a third of the roundings)
 #pragma unroll
         for (int p = 0; p < NP; p++) {
 #pragma unroll
             for (int k = 2 * p; k < (2 * p + 2 < NK ? 2 * p + 2 : NK); k++) {
-                const f16x8_t qh = sq.q[0][k][lane], ql = sq.q[PAIRS ? 1 : 0][k][lane];
+                const f16x8_t qh = sq.q[0][k][lane], ql = sq.q[1][k][lane];
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
                     const u32x4_t c = ring[p][t];
                     const f16x8_t ka = codes_f16(k % 2 ? u32x2_t{c[2], c[3]} : u32x2_t{c[0], c[1]});
                     const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-                    f32x4_t &sum = PAIRS && k % 2 ? odd[t] : S[t];
-                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh, k < (PAIRS ? 2 : 1) ? zero : sum, 0, 0, 0);
-                    if constexpr (PAIRS) low[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql, k ? low[t] : zero, 0, 0, 0);
+                    f32x4_t &sum = k % 2 ? odd[t] : S[t];
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh, k < 2 ? zero : sum, 0, 0, 0);
+                    low[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql, k ? low[t] : zero, 0, 0, 0);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -413,9 +414,8 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
             for (int d = 4 * p; d < (4 * p + 4 < 2 * NK ? 4 * p + 4 : 2 * NK); d++) ring[p][d % 4] = *(const u32x4_t *)(vp + ((size_t)(16 * d) << kv.page_shift));
             __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (PAIRS)
 #pragma unroll
-            for (int t = 0; t < 4; t++) S[t] += odd[t] + low[t];
+        for (int t = 0; t < 4; t++) S[t] += odd[t] + low[t];
         // Logarithms (base 2) of the weights times the value scale.  A scale that is not a number makes its tokens' scores NaN.
         const bool none = !(vs == vs);
         const int ev = none || hole ? 0 : (int)(__builtin_bit_cast(uint32_t, vs) >> 23 & 0xFFu) - 127;
@@ -453,31 +453,12 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
         f16x8_t ph[2], pl[2];
         float sum = 0.f;
         const float shift = e - M + weight_bias(A.out_type == ELEM_F32);
-        bool far = false;
-        if constexpr (!PAIRS) {  // (a row's weights lie in all four groups' lanes)
-            int least = 0x7FFFFFFF;
-#pragma unroll
-            for (int grp = 0; grp < 4; grp++) {
-                const int of_group = __builtin_amdgcn_readlane(hole ? 0x7FFFFFFF : ev, 16 * grp);
-                least = min(least, of_group);
-                e_top = max(e_top, of_group == 0x7FFFFFFF ? e_top : of_group);
-            }
-            far = least < e_top - kFar;
-        }
-        float far_sum = 0.f;
-        if (far) {
-            float shift_of = shift;
-            asm volatile("" : "+v"(shift_of));  // (exponentials of its own: those below are to mix with the matrix instructions)
-#pragma unroll
-            for (int i = 0; i < 16; i++) far_sum += __builtin_amdgcn_exp2f(fmaf(S[i / 4][i % 4], a, shift_of));
-        }
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
             const f32x2_t p = {__builtin_amdgcn_exp2f(fmaf(S[i / 4][i % 4], a, shift)), __builtin_amdgcn_exp2f(fmaf(S[i / 4][i % 4 + 1], a, shift))};
-            weights_f16<PAIRS>(p, ph[i / 8], pl[i / 8], i % 8);
-            if constexpr (PAIRS) sum += p[0] + p[1];
+            weights_f16<true>(p, ph[i / 8], pl[i / 8], i % 8);
+            sum += p[0] + p[1];
         }
-        if constexpr (!PAIRS) sum = far ? far_sum : weights_sum(ph[0]) + weights_sum(ph[1]);
         L = fmaf(sum, unscale, L);
         if (!plain) {  // bytes behind the last key may be anything
             const int32_t have = hole ? 0 : sh.len - key0 - (int32_t)g * 16;
@@ -505,7 +486,7 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
                     const u32x4_t c = ring[p][d % 4];
                     const f16x8_t va = codes_f16(u32x2_t{c[2 * u], c[2 * u + 1]});
                     acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[u], acc[d], 0, 0, 0);
-                    if constexpr (PAIRS) acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[u], acc[d], 0, 0, 0);
+                    acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[u], acc[d], 0, 0, 0);
                 }
             __builtin_amdgcn_sched_barrier(0);
             if (more) load_keys(kp, p);
@@ -973,11 +954,11 @@ int attention_launches(const AttentionArgs &A) {
     return (int)p.use_rows + (int)p.use_tiles + (int)join;
 }
 
-template <int NK, bool PAIRS>
+template <int NK>
 static void launch_rows(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, uint32_t items) {
     const dim3 grid(items, A.kv.kv_heads), threads(kAttnThreads);
-    if (A.softcap > 0.f) hipLaunchKernelGGL((attention_rows_kernel<NK, PAIRS, true>), grid, threads, 0, s, A, P, part);
-    else hipLaunchKernelGGL((attention_rows_kernel<NK, PAIRS, false>), grid, threads, 0, s, A, P, part);
+    if (A.softcap > 0.f) hipLaunchKernelGGL((attention_rows_kernel<NK, true>), grid, threads, 0, s, A, P, part);
+    else hipLaunchKernelGGL((attention_rows_kernel<NK, false>), grid, threads, 0, s, A, P, part);
 }
 template <int NK, bool QPAIRS, bool PAIRS>
 static void launch_tiles(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, uint32_t items) {
@@ -988,14 +969,13 @@ static void launch_tiles(hipStream_t s, const AttentionArgs &A, const Plan &P, c
 }
 // One f16 holds a 16-bit query, but 11 of an f32 query's 24 bits, and what a score loses grows with the score: f32 queries enter as f16 pairs
 // whatever the result's type (a causal prompt of 4096 f32 queries, 32/8 heads of 128, into bf16: 242 us for 203; 8/4 of 256 into f16: 195 for 191, and
-// 2.6e-4 from 64 bits for 4.6e-4).  The kernel for few rows, which waits for memory, takes its weights as pairs with them.
+// 2.6e-4 from 64 bits for 4.6e-4).
 template <int NK>
 static void launch_dim(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, bool tiles) {
     const uint32_t items = (uint32_t)Plans::items(A, P);
     const bool f32_query = A.q_type == ELEM_F32, f32_result = A.out_type == ELEM_F32;
     if (!tiles) {
-        if (f32_result || f32_query) launch_rows<NK, true>(s, A, P, part, items);
-        else launch_rows<NK, false>(s, A, P, part, items);
+        launch_rows<NK>(s, A, P, part, items);
     } else if (f32_result) {
         launch_tiles<NK, true, true>(s, A, P, part, items);
     } else if (f32_query) {

@@ -46,3 +46,31 @@ def test_f32_queries_keep_their_bits_whatever_the_result(be, new, out, head_dim)
     # sum of |q k|; exponents of at most 60 + |x|; one f16 of a weight: 2^-11
     e = 2.0 ** -20 * qk + 32 * U * (60 + xmax) + 2.0 ** -11
     close(got, want, 2 * e[..., None] * size + HALF[out] * np.abs(want) + TINY[out])
+
+
+def two_keys(be, many, t, out, xmax, softcap=0.0, head_dim=32):
+    """Every query sees two keys, with one channel in the product and values +1 and -1: a result is the difference of its two weights, so
+    what the weights are off by is not lost among larger errors.  Results, the definition's."""
+    rng = np.random.default_rng(7)
+    seqs = [(200, 200)] if many else [(1, 2 + 5 * i) for i in range(60)]
+    c = Cache(rng, seqs, 2, head_dim, 16)
+    for a in (c.k, c.v):
+        a[:] = 0
+    c.k[..., 0] = rng.integers(0x30, 0x38, c.k.shape[:-1]) | 0x80 * rng.integers(0, 2, c.k.shape[:-1])  # 0.5 .. 0.94, either sign
+    c.v[..., 0::2], c.v[..., 1::2] = 0x38, 0xB8  # 1, -1
+    c.ks[:], c.vs[:] = 1.0, 1.0
+    q = np.zeros((c.tokens, 4, head_dim))
+    q[..., 0] = rng.uniform(-xmax, xmax, q.shape[:2])
+    q = raw(q, t)[1]
+    want, _, _, _ = ref_attention(c, q, 1.0, True, 2, softcap, None)
+    return attention(be, c, q, t, out, 1.0, window=2, softcap=softcap), want
+
+
+@gpu
+@pytest.mark.parametrize("head_dim", [32, 128, 192])
+@pytest.mark.parametrize("t,out", [("f16", "f16"), ("bf16", "bf16"), ("f32", "f16")])
+def test_few_rows_into_16_bits_lose_nothing_but_the_results_rounding(be, t, out, head_dim):
+    got, want = two_keys(be, False, t, out, 0.004, head_dim=head_dim)
+    # logarithms of |x| < 0.01 (a few u), + 12 rounded at their size (16 u log2, half: 5.5 u), an exponential's last place (2 u), pairs (2 u): 12 u a
+    # weight at most, half the difference of two of them, a few u of sum, quotient and product
+    close(got, want, 32 * U + HALF[out] * np.abs(want) + TINY[out])
