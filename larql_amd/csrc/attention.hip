@@ -216,20 +216,24 @@ __device__ __forceinline__ float inverse_sum(const AttentionArgs &A, float l, fl
 }
 
 // The logarithm (base 2) of a capped score's weight, plus e: cap * tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1), where s a is the
-// exponent of that as a power of two (query_scale).  That is off by what 32 bits leave of the cap,
-// little beside the weights' own rounding for caps up to kLowCap.  SERIES: a score below 0.26 of its cap takes the series of tanh (next term
-// below 2e-8 of it), so that a cap far above the scores costs them nothing.  Many rows take it above kLowCap only (a causal prompt of 8192,
-// 32/8 heads of 128: 1001 us for 866), few rows, which wait for memory, always.
+// exponent of that as a power of two (query_scale).  That is off by what 32 bits leave of the cap: for a cap of 64 up to 2^-17 of a weight, little
+// beside one f16 of it, not beside a pair.  A score below 0.26 of its cap (kSeriesBelow) can take the series of tanh (next term below 2e-8 of it), so
+// that a cap above the scores costs them no precision.  Few rows, which wait for memory, compute both; many rows the series alone where a wavefront's
+// scores all allow it, and where weights are one f16 and the cap is at most kLowCap the closed form alone (4096 causal tokens of 32/8 heads
+// of 128, us: f16, closed 230, by the scores 235, both 285; f32 with a cap of 50 378, 386, 439, of 5 371, 434, 434).
 constexpr float kLowCap = 64.f;
-template <bool SERIES>
+enum class CapBy { WHOLE, SERIES, EITHER };
+constexpr float kSeriesBelow = 0.75f;  // of |s a|
+template <CapBy BY>
 __device__ __forceinline__ float capped(const AttentionArgs &A, float s, float a, float e) {
     const float c = A.softcap * kLog2E, z = s * a;
     const float whole = fmaf(-2.f * c, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(z) + 1.f), c + e);
-    if constexpr (!SERIES) return whole;
+    if constexpr (BY == CapBy::WHOLE) return whole;
     constexpr float u2 = 0.120113253f;  // (ln 2 / 2)^2: x / cap = z ln 2 / 2
     const float t = z * z;
-    const float series = fmaf(t, fmaf(t, fmaf(t, fmaf(t, u2 * u2 * u2 * u2 * 62.f / 2835.f, u2 * u2 * u2 * -17.f / 315.f), u2 * u2 * 2.f / 15.f), u2 / -3.f), 1.f);
-    return fabsf(z) < 0.75f ? fmaf(A.softcap * 0.5f * z, series, e) : whole;
+    const float poly = fmaf(t, fmaf(t, fmaf(t, fmaf(t, u2 * u2 * u2 * u2 * 62.f / 2835.f, u2 * u2 * u2 * -17.f / 315.f), u2 * u2 * 2.f / 15.f), u2 / -3.f), 1.f);
+    const float series = fmaf(A.softcap * 0.5f * z, poly, e);
+    return BY == CapBy::SERIES || fabsf(z) < kSeriesBelow ? series : whole;
 }
 // Scores s of a step with hidden keys, whose logarithms are s a + e: a hidden one is -inf, times a factor that is positive; a factor that is
 // not (a scale of 0, a block that is no number) goes into the scores that are seen.
@@ -424,7 +428,7 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
         const bool plain = key0 >= all_lo && key0 + (int32_t)kStep - 1 <= all_hi && __ballot(hole) == 0;
         if constexpr (CAP) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) S[i / 4][i % 4] = capped<true>(A, S[i / 4][i % 4], a, e);
+            for (int i = 0; i < 16; i++) S[i / 4][i % 4] = capped<CapBy::EITHER>(A, S[i / 4][i % 4], a, e);
             a = 1.f, e = 0.f;
         }
         if (!plain) {
@@ -572,7 +576,7 @@ __device__ __forceinline__ void reads_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x8, 4 * PER, 0);
 }
 
-enum Cap { CAP_NONE, CAP_LOW, CAP_ANY };  // no cap, up to kLowCap, above
+enum Cap { CAP_NONE, CAP_LOW, CAP_ANY };  // no cap, one up to kLowCap and weights of one f16, any other
 template <int NK, bool QPAIRS, bool PAIRS, Cap CAP>  // f16 pairs: queries, weights
 __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, 2)
     attention_tiles_kernel(AttentionArgs A, Plan P, Partials part) {
@@ -753,8 +757,17 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, 2
         if constexpr (CAP != CAP_NONE) {
 #pragma unroll
             for (int c = 0; c < KC; c++) {
+                float most = 0.f;
+                if constexpr (CAP == CAP_ANY)
 #pragma unroll
-                for (int j = 0; j < 8; j++) LARQL_X(c, j) = capped<CAP == CAP_ANY>(A, LARQL_X(c, j), a[c], e[c]);
+                    for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(LARQL_X(c, j)));
+                if (CAP == CAP_ANY && __ballot(most * a[c] >= kSeriesBelow) == 0) {  // (the usual case)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) LARQL_X(c, j) = capped<CapBy::SERIES>(A, LARQL_X(c, j), a[c], e[c]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) LARQL_X(c, j) = capped<CAP == CAP_ANY ? CapBy::EITHER : CapBy::WHOLE>(A, LARQL_X(c, j), a[c], e[c]);
+                }
                 a[c] = 1.f, e[c] = 0.f;
             }
         }
@@ -963,9 +976,11 @@ static void launch_rows(hipStream_t s, const AttentionArgs &A, const Plan &P, co
 template <int NK, bool QPAIRS, bool PAIRS>
 static void launch_tiles(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, uint32_t items) {
     const dim3 grid(items * A.kv.kv_heads), threads(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64);
-    if (A.softcap == 0.f) hipLaunchKernelGGL((attention_tiles_kernel<NK, QPAIRS, PAIRS, CAP_NONE>), grid, threads, 0, s, A, P, part);
-    else if (A.softcap <= kLowCap) hipLaunchKernelGGL((attention_tiles_kernel<NK, QPAIRS, PAIRS, CAP_LOW>), grid, threads, 0, s, A, P, part);
-    else hipLaunchKernelGGL((attention_tiles_kernel<NK, QPAIRS, PAIRS, CAP_ANY>), grid, threads, 0, s, A, P, part);
+    const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, threads, 0, s, A, P, part); };
+    if (A.softcap == 0.f) return launch(attention_tiles_kernel<NK, QPAIRS, PAIRS, CAP_NONE>);
+    if constexpr (!PAIRS)
+        if (A.softcap <= kLowCap) return launch(attention_tiles_kernel<NK, QPAIRS, PAIRS, CAP_LOW>);
+    launch(attention_tiles_kernel<NK, QPAIRS, PAIRS, CAP_ANY>);
 }
 // One f16 holds a 16-bit query, but 11 of an f32 query's 24 bits, and what a score loses grows with the score: f32 queries enter as f16 pairs
 // whatever the result's type (a causal prompt of 4096 f32 queries, 32/8 heads of 128, into bf16: 242 us for 203; 8/4 of 256 into f16: 195 for 191, and

@@ -74,3 +74,14 @@ def test_few_rows_into_16_bits_lose_nothing_but_the_results_rounding(be, t, out,
     # logarithms of |x| < 0.01 (a few u), + 12 rounded at their size (16 u log2, half: 5.5 u), an exponential's last place (2 u), pairs (2 u): 12 u a
     # weight at most, half the difference of two of them, a few u of sum, quotient and product
     close(got, want, 32 * U + HALF[out] * np.abs(want) + TINY[out])
+
+
+@gpu
+@pytest.mark.parametrize("cap", [1.0, 2.0, 30.0, 64.0, 65.0, 1e4])
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("head_dim", [32, 128, 256])
+def test_a_cap_costs_f32_results_nothing(be, many, cap, head_dim):
+    got, want = two_keys(be, many, "f32", "f32", 0.5, cap, head_dim)
+    # logarithms of |x| <= 0.5: a dozen roundings of them at most (6 u); + 7 rounded at its size (half of 8 u log2: 2.8 u); an exponential's last
+    # place (2 u), pairs (2 u): 13 u a weight, half the difference of two of them, a few u of sum, quotient and product
+    close(got, want, 24 * U + 8 * U * np.abs(want))
