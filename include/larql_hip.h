@@ -575,7 +575,8 @@ typedef struct {
  * tokens of sequence s with the new ones; its new tokens are rows q_start[s] .. q_start[s+1] of the activations and the last
  * ones of the sequence.  block_table[s] lists its pages; an entry outside [0, num_pages) is a hole: nothing is written
  * there, and its tokens are masked.  A sequence whose rows do not fit (q_start falling, beyond `tokens`, or more than
- * max_new_tokens of them) is left out, its rows untouched.  Up to 2^16 sequences, 2^24 new tokens and tables of 2^30 tokens
+ * max_new_tokens of them) is left out, its rows untouched, and the others are served.  No row belongs to two sequences (else
+ * some of their work is left undone).  Up to 2^16 sequences, 2^24 new tokens and tables of 2^30 tokens
  * (more: LARQL_UNSUPPORTED). */
 typedef struct {
     const int32_t *kv_len;         /* [sequences] */

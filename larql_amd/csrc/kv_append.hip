@@ -120,17 +120,22 @@ __device__ __forceinline__ bool find_page(const KvArgs &kv, uint32_t item, uint3
     return false;
 }
 
-// The sequence that row `token` belongs to.
+// The sequence that row `token` belongs to: whichever holds it (row starts may fall between sequences: the one between is left out).
 __device__ __forceinline__ bool find_token(const KvArgs &kv, uint32_t token, NewTokens &t) {
     const uint32_t lane = threadIdx.x % 64;
-    uint32_t s = 0;
     for (uint32_t base = 0; base < kv.sequences; base += 64) {
-        const bool before = base + lane < kv.sequences && kv.q_start[base + lane + 1] <= (int32_t)token;
-        s += (uint32_t)__popcll(__ballot(before));
+        NewTokens of = {};
+        if (base + lane < kv.sequences) of = new_tokens(kv, base + lane);
+        const uint64_t holds = __ballot(token - of.row < of.n);  // (a row before the first wraps round)
+        if (holds) {
+            const int at = (int)__builtin_ctzll(holds);
+            t.row = (uint32_t)__builtin_amdgcn_readlane((int)of.row, at);
+            t.n = (uint32_t)__builtin_amdgcn_readlane((int)of.n, at);
+            t.len = __builtin_amdgcn_readlane(of.len, at);
+            return true;
+        }
     }
-    if (s >= kv.sequences) return false;
-    t = new_tokens(kv, s);
-    return token >= t.row && token - t.row < t.n;
+    return false;
 }
 
 // A page's scale with its new elements: the exponent, and whether it is a number.  amax: the largest new |x| as bits (a NaN or an

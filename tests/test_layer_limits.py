@@ -7,7 +7,8 @@ import pytest
 
 import larql_amd as hip
 from larql_amd import _lib as L
-from test_layer_ops import FMT, HALF, ITEM, TINY, U, Cache, Dev, Layer, _call, _sound, close, e4m3, exponent, raw, ref_attention, values
+from test_layer_ops import (FMT, HALF, ITEM, TINY, U, Cache, Dev, Layer, _call, _sound, append_case, attention_case, close, e4m3, exponent, raw,
+                            ref_attention, values)
 
 gpu = pytest.mark.gpu
 
@@ -85,3 +86,47 @@ def test_a_cap_costs_f32_results_nothing(be, many, cap, head_dim):
     # logarithms of |x| <= 0.5: a dozen roundings of them at most (6 u); + 7 rounded at its size (half of 8 u log2: 2.8 u); an exponential's last
     # place (2 u), pairs (2 u): 13 u a weight, half the difference of two of them, a few u of sum, quotient and product
     close(got, want, 24 * U + 8 * U * np.abs(want))
+
+
+# ---- batches in which some sequences' rows do not fit ---------------------------------------------------------------
+
+# q_start, rows, max_new_tokens, and (new tokens, length) of the sequences, no new tokens for those that are left out
+UNEVEN = [([4, 6, 0, 2], 6, 2, [(2, 20), (0, 18), (2, 5)]),            # the second falls
+          ([0, 2, 1, 8], 7, 3, [(2, 20), (0, 18), (0, 5)]),            # ... and the third has more than max_new_tokens
+          ([0, 2, 1, 1], 7, 3, [(2, 20), (0, 18), (0, 5)]),
+          ([5, 7, 4, 5, 0, 4], 7, 4, [(2, 33), (0, 9), (1, 17), (0, 40), (4, 4)]),
+          ([-2, 0, 3, 9], 7, 3, [(0, 20), (3, 18), (0, 5)]),           # below 0, beyond the rows
+          ([3, 4, 0, 1, 3], 4, 1, [(1, 20), (0, 18), (1, 5), (0, 16)])]  # one token each: the kernel for that
+
+
+@gpu
+@pytest.mark.parametrize("starts,rows,most,seqs", UNEVEN)
+@pytest.mark.parametrize("page", [16, 64])
+def test_append_serves_the_sequences_whose_rows_fit(be, starts, rows, most, seqs, page):
+    c = Cache(np.random.default_rng(page), seqs, 2, 64, page)
+    c.q_start, c.tokens, c.max_new = np.array(starts, np.int32), rows, most
+    append_case(be, seqs, cache=c, page=page, norm=True)
+
+
+@gpu
+@pytest.mark.parametrize("many", [False, True])
+def test_attention_serves_the_sequences_whose_rows_fit(be, many):
+    n = 70 if many else 2
+    seqs = [(n, 100), (0, 18), (n, 90)]
+    c = Cache(np.random.default_rng(1), seqs, 2, 64, 16)
+    c.q_start, c.tokens, c.max_new = np.array([n, 2 * n, 0, n], np.int32), 2 * n, n
+    attention_case(be, seqs, cache=c)
+
+
+@gpu
+def test_queries_find_their_sequence_among_many(be):
+    seqs = [(0 if i % 5 == 2 else 1 + i % 3, 9 + i) for i in range(300)]
+    c = Cache(np.random.default_rng(2), seqs, 1, 32, 16)
+    at = np.cumsum([0] + [n for n, _ in seqs[::-1]]).astype(np.int32)  # the rows of later sequences first: every other start falls
+    starts, served = [], []
+    for (n, length), a in zip(seqs, at[:-1][::-1]):
+        starts += [a, a + n]  # a sequence, and one between its end and the next one's start that falls or is empty
+        served += [(n, length), (0, 7)]
+    c = Cache(np.random.default_rng(2), served[:-1], 1, 32, 16)
+    c.q_start, c.tokens, c.max_new = np.array(starts, np.int32), int(at[-1]), 3
+    append_case(be, served[:-1], cache=c, kv_heads=1, head_dim=32)
