@@ -536,7 +536,7 @@ int  larql_hip_dev_moe_layer_forward(larql_hip_ctx *ctx, larql_hip_moe_layer *la
  * ones: norm_offset does not enter).  gate is f32 [hidden] for all rows (gate_stride 0) or one row for each.  n is taken
  * from h' before h' is rounded to its format.  residual_out may be residual, and normed may be block (of the same element
  * size and stride, else LARQL_REFUSED_SHAPE); no other overlap.
- * Strides are elements between rows, at least hidden.  hidden <= 32768 (else LARQL_UNSUPPORTED). */
+ * Strides are elements between rows, at least hidden.  hidden <= 32768, rows < 2^31 (else LARQL_UNSUPPORTED). */
 typedef struct {
     size_t rows, hidden;
     const void *block;
@@ -576,8 +576,8 @@ typedef struct {
  * ones of the sequence.  block_table[s] lists its pages; an entry outside [0, num_pages) is a hole: nothing is written
  * there, and its tokens are masked.  A sequence whose rows do not fit (q_start falling, beyond `tokens`, or more than
  * max_new_tokens of them) is left out, its rows untouched, and the others are served.  No row belongs to two sequences (else
- * some of their work is left undone).  Up to 2^16 sequences, 2^24 new tokens and tables of 2^30 tokens
- * (more: LARQL_UNSUPPORTED). */
+ * some of their work is left undone).  Up to 2^16 sequences, 2^24 new tokens and tables of 2^30 tokens; and less than 2^31 workgroups a
+ * launch: pages of the new tokens times 2 kv_heads, or 128 query rows times kv_heads, about (more: LARQL_UNSUPPORTED). */
 typedef struct {
     const int32_t *kv_len;         /* [sequences] */
     const int32_t *block_table;    /* [sequences, table_width] */

@@ -2566,7 +2566,8 @@ static int check_residual_norm(larql_hip_ctx *c, const larql_hip_residual_norm *
     if (!a) return LARQL_E_ARG;
     memset(&A, 0, sizeof A);
     if (a->rows == 0 || a->hidden == 0) return LARQL_OK;
-    if (a->hidden > kNormMaxHidden || a->rows > 0x7FFFFFFFull) return fail(c, LARQL_UNSUPPORTED, "residual_norm: hidden above 32768");
+    if (a->hidden > kNormMaxHidden) return fail(c, LARQL_UNSUPPORTED, "residual_norm: hidden above 32768");
+    if (a->rows > kMaxBlocks) return fail(c, LARQL_UNSUPPORTED, "residual_norm: more than 2^31 - 1 rows");
     A.residual_type = elem_type(a->residual_format);
     A.block_type = a->block ? elem_type(a->block_format) : ELEM_F32;
     A.normed_type = a->normed ? elem_type(a->normed_format) : ELEM_F32;
@@ -2661,6 +2662,7 @@ static int check_kv_append(larql_hip_ctx *c, const larql_hip_kv_cache *k, const 
     A.inv_freq = a->inv_freq; A.q_norm = a->q_norm; A.k_norm = a->k_norm;
     A.q_heads = (uint32_t)a->q_heads; A.rot_dim = (uint32_t)a->rot_dim; A.interleaved = a->interleaved != 0;
     A.rope_scale = a->rope_scale; A.norm_offset = a->norm_offset; A.norm_eps = a->norm_eps;
+    if (kv_append_blocks(A) > kMaxBlocks) return fail(c, LARQL_UNSUPPORTED, "kv_append: too many pages for one launch");
     return LARQL_OK;
 }
 
@@ -2686,6 +2688,7 @@ static int check_attention(larql_hip_ctx *c, const larql_hip_kv_cache *k, const 
     A.q_heads = (uint32_t)a->q_heads; A.window = (uint32_t)a->window; A.causal = a->causal != 0;
     A.group = Divisor::by(A.q_heads / A.kv.kv_heads);
     A.scale = a->scale; A.softcap = a->softcap;
+    if (attention_blocks(A) > kMaxBlocks) return fail(c, LARQL_UNSUPPORTED, "attention: too many query rows for one launch");
     return LARQL_OK;
 }
 

@@ -592,10 +592,10 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, 2
     __shared__ float sh_s[2][G][4];  // of each group of 16 keys: key scale, log2 of the value scale, one over it, and whether the turn has a far one
     const KvArgs &kv = A.kv;
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = lane % Sh::kRows, hi = lane / Sh::kRows;  // column; part of a k step
-    const uint32_t kvh = blockIdx.x % kv.kv_heads, group = A.group.d;  // (neighbours: the heads, one for each XCD's cache)
+    const uint32_t block = block_number(), kvh = block % kv.kv_heads, group = A.group.d;  // (neighbours: the heads, one for each XCD's cache)
     Item it;
     Share sh;
-    if (!find_item(A, P, blockIdx.x / kv.kv_heads, false, it, sh)) return;
+    if (!find_item(A, P, block / kv.kv_heads, false, it, sh)) return;
     const uint32_t rows = sh.n * group;
     const uint32_t tile = sh.tiles - 1 - it.tile;  // (the last rows see the most keys: first)
 
@@ -957,6 +957,10 @@ static Partials partials_of(const AttentionArgs &A, const Plan &P, float *at, fl
 }
 static size_t partial_floats(const AttentionArgs &A, const Plan &P) { return Plans::slots(P) * A.kv.kv_heads * P.tile * (size_t)(A.kv.head_dim + 2); }
 
+uint64_t attention_blocks(const AttentionArgs &A) {
+    const Plans p = plans_of(A);
+    return std::max(p.use_rows ? Plans::items(A, p.rows) : 0, p.use_tiles ? Plans::items(A, p.tiles) : 0) * A.kv.kv_heads;
+}
 size_t attention_workspace_bytes(const AttentionArgs &A) {
     const Plans p = plans_of(A);
     return ((p.use_rows ? partial_floats(A, p.rows) : 0) + (p.use_tiles ? partial_floats(A, p.tiles) : 0)) * sizeof(float) + 16;
@@ -969,13 +973,13 @@ int attention_launches(const AttentionArgs &A) {
 
 template <int NK>
 static void launch_rows(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, uint32_t items) {
-    const dim3 grid(items, A.kv.kv_heads), threads(kAttnThreads);
+    const dim3 grid(items, A.kv.kv_heads), threads(kAttnThreads);  // (at most 2 * 2^16 tiles and the target: far below 2^24)
     if (A.softcap > 0.f) hipLaunchKernelGGL((attention_rows_kernel<NK, true>), grid, threads, 0, s, A, P, part);
     else hipLaunchKernelGGL((attention_rows_kernel<NK, false>), grid, threads, 0, s, A, P, part);
 }
 template <int NK, bool QPAIRS, bool PAIRS>
 static void launch_tiles(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, uint32_t items) {
-    const dim3 grid(items * A.kv.kv_heads), threads(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64);
+    const dim3 grid = grid_of((uint64_t)items * A.kv.kv_heads), threads(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64);
     const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, threads, 0, s, A, P, part); };
     if (A.softcap == 0.f) return launch(attention_tiles_kernel<NK, QPAIRS, PAIRS, CAP_NONE>);
     if constexpr (!PAIRS)
@@ -1001,7 +1005,6 @@ static void launch_dim(hipStream_t s, const AttentionArgs &A, const Plan &P, con
 }
 
 static hipError_t launch_plan(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, bool tiles) {
-    if (Plans::items(A, P) * A.kv.kv_heads > 0x7FFFFFFFull) return hipErrorInvalidValue;
     switch (A.kv.head_dim / 32) {
     case 1: launch_dim<1>(s, A, P, part, tiles); break;
     case 2: launch_dim<2>(s, A, P, part, tiles); break;

@@ -205,8 +205,9 @@ __device__ __forceinline__ void store_key(const KvAppendArgs &A, uint8_t *row, u
 template <uint32_t LPH>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_one_kernel(KvAppendArgs A, uint32_t blocks) {
     const KvArgs &kv = A.kv;
-    const uint32_t s = blockIdx.x / blocks, g = threadIdx.x % LPH;
-    const uint32_t head = (blockIdx.x % blocks) * (kAppendThreads / LPH) + threadIdx.x / LPH;  // keys, values, queries
+    const uint32_t s = block_number() / blocks, g = threadIdx.x % LPH;
+    if (s >= kv.sequences) return;
+    const uint32_t head = (block_number() % blocks) * (kAppendThreads / LPH) + threadIdx.x / LPH;  // keys, values, queries
     const bool is_k = head < kv.kv_heads, is_v = !is_k && head < 2 * kv.kv_heads, is_q = !is_k && !is_v && A.q && head < 2 * kv.kv_heads + A.q_heads;
     const bool in_head = 8 * g < kv.head_dim && (is_k || is_v || is_q), turns = 8 * g < A.rot_dim && !is_v;
     const NewTokens t = new_tokens(kv, s);
@@ -289,8 +290,10 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendArgs 
     const bool in_head = 8 * g0 < kv.head_dim, turns = 8 * g < A.rot_dim;
     Quad w = {};
     f32x4_t freq = {0.f, 0.f, 0.f, 0.f};
-    if (blockIdx.x >= page_blocks) {  // the queries of one token
-        const uint32_t token = blockIdx.x - page_blocks, first = threadIdx.x / LPH;
+    const uint32_t block = block_number();
+    if (block >= page_blocks) {  // the queries of one token
+        const uint32_t token = block - page_blocks, first = threadIdx.x / LPH;
+        if (!A.q || token >= kv.tokens) return;
         const char *src = (const char *)A.q + token * A.q_stride * elem_bytes(A.type);
         char *dst = (char *)A.q_out + token * A.q_out_stride * elem_bytes(A.type);
         const auto load = [&](uint32_t head) { return load_quad(A, src, A.type, min(head, A.q_heads - 1) * kv.head_dim, g); };
@@ -317,10 +320,10 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendArgs 
         }
         return;
     }
-    const uint32_t part_of = blockIdx.x % (2 * kv.kv_heads), head = part_of % kv.kv_heads;
+    const uint32_t part_of = block % (2 * kv.kv_heads), head = part_of % kv.kv_heads;
     const bool is_v = part_of >= kv.kv_heads;
     uint32_t s, j;
-    if (!find_page(kv, blockIdx.x / (2 * kv.kv_heads), s, j)) return;
+    if (!find_page(kv, block / (2 * kv.kv_heads), s, j)) return;
     const uint32_t page = kv_page(kv, kv.block_table + (size_t)s * kv.table_width, j << kv.page_shift);
     if (page == ~0u) return;
     const NewTokens t = new_tokens(kv, s);
@@ -417,9 +420,9 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendArgs 
 }
 
 template <uint32_t LPH>
-static void launch_lanes(hipStream_t s, const KvAppendArgs &A, uint32_t page_blocks, uint32_t grid) {
+static void launch_lanes(hipStream_t s, const KvAppendArgs &A, uint32_t page_blocks, dim3 grid) {
     const uint32_t passes = (1u << A.kv.page_shift) * LPH / kAppendThreads;
-#define LARQL_APPEND(NP) hipLaunchKernelGGL((kv_append_kernel<LPH, NP>), dim3(grid), dim3(kAppendThreads), 0, s, A, page_blocks)
+#define LARQL_APPEND(NP) hipLaunchKernelGGL((kv_append_kernel<LPH, NP>), grid, dim3(kAppendThreads), 0, s, A, page_blocks)
     if (passes <= 1) LARQL_APPEND(1);
     else if (passes <= 2) LARQL_APPEND(2);
     else if (passes <= 4) LARQL_APPEND(4);
@@ -428,30 +431,36 @@ static void launch_lanes(hipStream_t s, const KvAppendArgs &A, uint32_t page_blo
 #undef LARQL_APPEND
 }
 
-hipError_t kv_append_launch(hipStream_t s, const KvAppendArgs &A) {
-    const KvArgs &kv = A.kv;
+// Lanes of a head; one new token a sequence: workgroups of a sequence.
+static uint32_t lanes_of(const KvArgs &kv) { return kv.head_dim <= 32 ? 4 : kv.head_dim <= 64 ? 8 : kv.head_dim <= 128 ? 16 : 32; }
+static uint32_t one_blocks(const KvAppendArgs &A) {
+    return ((2 * A.kv.kv_heads + (A.q ? A.q_heads : 0)) * lanes_of(A.kv) + kAppendThreads - 1) / kAppendThreads;
+}
+// Several: n new tokens touch at most (n + 2 P - 2) / P pages.
+static uint64_t page_blocks_of(const KvArgs &kv) {
     const uint64_t P = 1u << kv.page_shift;
-    // n new tokens touch at most (n + 2 P - 2) / P pages
-    const uint64_t pages = (kv.tokens + kv.sequences * (2 * P - 2)) / P;
-    const uint64_t page_blocks = pages * 2 * kv.kv_heads, grid = page_blocks + (A.q ? kv.tokens : 0);
-    if (grid > 0x7FFFFFFFull) return hipErrorInvalidValue;
-    if (grid == 0) return hipSuccess;
-    const uint32_t groups = kv.head_dim / 8;
-    if (kv.max_new == 1) {
-        const uint32_t lanes = groups <= 4 ? 4 : groups <= 8 ? 8 : groups <= 16 ? 16 : 32;
-        const uint32_t blocks = ((2 * kv.kv_heads + (A.q ? A.q_heads : 0)) * lanes + kAppendThreads - 1) / kAppendThreads;
-        if ((uint64_t)kv.sequences * blocks > 0x7FFFFFFFull) return hipErrorInvalidValue;
-        const dim3 one(kv.sequences * blocks), threads(kAppendThreads);
-        if (lanes == 4) hipLaunchKernelGGL(kv_append_one_kernel<4>, one, threads, 0, s, A, blocks);
-        else if (lanes == 8) hipLaunchKernelGGL(kv_append_one_kernel<8>, one, threads, 0, s, A, blocks);
-        else if (lanes == 16) hipLaunchKernelGGL(kv_append_one_kernel<16>, one, threads, 0, s, A, blocks);
-        else hipLaunchKernelGGL(kv_append_one_kernel<32>, one, threads, 0, s, A, blocks);
+    return (kv.tokens + kv.sequences * (2 * P - 2)) / P * 2 * kv.kv_heads;
+}
+uint64_t kv_append_blocks(const KvAppendArgs &A) {
+    return A.kv.max_new == 1 ? (uint64_t)A.kv.sequences * one_blocks(A) : page_blocks_of(A.kv) + (A.q ? A.kv.tokens : 0);
+}
+
+hipError_t kv_append_launch(hipStream_t s, const KvAppendArgs &A) {
+    const dim3 grid = grid_of(kv_append_blocks(A)), threads(kAppendThreads);
+    const uint32_t lanes = lanes_of(A.kv);
+    if (A.kv.max_new == 1) {
+        const uint32_t blocks = one_blocks(A);
+        if (lanes == 4) hipLaunchKernelGGL(kv_append_one_kernel<4>, grid, threads, 0, s, A, blocks);
+        else if (lanes == 8) hipLaunchKernelGGL(kv_append_one_kernel<8>, grid, threads, 0, s, A, blocks);
+        else if (lanes == 16) hipLaunchKernelGGL(kv_append_one_kernel<16>, grid, threads, 0, s, A, blocks);
+        else hipLaunchKernelGGL(kv_append_one_kernel<32>, grid, threads, 0, s, A, blocks);
         return hipGetLastError();
     }
-    if (groups <= 4) launch_lanes<4>(s, A, (uint32_t)page_blocks, (uint32_t)grid);
-    else if (groups <= 8) launch_lanes<8>(s, A, (uint32_t)page_blocks, (uint32_t)grid);
-    else if (groups <= 16) launch_lanes<16>(s, A, (uint32_t)page_blocks, (uint32_t)grid);
-    else launch_lanes<32>(s, A, (uint32_t)page_blocks, (uint32_t)grid);
+    const uint32_t page_blocks = (uint32_t)page_blocks_of(A.kv);
+    if (lanes == 4) launch_lanes<4>(s, A, page_blocks, grid);
+    else if (lanes == 8) launch_lanes<8>(s, A, page_blocks, grid);
+    else if (lanes == 16) launch_lanes<16>(s, A, page_blocks, grid);
+    else launch_lanes<32>(s, A, page_blocks, grid);
     return hipGetLastError();
 }
 

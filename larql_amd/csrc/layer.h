@@ -8,6 +8,15 @@
 
 namespace larql {
 
+// A launch takes fewer than 2^32 threads in a dimension of its grid: workgroups beyond kGridRow go into a second one, whose last row may have
+// some that are too many.  Their number is below 2^31 (the callers' checks).
+constexpr uint32_t kGridRowShift = 20, kGridRow = 1u << kGridRowShift;
+constexpr uint64_t kMaxBlocks = 0x7FFFFFFFull;
+inline dim3 grid_of(uint64_t blocks) {
+    return blocks <= kGridRow ? dim3((uint32_t)blocks) : dim3(kGridRow, (uint32_t)((blocks + kGridRow - 1) >> kGridRowShift));
+}
+__device__ __forceinline__ uint32_t block_number() { return blockIdx.y << kGridRowShift | blockIdx.x; }
+
 enum ElemType : int32_t { ELEM_F32 = 0, ELEM_BF16 = 1, ELEM_F16 = 2 };
 __host__ __device__ constexpr uint32_t elem_bytes(int t) { return t == ELEM_F32 ? 4u : 2u; }
 
@@ -45,6 +54,7 @@ struct KvAppendArgs {
     float rope_scale, norm_offset, norm_eps;
 };
 constexpr size_t kMaxRowStride = 1u << 22;  // elements between tokens
+uint64_t kv_append_blocks(const KvAppendArgs &A);  // workgroups of a launch
 hipError_t kv_append_launch(hipStream_t s, const KvAppendArgs &A);
 
 // Division by a number that the host knows: (n * mul / 2^32 + n) / 2^shift, exact for every n below 2^31.
@@ -70,6 +80,7 @@ struct AttentionArgs {
     Divisor group;  // query heads of a key/value head
     float scale, softcap;
 };
+uint64_t attention_blocks(const AttentionArgs &A);  // workgroups of its largest launch
 size_t attention_workspace_bytes(const AttentionArgs &A);
 int attention_launches(const AttentionArgs &A);
 hipError_t attention_launch(hipStream_t s, const AttentionArgs &A, void *workspace);

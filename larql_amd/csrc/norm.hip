@@ -31,7 +31,7 @@ template <uint32_t TPR, int NC, bool VEC>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_norm_kernel(NormArgs A) {
     constexpr uint32_t kRows = TPR < 256 ? (TPR == 64 ? 4 : 1) : 1;
     __shared__ float part[2][16];
-    const uint32_t row = blockIdx.x * kRows + threadIdx.x / TPR, t = threadIdx.x % TPR;
+    const uint32_t row = block_number() * kRows + threadIdx.x / TPR, t = threadIdx.x % TPR;
     if (row >= A.rows) return;  // (whole waves, and only where a row is one wave's)
     const char *block = A.block ? (const char *)A.block + row * A.block_stride * elem_bytes(A.block_type) : nullptr;
     const char *res = (const char *)A.residual + row * A.residual_stride * elem_bytes(A.residual_type);
@@ -119,11 +119,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_norm_kernel(No
 template <uint32_t TPR, bool VEC>
 static void launch_rows(hipStream_t s, const NormArgs &A) {
     const uint32_t threads = TPR < 256 ? (TPR == 64 ? 256 : TPR) : TPR, rows = threads / TPR;
-    const uint32_t grid = (A.rows + rows - 1) / rows;
+    const dim3 grid = grid_of((A.rows + rows - 1) / rows);
     const uint32_t chunks = (A.hidden + TPR * 8 - 1) / (TPR * 8);
-    if (chunks <= 1) hipLaunchKernelGGL((residual_norm_kernel<TPR, 1, VEC>), dim3(grid), dim3(threads), 0, s, A);
-    else if (chunks <= 2) hipLaunchKernelGGL((residual_norm_kernel<TPR, 2, VEC>), dim3(grid), dim3(threads), 0, s, A);
-    else hipLaunchKernelGGL((residual_norm_kernel<TPR, kNormChunks, VEC>), dim3(grid), dim3(threads), 0, s, A);
+    if (chunks <= 1) hipLaunchKernelGGL((residual_norm_kernel<TPR, 1, VEC>), grid, dim3(threads), 0, s, A);
+    else if (chunks <= 2) hipLaunchKernelGGL((residual_norm_kernel<TPR, 2, VEC>), grid, dim3(threads), 0, s, A);
+    else hipLaunchKernelGGL((residual_norm_kernel<TPR, kNormChunks, VEC>), grid, dim3(threads), 0, s, A);
 }
 
 template <bool VEC>

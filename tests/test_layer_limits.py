@@ -130,3 +130,101 @@ def test_queries_find_their_sequence_among_many(be):
     c = Cache(np.random.default_rng(2), served[:-1], 1, 32, 16)
     c.q_start, c.tokens, c.max_new = np.array(starts, np.int32), int(at[-1]), 3
     append_case(be, served[:-1], cache=c, kv_heads=1, head_dim=32)
+
+
+# ---- more workgroups than one dimension of a grid takes (2^32 threads) ----------------------------------------------
+
+@gpu
+def test_norm_of_more_rows_than_a_grid_dimension_takes(be):
+    rows = (1 << 26) + 5  # four rows a workgroup of 256 threads
+    rng = np.random.default_rng(3)
+    bits, h = raw(rng.standard_normal(rows, dtype=np.float32) * 2, "bf16")
+    d = Dev(be)
+    p = d.put(bits)
+    args = hip.ResidualNorm(rows=rows, hidden=1, residual=p, residual_stride=1, residual_format=FMT["bf16"], normed=p, normed_stride=1,
+                            normed_format=FMT["bf16"], norm_offset=0.0, eps=0.5)
+    n = be.malloc(2 * rows)
+    args.normed = n
+    assert be.dev_residual_norm(args), be.last_error()
+    be.synchronize()
+    want = h / np.sqrt(h * h + 0.5)
+    close(values(be.d2h(n, (rows,), np.int16), "bf16"), want, (16 * U + HALF["bf16"]) * np.abs(want) + TINY["bf16"])
+    be.free(p)
+    be.free(n)
+
+
+@gpu
+@pytest.mark.parametrize("kernel", ["one", "several"])
+def test_append_of_more_workgroups_than_a_grid_dimension_takes(be, kernel):
+    """The new tokens of the last sequence, or the last rows, through a launch of more than 2^24 workgroups of 256 threads."""
+    rng = np.random.default_rng(4)
+    d = Dev(be)
+    h, dim, n, sequences, rows = (1024, 256, 1, 1 << 16, 1) if kernel == "one" else (1, 32, 5, 1, 1 << 24)
+    c = Cache(rng, [(n, 9)], h, dim, 16, width_more=0)
+    cache, batch = c.upload(be)
+    table, kv_len = np.full((sequences, 1), -1, np.int32), np.full(sequences, 3, np.int32)
+    q_start = np.zeros(sequences + 1, np.int32)
+    table[-1], kv_len[-1], q_start[-2:] = c.table[0, 0], 9, (rows - n, rows)
+    batch.block_table, batch.kv_len, batch.q_start = d.put(table), d.put(kv_len), d.put(q_start)
+    batch.sequences, batch.tokens, batch.max_new_tokens = sequences, rows, n
+    x = rng.standard_normal((n, h, dim)).astype(np.float32)
+    bits, x = raw(x.reshape(n, -1), "bf16")
+    width = h * dim
+    p = be.malloc(2 * rows * width)
+    q_out = be.malloc(2 * rows * width)
+    be.h2d(p + 2 * (rows - n) * width, bits)
+    args = hip.KvAppend(format=FMT["bf16"], q_heads=h, q=p, q_stride=width, q_out=q_out, q_out_stride=width, k=p, k_stride=width, v=p, v_stride=width)
+    assert be.dev_kv_append(cache, batch, args), be.last_error()
+    be.synchronize()
+    assert (be.d2h(q_out + 2 * (rows - n) * width, bits.shape, np.int16) == bits).all()
+    after = c.download(be)
+    page = c.table[0, 0]
+    for name, scales in (("k", "ks"), ("v", "vs")):
+        codes = e4m3(after[name])[page]
+        got = (codes if name == "k" else codes.transpose(0, 2, 1))[:, 9 - n: 9] * after[scales][page].astype(np.float64)[:, None, None]
+        y = x.reshape(n, h, dim).transpose(1, 0, 2)
+        close(got, y, np.maximum(2.0 ** -4 * np.abs(y), after[scales][page].astype(np.float64)[:, None, None] * 2.0 ** -10), name)
+        others = [i for i in range(c.pages) if i != page]
+        assert (after[name][others] == getattr(c, name)[others]).all()
+    be.free(p)
+    be.free(q_out)
+
+
+@gpu
+def test_attention_of_more_workgroups_than_a_grid_dimension_takes(be):
+    rng = np.random.default_rng(5)
+    d = Dev(be)
+    h, dim, n, sequences = 1024, 32, 40, 8300  # a workgroup of 512 threads for each sequence and head at least
+    c = Cache(rng, [(n, n)], h, dim, 64, width_more=0)
+    cache, batch = c.upload(be)
+    table, kv_len = np.full((sequences, 1), -1, np.int32), np.full(sequences, 3, np.int32)
+    q_start = np.zeros(sequences + 1, np.int32)
+    table[-1], kv_len[-1], q_start[-1] = c.table[0, 0], n, n
+    batch.block_table, batch.kv_len, batch.q_start, batch.sequences = d.put(table), d.put(kv_len), d.put(q_start), sequences
+    bits, q = raw(rng.standard_normal((n, h * dim)), "f32")
+    out = d.put(np.zeros((n, h * dim), np.float32))
+    args = hip.Attention(q=d.put(bits), q_stride=h * dim, q_format=FMT["f32"], out=out, out_stride=h * dim, out_format=FMT["f32"], q_heads=h, causal=1,
+                         scale=dim ** -0.5)
+    ws = be.attention_workspace_bytes(cache, batch, args)
+    assert be.dev_attention(cache, batch, args, be.malloc(ws), ws), be.last_error()
+    be.synchronize()
+    q = q.reshape(n, h, dim)
+    want, size, xmax, qk = ref_attention(c, q, dim ** -0.5, True, 0, 0.0, None)
+    e = 2.0 ** -20 * dim ** -0.5 * qk + 32 * U * (60 + xmax) + 2.0 ** -21
+    close(be.d2h(out, (n, h * dim), np.float32).reshape(n, h, dim), want, 2 * e[..., None] * size + U * np.abs(want))
+
+
+@pytest.mark.parametrize("op,batch,cache,other,code",
+                         [("app", {"tokens": 1 << 24, "max_new_tokens": 9}, {"kv_heads": 512}, {"k_stride": 1 << 15, "v_stride": 1 << 15}, L.E_ARG),
+                          ("app", {"tokens": 1 << 24, "max_new_tokens": 9}, {"kv_heads": 1024}, {"k_stride": 1 << 16, "v_stride": 1 << 16}, L.UNSUPPORTED),
+                          ("app", {"sequences": 1 << 16, "max_new_tokens": 1}, {"kv_heads": 1024}, {"k_stride": 1 << 16, "v_stride": 1 << 16}, L.E_ARG),
+                          ("att", {"tokens": 1 << 24}, {"kv_heads": 512}, {"q_heads": 8192, "q_stride": 1 << 19, "out_stride": 1 << 19}, L.E_ARG),
+                          ("att", {"tokens": 1 << 24, "max_new_tokens": 1 << 24}, {"kv_heads": 1024},
+                           {"q_heads": 16384, "q_stride": 1 << 20, "out_stride": 1 << 20}, L.UNSUPPORTED),
+                          ("norm", {}, {}, {"rows": 1 << 31}, L.UNSUPPORTED), ("norm", {}, {}, {"rows": (1 << 31) - 1}, L.E_ARG)])
+def test_calls_of_more_workgroups_than_a_launch_takes_are_refused(op, batch, cache, other, code):
+    s = _sound()
+    for which, fields in (("batch", batch), ("cache", cache), (op, other)):
+        for field, value in fields.items():
+            setattr(s[which], field, value)
+    assert _call(op, s) == code
