@@ -324,7 +324,8 @@ void larql_hip_plan_destroy(larql_hip_ctx *ctx, larql_hip_plan *plan);
  * matvecs as one command buffer (DecodeBackend::decode_token, larql-compute/src/backend/decode.rs:219-); here the
  * plans' launches are recorded once into a HIP graph — a plan's launches run in order, a plan after the one before
  * it — and a run replays it on the context's stream without synchronising: the per-launch submission cost is paid
- * by the graph, not by the caller.  Creating the sequence runs the plans once.  The plans must outlive it. */
+ * by the graph, not by the caller.  Creating the sequence runs its matvec plans once; plans of the layer operators (below) are
+ * recorded only.  The plans must outlive it. */
 typedef struct larql_hip_sequence larql_hip_sequence;
 int  larql_hip_sequence_create(larql_hip_ctx *ctx, larql_hip_plan *const *plans, size_t n_plans, larql_hip_sequence **out);
 int  larql_hip_sequence_run(larql_hip_ctx *ctx, larql_hip_sequence *seq);

@@ -1588,12 +1588,16 @@ struct larql_hip_plan {
     int launch_count() const { return (int)launches.size() + layer.launches(); }
 };
 
-static hipError_t enqueue_plan(larql_hip_ctx *c, const larql_hip_plan *plan) {
+static hipError_t enqueue_matvecs(larql_hip_ctx *c, const larql_hip_plan *plan) {
     for (const PreparedLaunch &P : plan->launches) {
         const hipError_t e = gemv_launch(c->stream, P.kind, P.L, P.threads, P.grid, P.lds);
         if (e != hipSuccess) return e;
     }
-    return plan->layer.enqueue(c->stream);
+    return hipSuccess;
+}
+static hipError_t enqueue_plan(larql_hip_ctx *c, const larql_hip_plan *plan) {
+    const hipError_t e = enqueue_matvecs(c, plan);
+    return e != hipSuccess ? e : plan->layer.enqueue(c->stream);
 }
 
 int larql_hip_plan_create(larql_hip_ctx *c, const larql_hip_matvec_job *pj, size_t n_jobs, larql_hip_plan **out) {
@@ -1654,8 +1658,9 @@ int larql_hip_sequence_create(larql_hip_ctx *c, larql_hip_plan *const *plans, si
         if (!plans[i]) return LARQL_E_ARG;
     std::lock_guard<std::mutex> lk(c->mu);
     HIPCHECK(c, hipSetDevice(c->device));
-    // once eagerly: whatever a kernel's first launch sets up (its LDS limit) happens outside the recording
-    for (size_t i = 0; i < n_plans; i++) HIPCHECK(c, enqueue_plan(c, plans[i]));
+    // The matvecs once eagerly: whatever a kernel's first launch sets up (its LDS limit) happens outside the recording.  Not the layer operators,
+    // which set nothing up and change what a later run reads: a residual in place, the cache's scales.
+    for (size_t i = 0; i < n_plans; i++) HIPCHECK(c, enqueue_matvecs(c, plans[i]));
     HIPCHECK(c, wait_stream(c));
     larql_hip_sequence *seq = new larql_hip_sequence();
     hipError_t e = hipStreamBeginCapture(c->stream, hipStreamCaptureModeThreadLocal);

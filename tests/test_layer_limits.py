@@ -228,3 +228,35 @@ def test_calls_of_more_workgroups_than_a_launch_takes_are_refused(op, batch, cac
         for field, value in fields.items():
             setattr(s[which], field, value)
     assert _call(op, s) == code
+
+
+# ---- recording -------------------------------------------------------------------------------------------------------
+
+@gpu
+def test_recording_a_layers_step_changes_nothing_that_it_works_on(be):
+    """What lies in the buffers then is no step's: a residual in place would be added to, a page's scale would grow for good."""
+    seqs = [(1, 3), (1, 31), (2, 40), (1, 90), (1, 1)]
+    a, b = (Layer(be, np.random.default_rng(24), seqs, d=224) for _ in range(2))
+    for layer in (a, b):
+        layer.norm.residual_out, layer.norm.normed = layer.x, layer.o  # in place
+    x = be.d2h(a.qkv, (a.c.tokens, (a.hq + 2 * a.h) * a.d), np.float32)
+    be.h2d(a.qkv, np.full_like(x, np.nan))  # not written yet
+
+    def state(layer):
+        return layer.results() + [be.d2h(layer.x, (layer.c.tokens, layer.hidden), np.float32)]
+
+    before = state(a)
+    plans = a.plans()
+    seq = be.sequence_create(plans)
+    assert seq
+    for got, want in zip(state(a), before):
+        assert (got.view(np.uint8) == want.view(np.uint8)).all()
+    be.h2d(a.qkv, x)
+    for _ in range(3):
+        assert be.sequence_run(seq)
+        b.eager()
+        for got, want in zip(state(a), state(b)):
+            assert (got.view(np.uint8) == want.view(np.uint8)).all()
+    be.sequence_destroy(seq)
+    for p in plans:
+        be.plan_destroy(p)
