@@ -51,9 +51,10 @@ struct Plan {
     int fits;                     // how often pieces are made longer to meet the target
 };
 
-// Steps of keys that the window lets a tile see, at most (its tokens may straddle).
-__host__ __device__ __forceinline__ uint64_t window_steps(const AttentionArgs &A, uint32_t tile) {
-    return A.window ? ((uint64_t)A.window + A.group.of(tile) + 1) / kStep + 2 : ~(uint64_t)0;
+// Steps of keys that the window lets a tile of a sequence with n new tokens see, at most.  Causal: the window and the tile's tokens, which may
+// straddle; else all keys behind the first one's window, so up to n more than the window.
+__host__ __device__ __forceinline__ uint64_t window_steps(const AttentionArgs &A, uint32_t tile, uint32_t n) {
+    return A.window ? ((uint64_t)A.window + (A.causal ? A.group.of(tile) : n) + 1) / kStep + 2 : ~(uint64_t)0;
 }
 
 // A sequence's share of the work: its query rows in tiles, and at most how many steps of keys one of them sees.
@@ -72,7 +73,7 @@ __device__ __forceinline__ Share share_of(const AttentionArgs &A, const Plan &P,
     const uint32_t rows = t.n * A.group.d;
     h.tiles = rows < P.rows_min || rows > P.rows_max ? 0u : (rows + P.tile - 1) / P.tile;
     h.steps = h.tiles ? ((uint32_t)h.len + kStep - 1) / kStep : 0;
-    h.steps = min((uint64_t)h.steps, window_steps(A, P.tile));
+    h.steps = min((uint64_t)h.steps, window_steps(A, P.tile, t.n));
     return h;
 }
 
@@ -146,8 +147,9 @@ struct Plans {
 };
 static Plans plans_of(const AttentionArgs &A) {
     const uint64_t group = A.group.d, most = A.kv.max_new * group;
-    const auto steps_of = [&](uint32_t tile) {
-        return std::min((((uint64_t)A.kv.table_width << A.kv.page_shift) + kStep - 1) / kStep, window_steps(A, tile));
+    const auto steps_of = [&](uint32_t tile, uint64_t rows) {  // of a sequence with at most so many rows
+        const uint32_t n = (uint32_t)std::min<uint64_t>(A.kv.max_new, rows / group);
+        return std::min((((uint64_t)A.kv.table_width << A.kv.page_shift) + kStep - 1) / kStep, window_steps(A, tile, n));
     };
     const uint32_t cus = 256;
     Plans p;
@@ -157,12 +159,12 @@ static Plans plans_of(const AttentionArgs &A) {
     // Rows so short that the launch of joining costs what it saves stay whole (1000 keys, us whole / split: 32/8 heads of 128 12.8 / 12.6, 16
     // sequences of them 14.5 / 16.9, 64/8 of 64 9.6 / 10.9; 2000 of the first 17.6 / 12.8; 8/4 heads of 256, f32: 500 keys 13.5 / 15.1, 1000 19.5 /
     // 15.2).
-    p.rows.split = steps_of(kRowsTile) > (A.kv.head_dim > 128 ? 8u : 16u);
+    p.rows.split = steps_of(kRowsTile, kFewRows) > (A.kv.head_dim > 128 ? 8u : 16u);
     // Many rows: as many as are resident, unless the tiles by themselves (of which a sequence's last is half full, say) are as many: splitting
     // then is a launch more for nothing (2048 tokens of 32/8 heads of 128: 76 us whole, 88 with it; 16 sequences of 32 tokens, 256 channels,
     // f32: 239 and 165).
     p.tiles = {kTilesTile, kFewRows + 1, 0xFFFFFFFFu, std::max((A.kv.head_dim > 128 ? 1 : 2) * cus / A.kv.kv_heads, 1u), 8, 1, 6};
-    p.tiles.split = steps_of(kTilesTile) > p.tiles.min_steps && A.kv.tokens * group / p.tiles.tile + A.kv.sequences / 2 < p.tiles.target;
+    p.tiles.split = steps_of(kTilesTile, most) > p.tiles.min_steps && A.kv.tokens * group / p.tiles.tile + A.kv.sequences / 2 < p.tiles.target;
     p.use_tiles = most > kFewRows;
     p.use_rows = !p.use_tiles || A.kv.sequences > 1;
     if (!p.use_rows) p.tiles.rows_min = 1;  // one sequence: one kernel, whatever its number of new tokens turns out to be

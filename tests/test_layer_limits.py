@@ -260,3 +260,29 @@ def test_recording_a_layers_step_changes_nothing_that_it_works_on(be):
     be.sequence_destroy(seq)
     for p in plans:
         be.plan_destroy(p)
+
+
+# ---- attention: long rows in pieces ----------------------------------------------------------------------------------
+
+def _workspace(**fields):
+    s = _sound()
+    s["batch"].table_width = 4096
+    for field, value in fields.items():
+        setattr(s["batch"] if field in ("tokens", "max_new_tokens") else s["att"], field, value)
+    return L.lib.larql_hip_attention_workspace_bytes(ctypes.byref(s["cache"]), ctypes.byref(s["batch"]), ctypes.byref(s["att"]))
+
+
+def test_the_keys_that_a_window_without_causal_lets_a_row_see():
+    """Those behind its start up to the sequence's end: with many new tokens far more than the window, so the row is split."""
+    for tokens in (3, 300):
+        sizes = {"tokens": tokens, "max_new_tokens": tokens, "window": 64}
+        assert _workspace(**sizes) == _workspace(causal=0, **sizes) < _workspace(tokens=tokens, max_new_tokens=tokens)
+    sizes = {"tokens": 5000, "max_new_tokens": 5000, "q_heads": 2}
+    assert _workspace(window=64, **sizes) < _workspace(window=64, causal=0, **sizes) == _workspace(**sizes)
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 40, 1500])
+@pytest.mark.parametrize("window", [1, 100, 5000])
+def test_attention_in_a_window_that_is_open_to_later_keys(be, new, window):
+    attention_case(be, [(new, 6000), (1, 2000), (min(new, 40), 40)], kv_heads=1, group=2, head_dim=64, page=64, causal=False, window=window, spoil_tail=True)
