@@ -120,10 +120,13 @@ template <uint32_t TPR, bool VEC>
 static void launch_rows(hipStream_t s, const NormArgs &A) {
     const uint32_t threads = TPR < 256 ? (TPR == 64 ? 256 : TPR) : TPR, rows = threads / TPR;
     const dim3 grid = grid_of((A.rows + rows - 1) / rows);
-    const uint32_t chunks = (A.hidden + TPR * 8 - 1) / (TPR * 8);
-    if (chunks <= 1) hipLaunchKernelGGL((residual_norm_kernel<TPR, 1, VEC>), grid, dim3(threads), 0, s, A);
-    else if (chunks <= 2) hipLaunchKernelGGL((residual_norm_kernel<TPR, 2, VEC>), grid, dim3(threads), 0, s, A);
-    else hipLaunchKernelGGL((residual_norm_kernel<TPR, kNormChunks, VEC>), grid, dim3(threads), 0, s, A);
+    const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, A); };
+    if constexpr (TPR == 1024) {  // the most threads: longer rows are more groups a thread
+        const uint32_t chunks = (A.hidden + TPR * 8 - 1) / (TPR * 8);
+        if (chunks > 2) return launch(residual_norm_kernel<TPR, kNormChunks, VEC>);
+        if (chunks > 1) return launch(residual_norm_kernel<TPR, 2, VEC>);
+    }
+    launch(residual_norm_kernel<TPR, 1, VEC>);
 }
 
 template <bool VEC>
