@@ -421,14 +421,14 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendArgs 
 
 template <uint32_t LPH>
 static void launch_lanes(hipStream_t s, const KvAppendArgs &A, uint32_t page_blocks, dim3 grid) {
-    const uint32_t passes = (1u << A.kv.page_shift) * LPH / kAppendThreads;
-#define LARQL_APPEND(NP) hipLaunchKernelGGL((kv_append_kernel<LPH, NP>), grid, dim3(kAppendThreads), 0, s, A, page_blocks)
-    if (passes <= 1) LARQL_APPEND(1);
-    else if (passes <= 2) LARQL_APPEND(2);
-    else if (passes <= 4) LARQL_APPEND(4);
-    else if (passes <= 8) LARQL_APPEND(8);
-    else LARQL_APPEND(16);
-#undef LARQL_APPEND
+    const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kAppendThreads), 0, s, A, page_blocks); };
+    constexpr auto passes = [](uint32_t page_tokens) { return (int)((LPH * page_tokens + kAppendThreads - 1) / kAppendThreads); };
+    switch (A.kv.page_shift) {
+    case 4: return launch(kv_append_kernel<LPH, passes(16)>);
+    case 5: return launch(kv_append_kernel<LPH, passes(32)>);
+    case 6: return launch(kv_append_kernel<LPH, passes(64)>);
+    default: return launch(kv_append_kernel<LPH, passes(128)>);
+    }
 }
 
 // Lanes of a head; one new token a sequence: workgroups of a sequence.
