@@ -34,9 +34,9 @@ constexpr uint32_t kTilesTile = 128;    // ... for many
 constexpr uint32_t kFewRows = 32;
 constexpr float kLog2E = 1.44269504088896341f;
 // Weights are held as 2^(t + e - M + bias) with t + e - M <= 3; M is whole and only moves where a score leaves that range, so it brings no
-// rounding.  f32 results: the bias is small, for the exponent is rounded as a number of its size; an f16 pair keeps 22 bits down to 2^-10 of the
-// largest and 2^-32 of it beyond (131072 equal weights 2^-17 of one that weighs as much as they all: 2^-15 each, at random).  16-bit results: as
-// large as fits; one f16 keeps 11 bits down to 2^-26 of the largest, 2^-37 of it beyond, a pair the same floor.
+// rounding.  f32 results: the bias is small, for the exponent is rounded as a number of its size; an f16 pair keeps 22 bits down to 2^-9 of the
+// largest, which is 2^6 at least, and is off by 2^-25 beyond: 2^-31 of it (131072 equal weights 2^-17 of one that weighs as much as they all: 2^-14
+// each, at random).  16-bit results: as large as fits; one f16 keeps 11 bits down to 2^-25 of the largest, a pair 22 down to 2^-14, 2^-36 beyond.
 constexpr float kLowBias = 7.f, kHighBias = 12.f, kSlack = 3.f;
 __device__ __forceinline__ float weight_bias(bool f32_result) { return f32_result ? kLowBias : kHighBias; }
 constexpr float kNoMax = -1e30f;

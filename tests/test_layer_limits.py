@@ -286,3 +286,28 @@ def test_the_keys_that_a_window_without_causal_lets_a_row_see():
 @pytest.mark.parametrize("window", [1, 100, 5000])
 def test_attention_in_a_window_that_is_open_to_later_keys(be, new, window):
     attention_case(be, [(new, 6000), (1, 2000), (min(new, 40), 40)], kv_heads=1, group=2, head_dim=64, page=64, causal=False, window=window, spoil_tail=True)
+
+
+@gpu
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("t,out", [("f32", "f32"), ("f16", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
+def test_small_weights_are_held_to_their_floor(be, many, t, out):
+    """A row of two keys with values in channels of their own: what is lost of a small weight shows where nothing else is added."""
+    rng = np.random.default_rng(8)
+    seqs = [(200, 200)] if many else [(1, 2 + 5 * i) for i in range(60)]
+    c = Cache(rng, seqs, 1, 64, 16)
+    for a in (c.k, c.v):
+        a[:] = 0
+    c.k[:, :, 0::2, 0], c.k[:, :, 1::2, 0] = 0x38, 0xB8              # keys 1, -1
+    c.v[:, :, 0::2, 0::2], c.v[:, :, 1::2, 1::2] = 0x38, 0x38        # the one's value in even channels, the other's in odd ones
+    c.ks[:], c.vs[:] = 1.0, 1.0
+    q = np.zeros((c.tokens, 4, 64))
+    q[..., 0] = rng.uniform(-13, 13, q.shape[:2])                    # weights down to 2^-37 of each other
+    q = raw(q, t)[1]
+    want, _, _, _ = ref_attention(c, q, 1.0, True, 2, 0.0, None)
+    got = attention(be, c, q, t, out, 1.0, window=2)
+    # scores of at most 13 with a few roundings of them, exponents of at most 64: 128 u of a weight; its floor, the larger one's being 1 at most
+    floor = 2.0 ** -31 if out == "f32" else 2.0 ** -36
+    weight = 2.0 ** -10 if many and out != "f32" else 128 * U
+    close(got, want, weight * np.abs(want) + floor + HALF[out] * np.abs(want))
+    assert (want[..., :2].min(-1) < floor / 2).any()
