@@ -30,7 +30,7 @@ constexpr uint32_t kAttnWaves = kAttnThreads / 64;
 constexpr uint32_t kRowsTile = 16;      // query rows of a workgroup of the kernel for few rows
 constexpr uint32_t kTilesTile = 128;    // ... for many
 // A sequence with at most this many rows for each key/value head goes through the former.  16 sequences of 4000 keys, us through it / through the
-// latter: 24 rows 51 / 53 (128 channels, bf16), 86 / 98 (256, f32); 32 rows 51 / 54, 87 / 101; 56 rows 93 / 62, 156 / 111.
+// latter: 24 rows 51 / 54 (128 channels, bf16), 85 / 97 (256, f32); 32 rows 51 / 53, 86 / 99; 56 rows 94 / 62, 154 / 106.
 constexpr uint32_t kFewRows = 32;
 constexpr float kLog2E = 1.44269504088896341f;
 // Weights are held as 2^(t + e - M + bias) with t + e - M <= 3; M is whole and only moves where a score leaves that range, so it brings no
@@ -79,7 +79,9 @@ __device__ __forceinline__ Share share_of(const AttentionArgs &A, const Plan &P,
 
 // What the wavefront that serves item `item` of a head works on; false beyond the last.  Every wavefront finds it from the lengths:
 // tiles of sequences in order, the keys that a tile sees in equal pieces, as many as P.target asks for.  Pieces of split tiles
-// have places for their partial results, `slot` on; `split_tiles`: items count split tiles instead.
+// have places for their partial results, `slot` on; `split_tiles`: items count split tiles instead.  Lengths of more than 64 sequences are read
+// once more for each sum and for the search: one token each over 500 keys, 1024 sequences of 8/2 heads of 128 take 65 us (4.1 TB/s), 4096 of 4/1 heads
+// 231 (2.3).
 struct Item {
     uint32_t s, tile, piece, pieces, slot;
     // the steps of this piece, of those from `first` to before `end` that its tile sees
@@ -154,11 +156,11 @@ static Plans plans_of(const AttentionArgs &A) {
     const uint32_t cus = 256;
     Plans p;
     // Pieces of few rows: as many as workgroups are resident, 2 a compute unit above 128 channels (131072 keys of 256, us with 1, 2, 3, 4 of
-    // them: 148, 103, 125, 110, joining included), 3 below (64 sequences, 64 channels: 44, 37, 33, 37); a wavefront's step each at least.
+    // them: 148, 103, 125, 110, joining included), 3 below (64 sequences, 64 channels, with 2, 3, 4: 38, 34, 37); a wavefront's step each at least.
     p.rows = {kRowsTile, 1, kFewRows, std::max((A.kv.head_dim > 128 ? 2 : 3) * cus / A.kv.kv_heads, 1u), kAttnWaves, 1, 0};
-    // Rows so short that the launch of joining costs what it saves stay whole (1000 keys, us whole / split: 32/8 heads of 128 12.8 / 12.6, 16
-    // sequences of them 14.5 / 16.9, 64/8 of 64 9.6 / 10.9; 2000 of the first 17.6 / 12.8; 8/4 heads of 256, f32: 500 keys 13.5 / 15.1, 1000 19.5 /
-    // 15.2).
+    // Rows so short that the launch of joining costs what it saves stay whole (1000 keys, us whole / split: 32/8 heads of 128 13.4 / 12.8, 16
+    // sequences of them 14.6 / 17.2, 64/8 of 64 10.0 / 10.8; 2000 of the first 20.7 / 13.0; 8/4 heads of 256, f32: 500 keys 13.0 / 14.7, 1000 19.1 /
+    // 15.0).
     p.rows.split = steps_of(kRowsTile, kFewRows) > (A.kv.head_dim > 128 ? 8u : 16u);
     // Many rows: as many as are resident, unless the tiles by themselves (of which a sequence's last is half full, say) are as many: splitting
     // then is a launch more for nothing (2048 tokens of 32/8 heads of 128: 76 us whole, 88 with it; 16 sequences of 32 tokens, 256 channels,
@@ -284,8 +286,10 @@ __device__ __forceinline__ void query_f16(const Eight &q, float mul, f16x8_t &h,
 // 16 query rows a workgroup, as the columns of v_mfma_f32_16x16x32_f16; its wavefronts take steps of 64 keys in turn and add up at the
 // end.  A wavefront reads its step's codes straight into the registers that the matrix instructions' operands are converted
 // from, 64 x head_dim bytes of K and then of V through ONE set of registers: as a part of the keys is multiplied its registers take a part
-// of the step's values, and as that is multiplied a part of the next step's keys, so about 64 x head_dim bytes are always in flight and
-// two wavefronts fit a SIMD above 128 channels and three below.  The queries' operands are read from LDS.
+// of the step's values, and as that is multiplied a part of the next step's keys, so two wavefronts fit a SIMD above 128 channels and three
+// below.  The loads do not stay in flight throughout: the two page numbers read in a step are compared where they are read (kv_page), and
+// each waits for every load before it, so the step's values have arrived before the next keys are asked for; other wavefronts fill that gap.
+// The queries' operands are read from LDS.
 // Queries and weights are f16 pairs for every result: memory, not the matrix instructions, is waited for (one token of 131072 keys of 16/8 heads of
 // 128 into bf16, 52 us in pairs, 58 as one f16; 64 sequences of 64/8 heads of 64: 34.6, 33.3, of 500 keys each: 12, 11).
 template <int NK, bool CAP>
@@ -359,8 +363,8 @@ __global__ void __launch_bounds__(kAttnThreads, NK > 4 ? 2 : 3) attention_rows_k
     };
     uint32_t page_k = page_of(step, gk), page_v = page_of(step, g);
     __builtin_amdgcn_sched_barrier(0);
-    // The queries' elements are on their way before the keys'.  Channels of the lane's operand k: two operands' lie in one 16-byte piece of
-    // a key's row.
+    // The queries' elements, before the keys': each piece is converted by its type where it is loaded, so one is waited for before the next leaves.
+    // Channels of the lane's operand k: two operands' lie in one 16-byte piece of a key's row.
     Eight q[NK];
     const uint32_t q_row = live ? row : last_row;
 #pragma unroll
@@ -642,7 +646,8 @@ __global__ void __launch_bounds__(Shape<tiles_narrow(NK, PAIRS)>::kWaves * 64, 2
     u32x4_t kc[kPieces], vc[kPieces];
     float ks = 0.f, vs = 0.f;
     int e_top = -1000;  // the largest logarithm of a value scale met
-    // The pages of a step, that of group lane % 4 in a lane: read one step before its codes.
+    // The pages of a step, that of group lane % 4 in a lane: read one step before its codes.  (A page number is compared where it is read: behind a
+    // step's staging loads that waits for them too, once a turn and before the turn's matrix instructions.)
     const auto pages_of = [&](uint32_t st) -> uint32_t {
         const uint32_t key = st * kKeys + lane % G * 16;
         return st >= end || (int32_t)key >= sh.len ? ~0u : kv_page(kv, table, key);
@@ -990,7 +995,8 @@ static void launch_tiles(hipStream_t s, const AttentionArgs &A, const Plan &P, c
 }
 // One f16 holds a 16-bit query, but 11 of an f32 query's 24 bits, and what a score loses grows with the score: f32 queries enter as f16 pairs
 // whatever the result's type (a causal prompt of 4096 f32 queries, 32/8 heads of 128, into bf16: 242 us for 203; 8/4 of 256 into f16: 195 for 191, and
-// 2.6e-4 from 64 bits for 4.6e-4).
+// 2.6e-4 from 64 bits for 4.6e-4).  Weights of many rows into 16 bits are one f16: pairs, a second product more, would take 782 us for 632 (a causal
+// prompt of 8192, 32/8 heads of 128, bf16: 1.65e-3 from 64 bits for 1.66e-3) and 231 for 187 (4096, f16: 2.1e-4 for 2.5e-4).
 template <int NK>
 static void launch_dim(hipStream_t s, const AttentionArgs &A, const Plan &P, const Partials &part, bool tiles) {
     const uint32_t items = (uint32_t)Plans::items(A, P);
