@@ -577,8 +577,8 @@ typedef struct {
  * ones of the sequence.  block_table[s] lists its pages; an entry outside [0, num_pages) is a hole: nothing is written
  * there, and its tokens are masked.  A sequence whose rows do not fit (q_start falling, beyond `tokens`, or more than
  * max_new_tokens of them) is left out, its rows untouched, and the others are served.  No row belongs to two sequences (else
- * some of their work is left undone).  Up to 2^16 sequences, 2^24 new tokens and tables of 2^30 tokens; and less than 2^31 workgroups a
- * launch: pages of the new tokens times 2 kv_heads, or 128 query rows times kv_heads, about (more: LARQL_UNSUPPORTED). */
+ * some of their work is left undone).  Up to 2^16 sequences, 2^24 new tokens and tables of 2^30 tokens, and what one launch takes:
+ * pages with new tokens times 2 kv_heads, or tiles of 128 query rows times kv_heads, about 2^31 (more: LARQL_UNSUPPORTED). */
 typedef struct {
     const int32_t *kv_len;         /* [sequences] */
     const int32_t *block_table;    /* [sequences, table_width] */
@@ -620,9 +620,10 @@ int larql_hip_dev_kv_append(larql_hip_ctx *ctx, const larql_hip_kv_cache *cache,
  * x = scale * q.k, softcap * tanh(x / softcap) where softcap is not 0 (then at least 2^-20); a query at position p sees keys <= p (`causal`) and
  * > p - window (window > 0); `sinks` [q_heads] (or NULL) adds exp(sink) to the sum of the weights.  A query that sees
  * nothing gives zeros.  Sums are f32.  Queries enter the matrix instructions whole (16-bit types) or as f16 pairs (f32: about
- * 22 bits).  Weights are f16 pairs (about 22 bits), but one f16 (11 bits) for 16-bit results of sequences with more than 32 new tokens
- * times query heads of a key/value head, and, in a batch of one sequence, wherever max_new_tokens allows so many.  Below that a weight times its
- * block's value scale is off by up to 2^-31 of the row's largest such product where `out` is f32, 2^-36 otherwise.  Results may differ in their last bits with the batch around a sequence: long
+ * 22 bits), elements to 2^-39 of the row's largest at the least.  Weights are f16 pairs (about 22 bits), but one f16 (11 bits) for 16-bit
+ * results of sequences with more than 32 new tokens times query heads of a key/value head, and, in a batch of one sequence,
+ * wherever max_new_tokens allows so many.  Below that a weight times its block's value scale is off by up to 2^-31 of the row's
+ * largest such product where `out` is f32, 2^-36 otherwise.  Results may differ in their last bits with the batch around a sequence: long
  * rows are split by the work that there is.  workspace: larql_hip_attention_workspace_bytes(...) (0: a call that is refused or
  * has nothing to do) of device memory, 16-byte aligned, not shared with a call that may run at the same time; it depends on
  * the batch's sizes, not on what the device memory holds. */
