@@ -7,7 +7,7 @@ import pytest
 
 import larql_amd as hip
 from larql_amd import _lib as L
-from test_layer_ops import (FMT, HALF, ITEM, TINY, U, Cache, Dev, Layer, _call, _sound, append_case, attention_case, close, e4m3, exponent, raw,
+from test_layer_ops import (FMT, HALF, TINY, U, Cache, Dev, Layer, _call, _sound, append_case, attention_case, close, e4m3, raw,
                             ref_attention, values)
 
 gpu = pytest.mark.gpu
